@@ -148,8 +148,7 @@ def prepare(case, seed):
         # channels of keys differ in size
         channel = normal(case["kv"], case["d"]).abs() + 0.2
         s.k, s.v = (normal(*shape) * channel).to(TYPES[case["type"]]), normal(*shape).to(TYPES[case["type"]])
-        first = torch.from_numpy(rng.integers(0, case["cap"] - case["rows"] + 1, size=case["slots"])).cuda()
-        s.positions = first[:, None] + torch.arange(case["rows"], device="cuda")
+        s.starts = torch.from_numpy(rng.integers(0, case["cap"] - case["rows"] + 1, size=case["slots"])).cuda()
         whole = (case["slots"], case["kv"], case["cap"])
         s.k_codes, s.v_codes = (torch.zeros(*whole, case["d"], device="cuda", dtype=torch.int8).view(CODES[case["cache"]]) for _ in "kv")
         s.k_scale, s.v_scale = (torch.zeros(*whole, device="cuda") for _ in "kv")
@@ -243,8 +242,8 @@ def run(state):
         where = state.k_codes, state.v_codes, state.k_scale, state.v_scale
         if own:
             from dyninfer_b200 import ops
-            ops.kv_write(state.k, state.v, state.positions, *where)
-            return ops.kv_read(state.positions, *where, dtype=TYPES[case["type"]])
+            ops.kv_write(state.k, state.v, state.starts, *where)
+            return ops.kv_read(state.starts, case["rows"], *where, dtype=TYPES[case["type"]])
         return _cache(state, case, where)
     if case["kind"] == "attend":
         if own:
@@ -274,7 +273,7 @@ def _cache(state, case, where):
     k_codes, v_codes, k_scale, v_scale = where
     slot = torch.arange(case["slots"], device="cuda")[:, None, None]
     head = torch.arange(case["kv"], device="cuda")
-    at = slot, head, state.positions[..., None]
+    at = slot, head, (state.starts[:, None] + torch.arange(case["rows"], device="cuda"))[..., None]
     for x, codes, scales in ((state.k, k_codes, k_scale), (state.v, v_codes, v_scale)):
         new, scale = _quantised(x, case["cache"])
         codes.view(torch.int8)[at] = new.view(torch.int8)
@@ -353,7 +352,7 @@ def work(case):
     if case["kind"] == "cache":
         n = 2 * case["slots"] * case["rows"] * case["kv"]      # rows of keys and values
         # values in, codes and scales out, codes and scales in, values out
-        return {"bytes": n * (2 * case["d"] * size + 2 * (case["d"] + 4)) + 16 * case["slots"] * case["rows"], "flops": 4 * n * case["d"]}
+        return {"bytes": n * (2 * case["d"] * size + 2 * (case["d"] + 4)) + 16 * case["slots"], "flops": 4 * n * case["d"]}
     if case["kind"] == "attend":
         keys = case["slots"] * (case["len"] * 7 / 8 + case["rows"])
         row = case["d"] * SIZE[case["cache"]] + (4 if case["cache"] in CODES else 0)
