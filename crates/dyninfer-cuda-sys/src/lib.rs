@@ -26,6 +26,10 @@ pub const DYNINFER_ENC_Q4_K: i32 = 8;
 pub const DYNINFER_ENC_Q5_K: i32 = 9;
 pub const DYNINFER_ENC_IQ4_XS: i32 = 10;
 
+/// Cache types of one byte per element.
+pub const DYNINFER_KV_Q8: i32 = 32;
+pub const DYNINFER_KV_E4M3: i32 = 33;
+
 /// Opaque session: one KV cache, one parameter arena, one stream.
 #[repr(C)]
 pub struct dyninfer_cuda_session_t {
@@ -150,6 +154,108 @@ unsafe extern "C" {
         v_dev: *const f32,
         n: i64,
         out_index_dev: *mut i64,
+        stream: *mut c_void,
+    ) -> c_int;
+
+    // ---- speculative decoding (strides are host arrays that count elements)
+    pub fn dyninfer_cuda_rotary(
+        x_dev: *const c_void,
+        type: c_int,
+        x_strides: *const i64,
+        positions_dev: *const i64,
+        frequencies: *const f64,
+        rotary_dim: i64,
+        interleaved: c_int,
+        magnitude: f64,
+        batch: i64,
+        rows: i64,
+        heads: i64,
+        d: i64,
+        y_dev: *mut c_void,
+        y_strides: *const i64,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn dyninfer_cuda_kv_write(
+        k_dev: *const c_void,
+        v_dev: *const c_void,
+        type: c_int,
+        x_strides: *const i64,
+        k_cache_dev: *mut c_void,
+        v_cache_dev: *mut c_void,
+        kv_type: c_int,
+        cache_strides: *const i64,
+        k_scale_dev: *mut f32,
+        v_scale_dev: *mut f32,
+        scale_strides: *const i64,
+        starts_dev: *const i64,
+        counts_dev: *const i64,
+        batch: i64,
+        rows: i64,
+        kv_heads: i64,
+        d: i64,
+        kv_cap: i64,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn dyninfer_cuda_kv_read(
+        k_dev: *mut c_void,
+        v_dev: *mut c_void,
+        type: c_int,
+        x_strides: *const i64,
+        k_cache_dev: *const c_void,
+        v_cache_dev: *const c_void,
+        kv_type: c_int,
+        cache_strides: *const i64,
+        k_scale_dev: *const f32,
+        v_scale_dev: *const f32,
+        scale_strides: *const i64,
+        starts_dev: *const i64,
+        batch: i64,
+        rows: i64,
+        kv_heads: i64,
+        d: i64,
+        kv_cap: i64,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn dyninfer_cuda_tree_attention(
+        q_dev: *const c_void,
+        q_type: c_int,
+        q_strides: *const i64,
+        k_cache_dev: *const c_void,
+        v_cache_dev: *const c_void,
+        kv_type: c_int,
+        cache_strides: *const i64,
+        k_scale_dev: *const f32,
+        v_scale_dev: *const f32,
+        scale_strides: *const i64,
+        lengths_dev: *const i64,
+        mask_dev: *const u8,
+        mask_strides: *const i64,
+        batch: i64,
+        rows: i64,
+        heads: i64,
+        kv_heads: i64,
+        d: i64,
+        kv_cap: i64,
+        scale: f32,
+        ctx_dev: *mut c_void,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn dyninfer_cuda_verify_draft(
+        tokens_dev: *const i64,
+        parents_dev: *const i64,
+        parents_stride: i64,
+        target_dev: *const c_void,
+        target_strides: *const i64,
+        draft_dev: *const c_void,
+        draft_strides: *const i64,
+        type: c_int,
+        uniforms_dev: *const f32,
+        batch: i64,
+        nodes: i64,
+        vocab: i64,
+        accepted_dev: *mut i64,
+        path_dev: *mut i64,
+        next_dev: *mut i64,
         stream: *mut c_void,
     ) -> c_int;
 

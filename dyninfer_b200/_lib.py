@@ -14,6 +14,7 @@ LIB_PATH = os.environ.get("DYNINFER_CUDA_LIB") or os.path.join(HERE, "libdyninfe
 
 ENC = {"plain.f32": 0, "plain.f16": 1, "plain.bf16": 2, "gguf.q4_0": 3, "gguf.q4_1": 4,
        "gguf.q8_0": 5, "gguf.q6_k": 6, "mlx.affine.u4": 7, "gguf.q4_k": 8, "gguf.q5_k": 9, "gguf.iq4_xs": 10}
+KV = {"q8": 32, "e4m3": 33}     # 8-bit cache types
 ENC_NAME = {v: k for k, v in ENC.items()}
 
 
@@ -44,6 +45,7 @@ class AllocatorStatistics(C.Structure):
 
 _P = C.c_void_p
 _I64 = C.c_int64
+_S = C.POINTER(C.c_int64)   # strides, in host memory
 PROTOTYPES = {
     "dyninfer_cuda_abi_version": (C.c_int, []),
     "dyninfer_cuda_last_error": (C.c_char_p, []),
@@ -61,6 +63,16 @@ PROTOTYPES = {
     "dyninfer_cuda_argmax": (C.c_int, [_P, _I64, _P, _P, _P]),
     "dyninfer_cuda_argmax_static_max_n": (_I64, []),
     "dyninfer_cuda_argmax_static": (C.c_int, [_P, _I64, _P, _P]),
+    "dyninfer_cuda_rotary": (C.c_int, [_P, C.c_int, _S, _P, _P, _I64, C.c_int, C.c_double, _I64, _I64, _I64, _I64,
+                                       _P, _S, _P]),
+    "dyninfer_cuda_kv_write": (C.c_int, [_P, _P, C.c_int, _S, _P, _P, C.c_int, _S, _P, _P, _S, _P, _P,
+                                         _I64, _I64, _I64, _I64, _I64, _P]),
+    "dyninfer_cuda_kv_read": (C.c_int, [_P, _P, C.c_int, _S, _P, _P, C.c_int, _S, _P, _P, _S, _P,
+                                        _I64, _I64, _I64, _I64, _I64, _P]),
+    "dyninfer_cuda_tree_attention": (C.c_int, [_P, C.c_int, _S, _P, _P, C.c_int, _S, _P, _P, _S, _P, _P, _S,
+                                               _I64, _I64, _I64, _I64, _I64, _I64, C.c_float, _P, _P]),
+    "dyninfer_cuda_verify_draft": (C.c_int, [_P, _P, _I64, _P, _S, _P, _S, C.c_int, _P, _I64, _I64, _I64,
+                                             _P, _P, _P, _P]),
     "dyninfer_cuda_session_create_with_file_params": (
         C.c_int, [C.c_char_p, C.c_char_p, C.POINTER(ParameterFile), C.c_size_t,
                   C.POINTER(FileParam), C.c_size_t, C.POINTER(_P)]),

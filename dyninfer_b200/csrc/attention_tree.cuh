@@ -1,0 +1,789 @@
+// Attention of a tree of drafted tokens over a cache (one token is the plain decode step), on tensor cores.
+//
+// Row t of sequence b (t < T) sees the cache's keys 0 .. len_b - 1 and, of the tree's own keys at len_b + j, those with
+// mask[b][t][j]; out = softmax(scale q K^T) V, zeros where a row sees nothing. Caches hold bf16, f16, or 8-bit codes with one
+// f32 scale per (head, position).
+//
+// The T * G rows that share a kv head (G query heads) are one block of rows, so that a key or value is fetched once for all of
+// them. Work on a (sequence, kv head) is split over the keys: over the key groups of a block and over the blocks of a cluster,
+// each with a running (maximum, sum, output) of its own; the states meet in a fixed order, in shared memory.
+//   S = Q K^T  mma.sync m16n8k16. The order of the head's dimensions inside the product is free, so 8-bit keys are read 16
+//              bytes per lane as they lie and become exact f16 numbers in a register; the key's scale multiplies the score.
+//   O += P V   the accumulators of S are the A operand of P. 8-bit values are read 16 bytes of one key per lane, and two keys'
+//              bytes are interleaved on the way to f16; the value's scale goes into P. 2-byte values come by ldmatrix.trans.
+// Precision. Operands are f16 (bf16 for bf16 caches); what does not fit goes as two or three terms (an f32 query: 22 or 24
+// bits). A row of Q enters times a power of two that brings its largest element to 2^8 .. 2^9 (f16 has five bits of
+// exponent), P as p 2^14 scaled by the tile's largest value scale. An mma truncates where it adds to its accumulator, always
+// toward zero, so a tile's P V starts from zero and joins the running output by a rounded fma.
+#pragma once
+
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+#include "kv_codes.cuh"
+#include "ring.cuh"
+
+namespace dyn {
+
+enum { TREE_BF16 = 0, TREE_F16 = 1, TREE_Q8 = 2, TREE_E4M3 = 3 };
+
+struct TreeArgs {
+  const void* q;            // [batch][rows][heads][d]
+  void* out;                // the same, dense
+  const uint8_t *k, *v;     // [batch][kv head][cap][d]
+  const float *ks, *vs;     // [batch][kv head][cap]; NULL for 2-byte caches
+  const int64_t* lengths;   // [batch] keys in front of the tree; below zero: the sequence is passed over
+  const uint8_t* mask;      // [batch][rows][rows]; NULL: each row sees the tree's keys up to its own
+  int64_t qs[3];            // elements between batch entries, rows, heads
+  int64_t kst[3], vst[3];   // bytes between batch entries, heads, keys
+  int64_t kss[2], vss[2];   // floats between batch entries, heads
+  int64_t ms[2];            // bytes between batch entries, rows
+  int64_t batch, cap;
+  int rows, heads, kv_heads, group, d, splits, row_blocks;
+  float scale;
+};
+
+int tree_attention_bf16(const TreeArgs& a, int q_type, cudaStream_t s);
+int tree_attention_f16(const TreeArgs& a, int q_type, cudaStream_t s);
+int tree_attention_q8(const TreeArgs& a, int q_type, cudaStream_t s);
+int tree_attention_e4m3(const TreeArgs& a, int q_type, cudaStream_t s);
+
+namespace tree {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
+  const int n = live ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool live) {
+  const int n = live ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
+
+// Operand type of the products: f16, or bf16 for bf16 caches.
+template <bool BF>
+struct Op {
+  __device__ static __forceinline__ uint32_t pack(float x, float y) {
+    if (BF) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  // x and y keep what the packed pair left of them
+  __device__ static __forceinline__ uint32_t take(float& x, float& y) {
+    if (BF) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+      x -= __low2float(h), y -= __high2float(h);
+      return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(x, y);
+    x -= __low2float(h), y -= __high2float(h);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ static __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF)
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+          : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ float lds4(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+// Four codes of one word as two f16 pairs, in order. q8: whole numbers; e4m3: the value times 2^-8.
+template <bool E4M3>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t* lo, uint32_t* hi) {
+  if (E4M3) {
+    *lo = kv_e4m3_to_half2(prmt(w, 0, 0x1404)), *hi = kv_e4m3_to_half2(prmt(w, 0, 0x3424));
+  } else {
+    w ^= 0x80808080u;
+    *lo = kv_q8_to_half2(prmt(w, 0x64646464u, 0x4140)), *hi = kv_q8_to_half2(prmt(w, 0x64646464u, 0x4342));
+  }
+}
+// Entry i (0 .. 3) of two words, interleaved: (x_i, y_i) as an f16 pair; r[i].
+template <bool E4M3>
+__device__ __forceinline__ void widen_pairs(uint32_t x, uint32_t y, uint32_t (&r)[4]) {
+  if (E4M3) {
+    r[0] = kv_e4m3_to_half2(prmt(x, y, 0x4000)), r[1] = kv_e4m3_to_half2(prmt(x, y, 0x5010));
+    r[2] = kv_e4m3_to_half2(prmt(x, y, 0x6020)), r[3] = kv_e4m3_to_half2(prmt(x, y, 0x7030));
+  } else {
+    const uint32_t lo = prmt(x, y, 0x5140) ^ 0x80808080u, hi = prmt(x, y, 0x7362) ^ 0x80808080u;
+    r[0] = kv_q8_to_half2(prmt(lo, 0x64646464u, 0x4140)), r[1] = kv_q8_to_half2(prmt(lo, 0x64646464u, 0x4342));
+    r[2] = kv_q8_to_half2(prmt(hi, 0x64646464u, 0x4140)), r[3] = kv_q8_to_half2(prmt(hi, 0x64646464u, 0x4342));
+  }
+}
+
+// CT: cache; TQ: type of q and out; D: head dimensions, d filled up with zeros; MT: 16-row tiles per warp; WR: warps along the
+// rows; WK: key groups.
+template <int CT, typename TQ, int D_, int MT_, int WR_, int WK_>
+struct Cfg {
+  static constexpr int D = D_, MT = MT_, WR = WR_, WK = WK_;
+  static constexpr bool BF = CT == TREE_BF16, WIDE = CT == TREE_BF16 || CT == TREE_F16, E4M3 = CT == TREE_E4M3;
+  static constexpr int ES = WIDE ? 2 : 1;
+  static constexpr bool QF = std::is_same<TQ, float>::value, QB = std::is_same<TQ, __nv_bfloat16>::value;
+  static constexpr int QT = BF ? (QB ? 1 : QF ? 3 : 2) : (QF ? 2 : 1);   // terms of Q
+  static constexpr int PT = BF ? (QF ? 3 : 2) : (QB ? 1 : 2);            // terms of P
+  static constexpr int RB = 16 * MT * WR;                                // rows of a block
+  static constexpr int THREADS = 32 * WR * WK;
+  static constexpr int KT = (WIDE ? 16 : 32) * (WR >= 2 ? 2 : 1);        // keys of a tile
+  static constexpr int STAGES = 3;
+  static constexpr int TILE = KT * D * ES;
+  static constexpr int STAGE = 2 * TILE + (WIDE ? 0 : 2 * KT * 4);
+  static constexpr int RING = STAGE * STAGES * WK;
+  static constexpr bool QREG = MT == 1;                                  // Q stays in registers, else in shared memory
+  static constexpr int QSM = QREG ? 0 : RB * D * 2 * QT;
+  static constexpr int STATE = WK * RB * (D + 2) * 4;                    // (output, maximum, sum) of every key group
+  static constexpr int BODY = RING > STATE ? RING : STATE;
+  static constexpr int SMEM = BODY + QSM;
+};
+
+template <typename C>
+__device__ __forceinline__ uint32_t k_chunk(int key, int chunk) {  // byte offset of a 16-byte chunk of a key's row in a tile
+  constexpr int PER = C::D * C::ES / 16;
+  if (C::WIDE) return (uint32_t)(key * PER + (chunk ^ (key & 7 & (PER - 1)))) * 16;
+  return (uint32_t)(key * PER + (PER == 8 ? chunk ^ ((key & 1) << 2) : chunk)) * 16;
+}
+template <typename C>
+__device__ __forceinline__ uint32_t v_chunk(int key, int chunk) {
+  constexpr int PER = C::D * C::ES / 16;
+  return (uint32_t)(key * PER + (chunk ^ (key & 7 & (PER - 1)))) * 16;
+}
+
+__device__ __forceinline__ bool sees(const TreeArgs& a, int64_t b, int row, int64_t j) {
+  if (j < 0) return true;
+  if (j >= a.rows) return false;
+  return a.mask ? a.mask[b * a.ms[0] + row * a.ms[1] + j] != 0 : j <= row;
+}
+
+template <int CT, typename TQ, int D, int MT, int WR, int WK>
+__global__ void __launch_bounds__(32 * WR * WK) tree_attention_kernel(const __grid_constant__ TreeArgs a) {
+  using C = Cfg<CT, TQ, D, MT, WR, WK>;
+  using O = Op<C::BF>;
+  constexpr int KT = C::KT, NT = D / 8, KS = D / 16, NK = KT / 8;
+  extern __shared__ __align__(128) uint8_t tree_shared[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+  const int wr = warp % WR, wk = warp / WR;
+  const int split = (int)blockIdx.x % a.splits;
+  const int64_t pair = blockIdx.x / a.splits;
+  const int64_t b = pair / a.kv_heads;
+  const int kvh = (int)(pair - b * a.kv_heads);
+  const int total_rows = a.rows * a.group, row0 = blockIdx.y * C::RB;
+
+  int64_t len = a.lengths[b];
+  int64_t keys = 0;
+  if (len >= 0) {
+    len = len < a.cap ? len : a.cap;
+    keys = len + a.rows < a.cap ? len + a.rows : a.cap;
+  }
+  const uint8_t* kb = a.k + b * a.kst[0] + kvh * a.kst[1];
+  const uint8_t* vb = a.v + b * a.vst[0] + kvh * a.vst[1];
+  const float* ksb = C::WIDE ? nullptr : a.ks + b * a.kss[0] + kvh * a.kss[1];
+  const float* vsb = C::WIDE ? nullptr : a.vs + b * a.vss[0] + kvh * a.vss[1];
+
+  // ---- tiles: the group takes every (splits * WK)-th one ----
+  const int64_t tiles = (keys + KT - 1) / KT;
+  const int64_t first = (int64_t)split * WK + wk, step = (int64_t)a.splits * WK;
+  const uint32_t ring = smem_u32(tree_shared) + (uint32_t)(wk * C::STAGES * C::STAGE);
+  const int gtid = wr * 32 + lane;
+  const int chunks = a.d * C::ES / 16;
+  auto fetch = [&](int64_t tile, int stage) {
+    if (tile < tiles) {
+      const uint32_t at = ring + (uint32_t)(stage * C::STAGE);
+      const int64_t key0 = tile * KT;
+      constexpr int PER = D * C::ES / 16;
+#pragma unroll
+      for (int i = 0; i < KT * PER / (32 * WR); i++) {
+        const int u = i * 32 * WR + gtid, key = u / PER, c = u % PER;
+        const int64_t kk = key0 + key;
+        const bool live = kk < keys && c < chunks;
+        cp16(at + k_chunk<C>(key, c), live ? kb + kk * a.kst[2] + c * 16 : kb, live);
+        cp16(at + C::TILE + v_chunk<C>(key, c), live ? vb + kk * a.vst[2] + c * 16 : vb, live);
+      }
+      if (!C::WIDE) {
+        for (int u = gtid; u < KT; u += 32 * WR) {
+          const int64_t kk = key0 + u;
+          const bool live = kk < keys;
+          cp4(at + 2 * C::TILE + u * 4, live ? ksb + kk : ksb, live);
+          cp4(at + 2 * C::TILE + (KT + u) * 4, live ? vsb + kk : vsb, live);
+        }
+      }
+    }
+    cp_commit();
+  };
+  auto begin = [&] {
+#pragma unroll
+    for (int i = 0; i < C::STAGES - 1; i++) fetch(first + i * step, i);
+  };
+  begin();
+
+  // ---- Q: this warp's rows, in the order in which keys' dimensions come out ----
+  // element e (0 .. 3) of k16 step s at lane quarter t: 2-byte keys 16 s + 2 t + {0, 1, 8, 9}; 8-bit keys lie 16 bytes per lane
+  uint32_t qf[C::QREG ? C::QT : 1][C::QREG ? KS : 1][4];
+  uint8_t* qs = tree_shared + C::BODY;
+  float mult[MT][2];  // what a row's scores are multiplied with: log2(e) * scale / the row's power of two
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    float x[2][KS][4];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int r = row0 + (wr * MT + m) * 16 + g + 8 * h;
+      const bool live = r < total_rows;
+      const int tr = live ? r / a.group : 0, gh = live ? r - tr * a.group : 0;
+      const TQ* src = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
+      float top = 0.f;
+#pragma unroll
+      for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int dim = C::WIDE ? 16 * s + 2 * t + (e & 1) + 8 * (e >> 1) : s / 4 * 64 + t * 16 + s % 4 * 4 + e;
+          x[h][s][e] = live && dim < a.d ? kv_float(src[dim]) : 0.f;
+          top = fmaxf(top, fabsf(x[h][s][e]));
+        }
+      float mul = 1.f, inv = 1.f;
+      if (!C::BF) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the row's largest element to 2^8 .. 2^9; zeros, infinities and extremes of f32 keep a bounded factor
+        int ex = (int)((__float_as_uint(top) >> 23) & 0xff);
+        ex = ex < 20 ? 20 : ex > 250 ? 250 : ex;
+        mul = __uint_as_float((uint32_t)(262 - ex) << 23), inv = __uint_as_float((uint32_t)(ex - 8) << 23);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[h][s][e] *= mul;
+      }
+      mult[m][h] = a.scale * LOG2E * inv * (C::E4M3 ? 256.f : 1.f);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int n = 0; n < C::QT; n++) {
+        uint32_t f[4];
+        f[0] = O::take(x[0][s][0], x[0][s][1]), f[1] = O::take(x[1][s][0], x[1][s][1]);
+        f[2] = O::take(x[0][s][2], x[0][s][3]), f[3] = O::take(x[1][s][2], x[1][s][3]);
+        if (C::QREG) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) qf[C::QREG ? n : 0][C::QREG ? s : 0][i] = f[i];
+        } else if (wk == 0) {
+          *reinterpret_cast<uint4*>(qs + ((((wr * MT + m) * C::QT + n) * KS + s) * 32 + lane) * 16) = make_uint4(f[0], f[1], f[2], f[3]);
+        }
+      }
+  }
+  if (!C::QREG) __syncthreads();
+  const uint32_t qaddr = smem_u32(qs) + (uint32_t)(wr * MT * C::QT * KS * 512 + lane * 16);
+
+  // ---- the running state ----
+  float out[MT][NT][4], top[MT][2], sum[MT][2];
+  // 2-byte values that are not finite: weight 0, or a weight's zero second term, times one is not a number. Where a result is
+  // not finite the keys are gone through once more, with such entries left out of the products and added one by one.
+  for (bool careful = false;; careful = true) {
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) out[m][n][e] = 0.f;
+    top[m][0] = top[m][1] = -INFINITY, sum[m][0] = sum[m][1] = 0.f;
+  }
+
+  int stage = 0;
+  for (int64_t tile = first; tile < tiles; tile += step) {
+    cp_wait<C::STAGES - 2>();
+    if (WR > 1)
+      asm volatile("bar.sync %0, %1;" ::"r"(wk + 1), "n"(32 * WR) : "memory");
+    else
+      __syncwarp();
+    {
+      int ahead = stage + C::STAGES - 1;
+      if (ahead >= C::STAGES) ahead -= C::STAGES;
+      fetch(tile + (C::STAGES - 1) * step, ahead);
+    }
+    const uint32_t kt = ring + (uint32_t)(stage * C::STAGE), vt = kt + C::TILE, st = vt + C::TILE;
+    if (++stage == C::STAGES) stage = 0;
+
+    // S
+    float sc[MT][NK][4];
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int j = 0; j < NK; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) sc[m][j][e] = 0.f;
+    if (C::WIDE) {
+#pragma unroll
+      for (int s = 0; s < KS; s++) {
+        uint32_t kf[NK][2];
+#pragma unroll
+        for (int j = 0; j < NK; j += 2) {
+          uint32_t r[4];
+          const int key = j * 8 + (lane & 7) + ((lane >> 4) << 3);
+          ldsm4(r, kt + k_chunk<C>(key, 2 * s + ((lane >> 3) & 1)));
+          kf[j][0] = r[0], kf[j][1] = r[1], kf[j + 1][0] = r[2], kf[j + 1][1] = r[3];
+        }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int n = C::QT - 1; n >= 0; n--) {
+            uint32_t f[4];
+            if (C::QREG) {
+#pragma unroll
+              for (int i = 0; i < 4; i++) f[i] = qf[C::QREG ? n : 0][C::QREG ? s : 0][i];
+            } else {
+              const uint4 w = lds16(qaddr + (uint32_t)(((m * C::QT + n) * KS + s) * 512));
+              f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
+            }
+#pragma unroll
+            for (int j = 0; j < NK; j++) O::mma(sc[m][j], f, kf[j][0], kf[j][1]);
+          }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < D / 64; h++) {
+        uint4 raw[NK];
+#pragma unroll
+        for (int j = 0; j < NK; j++) raw[j] = lds16(kt + k_chunk<C>(j * 8 + g, h * 4 + t));
+#pragma unroll
+        for (int s4 = 0; s4 < 4; s4++) {
+          const int s = h * 4 + s4;
+          uint32_t kf[NK][2];
+#pragma unroll
+          for (int j = 0; j < NK; j++)
+            widen<C::E4M3>(s4 == 0 ? raw[j].x : s4 == 1 ? raw[j].y : s4 == 2 ? raw[j].z : raw[j].w, &kf[j][0], &kf[j][1]);
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = C::QT - 1; n >= 0; n--) {
+              uint32_t f[4];
+              if (C::QREG) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) f[i] = qf[C::QREG ? n : 0][C::QREG ? s : 0][i];
+              } else {
+                const uint4 w = lds16(qaddr + (uint32_t)(((m * C::QT + n) * KS + s) * 512));
+                f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
+              }
+#pragma unroll
+              for (int j = 0; j < NK; j++) O::mma(sc[m][j], f, kf[j][0], kf[j][1]);
+            }
+        }
+      }
+    }
+
+    // scores in powers of two, masked
+    const int64_t key0 = tile * KT;
+    float vscale[C::WIDE ? 1 : NK][2];
+    float pmul = C::BF ? 1.f : 16384.f, punit = C::BF ? 1.f : 0x1p-14f;
+    if (!C::WIDE) {
+      float most = 0.f;
+#pragma unroll
+      for (int j = 0; j < NK; j++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          vscale[C::WIDE ? 0 : j][e] = lds4(st + (uint32_t)(KT + j * 8 + 2 * t + e) * 4);
+          most = fmaxf(most, vscale[C::WIDE ? 0 : j][e]);
+          const float kscale = lds4(st + (uint32_t)(j * 8 + 2 * t + e) * 4);
+#pragma unroll
+          for (int m = 0; m < MT; m++) sc[m][j][e] *= kscale, sc[m][j][e + 2] *= kscale;
+        }
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      int ex = (int)(__float_as_uint(most) >> 23);
+      ex = ex < 30 ? 30 : ex > 240 ? 240 : ex;
+      pmul = __uint_as_float((uint32_t)(254 + 13 - ex) << 23);   // the tile's largest value scale to 2^13 .. 2^14
+      punit = __uint_as_float((uint32_t)(ex - 13 + (C::E4M3 ? 8 : 0)) << 23);
+    }
+    const bool tail = key0 + KT > len;
+    uint32_t vis[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; m++) vis[m][0] = vis[m][1] = 0xffffffffu;
+    if (tail) {
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int r = row0 + (wr * MT + m) * 16 + g + 8 * h;
+          const int tr = r < total_rows ? r / a.group : 0;
+          uint32_t bits = 0;
+#pragma unroll
+          for (int j = 0; j < NK; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+              if (key0 + j * 8 + 2 * t + e < keys && sees(a, b, tr, key0 + j * 8 + 2 * t + e - len)) bits |= 1u << (2 * j + e);
+          vis[m][h] = bits;
+        }
+    }
+    float decay[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        // the maximum in powers of two; a score and its maximum go through one fma, so that the score is not rounded before
+        // the difference. Masked entries are -infinity by a choice, not by a product with a factor that may be zero
+        float best = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NK; j++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float s = sc[m][j][2 * h + e] * mult[m][h];
+            best = fmaxf(best, !tail || vis[m][h] >> (2 * j + e) & 1 ? s : -INFINITY);
+          }
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+        best = fmaxf(best, top[m][h]);
+        const float base = best == -INFINITY ? 0.f : best;
+        decay[m][h] = ex2(top[m][h] - base);
+        top[m][h] = best;
+        float part = 0.f;
+#pragma unroll
+        for (int j = 0; j < NK; j++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            float p = ex2(fmaf(sc[m][j][2 * h + e], mult[m][h], -base));
+            if (tail && !(vis[m][h] >> (2 * j + e) & 1)) p = 0.f;
+            sc[m][j][2 * h + e] = p;
+            part += p;
+          }
+        sum[m][h] = sum[m][h] * decay[m][h] + part;
+      }
+    // weights as operands
+    uint32_t pf[MT][C::PT][NK / 2][4];
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int j = 0; j < NK; j++) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          w[e] = sc[m][j][e] * pmul;
+          if (!C::WIDE) {
+            w[e] *= vscale[C::WIDE ? 0 : j][e & 1];
+            if (tail && !(vis[m][e >> 1] >> (2 * j + (e & 1)) & 1)) w[e] = 0.f;  // the scale of a key that is not seen
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < C::PT; n++) {
+          pf[m][n][j / 2][(j & 1) * 2] = O::take(w[0], w[1]);
+          pf[m][n][j / 2][(j & 1) * 2 + 1] = O::take(w[2], w[3]);
+        }
+      }
+    bool odd = false;
+    if (C::WIDE && careful) {
+      constexpr int PER = D * C::ES / 16;
+      for (int u = lane; u < KT * PER; u += 32) {
+        const uint4 w = lds16(vt + (uint32_t)u * 16);
+        const uint32_t mask = C::BF ? 0x7f807f80u : 0x7c007c00u, x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          odd |= ((x[i] & mask & 0xffffu) == (mask & 0xffffu)) || ((x[i] & mask & 0xffff0000u) == (mask & 0xffff0000u));
+      }
+      odd = __any_sync(0xffffffffu, odd);
+    }
+    // O = O * decay + P V
+#pragma unroll
+    for (int nb = 0; nb < NT / 2; nb++) {
+      // two n8 tiles at a time (2-byte), or four (8-bit: a word of four dimensions)
+      if (C::WIDE) {
+        float u[MT][2][4];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) u[m][i][e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < NK / 2; kk++) {
+          uint32_t r[4];
+          const int key = kk * 16 + (lane & 15);
+          ldsm4t(r, vt + v_chunk<C>(key, 2 * nb + (lane >> 4)));
+          if (odd) {
+            const uint32_t mask = C::BF ? 0x7f80u : 0x7c00u;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              if ((r[i] & mask) == mask) r[i] &= 0xffff0000u;
+              if ((r[i] >> 16 & mask) == mask) r[i] &= 0xffffu;
+            }
+          }
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = C::PT - 1; n >= 0; n--) {
+              O::mma(u[m][0], pf[m][n][kk], r[0], r[1]);
+              O::mma(u[m][1], pf[m][n][kk], r[2], r[3]);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) out[m][2 * nb + i][e] = out[m][2 * nb + i][e] * decay[m][e >> 1] + u[m][i][e] * punit;
+      }
+    }
+    if (C::WIDE && odd) {
+      // the entries left out, to the rows that see their keys
+#pragma unroll 1
+      for (int key = 0; key < KT; key++) {
+        const int j = key / 8, from = (lane & ~3) + (key & 7) / 2;
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+          // which of the two columns is a matter of the key: picked without indexing registers
+          float p0 = 0.f, p1 = 0.f;
+          uint32_t s0 = 0, s1 = 0;
+#pragma unroll
+          for (int jj = 0; jj < NK; jj++)
+            if (jj == j) {
+              p0 = key & 1 ? sc[m][jj][1] : sc[m][jj][0], p1 = key & 1 ? sc[m][jj][3] : sc[m][jj][2];
+              s0 = vis[m][0] >> (2 * jj + (key & 1)) & 1, s1 = vis[m][1] >> (2 * jj + (key & 1)) & 1;
+            }
+          p0 = __shfl_sync(0xffffffffu, p0, from), p1 = __shfl_sync(0xffffffffu, p1, from);
+          s0 = __shfl_sync(0xffffffffu, s0, from), s1 = __shfl_sync(0xffffffffu, s1, from);
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            uint32_t w;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vt + v_chunk<C>(key, n) + 4 * t));
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              const uint32_t half = e ? w >> 16 : w & 0xffffu, mask = C::BF ? 0x7f80u : 0x7c00u;
+              if ((half & mask) == mask) {
+                const float val = C::BF ? __bfloat162float(__ushort_as_bfloat16((unsigned short)half)) : __half2float(__ushort_as_half((unsigned short)half));
+                if (s0) out[m][n][e] += p0 * val;
+                if (s1) out[m][n][e + 2] += p1 * val;
+              }
+            }
+          }
+        }
+      }
+    }
+    if (!C::WIDE) {
+      // lane g has D / 8 consecutive dimensions of a key: n8 tile i is dimension g * D / 8 + i
+      constexpr int WORDS = D / 32;  // words of a key per lane
+#pragma unroll
+      for (int w4 = 0; w4 < WORDS; w4++) {
+        float u[MT][4][4];
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) u[m][i][e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < NK / 2; kk++) {
+          uint32_t x[4];
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int key = kk * 16 + 2 * t + (i & 1) + 8 * (i >> 1), at = g * (D / 8) + w4 * 4;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x[i]) : "r"(vt + v_chunk<C>(key, at / 16) + (uint32_t)(at % 16)));
+          }
+          uint32_t r0[4], r1[4];
+          widen_pairs<C::E4M3>(x[0], x[1], r0);
+          widen_pairs<C::E4M3>(x[2], x[3], r1);
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int n = C::PT - 1; n >= 0; n--)
+#pragma unroll
+              for (int i = 0; i < 4; i++) O::mma(u[m][i], pf[m][n][kk], r0[i], r1[i]);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) out[m][w4 * 4 + i][e] = out[m][w4 * 4 + i][e] * decay[m][e >> 1] + u[m][i][e] * punit;
+      }
+    }
+  }
+  cp_wait<0>();
+  if (!C::WIDE || careful) break;
+  bool finite = true;
+#pragma unroll
+  for (int m = 0; m < MT; m++)
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) finite = finite && fabsf(out[m][n][e]) < INFINITY;
+  if (!__syncthreads_or(!finite)) break;
+  begin();
+  }
+#pragma unroll
+  for (int m = 0; m < MT; m++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 1);
+      sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 2);
+    }
+  __syncthreads();  // the ring becomes the states' place
+
+  // ---- states of the key groups, then of the cluster's blocks ----
+  float* so = reinterpret_cast<float*>(tree_shared);          // [WK][RB][D]
+  float* sm = so + WK * C::RB * D;                             // [WK][RB] (maximum, sum)
+#pragma unroll
+  for (int m = 0; m < MT; m++)
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int r = (wr * MT + m) * 16 + g + 8 * h;
+      float* to = so + (wk * C::RB + r) * D;
+      if (C::WIDE) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) *reinterpret_cast<float2*>(to + n * 8 + 2 * t) = make_float2(out[m][n][2 * h], out[m][n][2 * h + 1]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; e++)
+#pragma unroll
+          for (int n = 0; n < NT; n += 4)
+            *reinterpret_cast<float4*>(to + (2 * t + e) * (D / 8) + n) =
+                make_float4(out[m][n][2 * h + e], out[m][n + 1][2 * h + e], out[m][n + 2][2 * h + e], out[m][n + 3][2 * h + e]);
+      }
+      if (t == 0) sm[(wk * C::RB + r) * 2] = top[m][h], sm[(wk * C::RB + r) * 2 + 1] = sum[m][h];
+    }
+  __syncthreads();
+  // group states into the first one: a thread takes four dimensions of a row
+  const int live_rows = min(C::RB, total_rows - row0);
+  if (WK > 1) {
+    float best[1];
+    for (int i = threadIdx.x; i < live_rows * (D / 4); i += C::THREADS) {
+      const int r = i / (D / 4), c = i % (D / 4) * 4;
+      best[0] = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WK; w++) best[0] = fmaxf(best[0], sm[(w * C::RB + r) * 2]);
+      const float base = best[0] == -INFINITY ? 0.f : best[0];
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WK; w++) {
+        const float f = ex2(sm[(w * C::RB + r) * 2] - base);
+        const float4 x = *reinterpret_cast<const float4*>(so + (w * C::RB + r) * D + c);
+        o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+      }
+      *reinterpret_cast<float4*>(so + r * D + c) = o;
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < live_rows; r += C::THREADS) {
+      float m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < WK; w++) m = fmaxf(m, sm[(w * C::RB + r) * 2]);
+#pragma unroll
+      for (int w = 0; w < WK; w++) l += sm[(w * C::RB + r) * 2 + 1] * ex2(sm[(w * C::RB + r) * 2] - (m == -INFINITY ? 0.f : m));
+      sm[r * 2] = m, sm[r * 2 + 1] = l;
+    }
+  }
+  if (a.splits > 1)
+    asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
+  else
+    __syncthreads();
+  // a block of the cluster takes every splits-th piece of four dimensions
+  const uint32_t so_at = smem_u32(so), sm_at = smem_u32(sm);
+  for (int i = split * C::THREADS + threadIdx.x; i < live_rows * (D / 4); i += a.splits * C::THREADS) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    float m = -INFINITY, l = 0.f;
+    float o[4] = {};
+    for (int p = 0; p < a.splits; p++) {
+      uint32_t at_m, at_o;
+      float pm, pl, x[4];
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_m) : "r"(sm_at + (uint32_t)r * 8), "r"(p));
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_o) : "r"(so_at + (uint32_t)(r * D + c) * 4), "r"(p));
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(pm), "=f"(pl) : "r"(at_m) : "memory");
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(at_o) : "memory");
+      const float next = fmaxf(m, pm), base = next == -INFINITY ? 0.f : next;
+      const float fa = ex2(m - base), fb = ex2(pm - base);
+      l = l * fa + pl * fb;
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] = o[e] * fa + x[e] * fb;
+      m = next;
+    }
+    const int tr = (row0 + r) / a.group, gh = row0 + r - tr * a.group;
+    TQ* to = static_cast<TQ*>(a.out) + ((b * a.rows + tr) * a.heads + (int64_t)kvh * a.group + gh) * a.d + c;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (c < a.d) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) kv_store(o[e] * inv, to + e);
+    }
+  }
+  if (a.splits > 1) asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");  // others read this block's states
+}
+
+template <int CT, typename TQ, int D, int MT, int WR, int WK>
+int run(TreeArgs a, cudaStream_t s) {
+  using C = Cfg<CT, TQ, D, MT, WR, WK>;
+  auto kernel = tree_attention_kernel<CT, TQ, D, MT, WR, WK>;
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), C::SMEM)) return 1;
+  const int64_t pairs = a.batch * a.kv_heads;
+  a.row_blocks = (int)(((int64_t)a.rows * a.group + C::RB - 1) / C::RB);
+  // blocks of a cluster: as many as two per SM leave room for, at least two tiles for each key group at full capacity
+  int splits = 16;
+  while (splits > 1 && (pairs * a.row_blocks * splits > 2 * std::max(1, sm_count()) || a.cap < (int64_t)splits * WK * C::KT * 2)) splits /= 2;
+  if (splits > 8) DYN_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  a.splits = splits;
+  DYN_CHECK(pairs * splits <= 0x7fffffff && a.row_blocks <= 65535, "tree_attention: too many sequences or rows for one call");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(pairs * splits), (unsigned)a.row_blocks), cfg.blockDim = dim3(C::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM, cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  DYN_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+  count_launch();
+  return 0;
+}
+
+template <int CT, typename TQ, int D>
+int by_rows(const TreeArgs& a, cudaStream_t s) {
+  const int64_t rows = (int64_t)a.rows * a.group;
+  if (rows <= 16) return run<CT, TQ, D, 1, 1, 4>(a, s);
+  if (rows <= 32) return run<CT, TQ, D, 2, 1, 4>(a, s);
+  if (rows <= 64) return run<CT, TQ, D, 2, 2, 2>(a, s);
+  return run<CT, TQ, D, 2, 4, 1>(a, s);
+}
+
+template <int CT>
+int by_type(const TreeArgs& a, int q_type, cudaStream_t s) {
+  if (a.d <= 64) {
+    if (q_type == E_F32) return by_rows<CT, float, 64>(a, s);
+    if (q_type == E_F16) return by_rows<CT, __half, 64>(a, s);
+    return by_rows<CT, __nv_bfloat16, 64>(a, s);
+  }
+  if (q_type == E_F32) return by_rows<CT, float, 128>(a, s);
+  if (q_type == E_F16) return by_rows<CT, __half, 128>(a, s);
+  return by_rows<CT, __nv_bfloat16, 128>(a, s);
+}
+
+}  // namespace tree
+}  // namespace dyn

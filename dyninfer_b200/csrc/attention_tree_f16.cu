@@ -1,0 +1,8 @@
+// Tree attention over f16 caches.
+#include "attention_tree.cuh"
+
+namespace dyn {
+
+int tree_attention_f16(const TreeArgs& a, int q_type, cudaStream_t s) { return tree::by_type<TREE_F16>(a, q_type, s); }
+
+}  // namespace dyn

@@ -454,6 +454,35 @@ int launch_attention_split(const AttnArgs& a, float* part, int nsplit, cudaStrea
 size_t attention_prefill_scratch_bytes(const AttnArgs& a);
 int launch_attention_prefill(const AttnArgs& a, int64_t base_pos, int64_t seq, cudaStream_t s, bool* handled);
 
+// ---- operators of speculative decoding (rotary.cu, kv_quant.cu, attention_tree*.cu, verify_draft.cu) ----
+constexpr int ROTARY_MAX_DIM = 256;
+// Strides count elements between batch entries, rows and heads; `frequencies` [rot / 2] is a host array. y may be x.
+int launch_rotary(const void* x, int type, int64_t batch, int64_t rows, int64_t heads, int64_t d, const int64_t* x_strides,
+                  const int64_t* positions, const double* frequencies, int64_t rot, bool interleaved, double magnitude, void* y,
+                  const int64_t* y_strides, cudaStream_t s);
+
+// Rows of keys and values [batch][rows][heads][d] beside the 8-bit cache they are written to or read from.
+struct KvRows {
+  void* x[2];                    // keys, values of `type`
+  const int64_t* x_strides;      // [2][3] elements between batch entries, rows, heads
+  void* codes[2];                // [slot][head][cap][d] bytes
+  const int64_t* code_strides;   // [2][3] between slots, heads, rows
+  float* scales[2];              // [slot][head][cap]
+  const int64_t* scale_strides;  // [2][2] between slots, heads
+  const int64_t* starts;         // [batch] cache row of row 0
+  const int64_t* counts;         // [batch] rows there are; NULL: all
+  int64_t batch, rows, heads, d, cap;
+  int type;
+  bool e4m3;
+};
+int launch_kv_rows(const KvRows& r, bool write, cudaStream_t s);
+
+// Strides count elements between batch entries and nodes; `draft` may be NULL.
+int launch_verify_draft(const int64_t* tokens, const int64_t* parents, int64_t parents_stride, const void* target,
+                        const int64_t* target_strides, const void* draft, const int64_t* draft_strides, int type,
+                        const float* uniforms, int64_t batch, int64_t nodes, int64_t vocab, int64_t* accepted, int64_t* path,
+                        int64_t* next, cudaStream_t s);
+
 size_t argmax_scratch_bytes(int64_t n);
 int launch_argmax(const float* v, int64_t n, int64_t* out, void* scratch, cudaStream_t s);
 int launch_argmax_rows(const float* v, int64_t rows, int64_t n, int64_t* out, cudaStream_t s);

@@ -1,0 +1,287 @@
+// Verification of a tree of drafted tokens against the target's probabilities, with given random numbers.
+//
+// Node 0 is the last token of the text; every other node stands behind its parent, and the target's row i is the distribution of
+// the token behind node i. From node 0 on, the children c of the node reached are tried in order: with r_0 = p (the target's row
+// of the node), Z_0 = 1,
+//   c is taken    if u_c q(c) Z_m < r_m(c)                      (q: the draft's row of the node; 1 without a draft)
+//   if refused    r_{m+1} = max(r_m / Z_m - q, 0), Z_{m+1} = sum of it;   without a draft r_{m+1} = r_m with c's entry gone and
+//                 Z_{m+1} = Z_m - r_m(c).
+// The last token is drawn from what is left at the node where no child was taken: the first v with r(0) + .. + r(v) above
+// u_0 times the sum. Where nothing is left, from the target's row itself; where that has no finite positive sum, it is -1.
+// Every sum is in 64 bits: a border between two of 150000 entries is a matter of 1e-9, and the answer is a whole number.
+//
+// Whether a child is taken depends on single entries, which are fetched for all nodes at once; what costs is one pass over a
+// row of target (and draft) per refusal, about 1.2 MB for 150000 entries, so memory and latency bound it. A cluster of up to 16
+// blocks takes a sequence, every warp a run of entries; the warps' sums meet through shared memory, in one order everywhere, so
+// that all blocks walk the tree alike without asking one another. The sums are also what the draw searches: the warp
+// whose run holds the border looks through its own run once more, out of the caches.
+#include <algorithm>
+
+#include "common.cuh"
+#include "ring.cuh"
+
+namespace dyn {
+
+namespace {
+
+constexpr int VD_THREADS = 512, VD_WARPS = VD_THREADS / 32, VD_LOADS = 8;
+
+struct VdArgs {
+  const int64_t *tokens, *parents;  // [batch][nodes]
+  int64_t parents_stride;           // 0: one tree for all
+  const void *target, *draft;       // [batch][nodes][vocab]; draft may be NULL
+  int64_t ts[2], ds[2];             // elements between batch entries and nodes
+  const float* uniforms;            // [batch][nodes]
+  int64_t *accepted, *path, *next;  // [batch], [batch][nodes], [batch]
+  int nodes, blocks;                // blocks of a cluster
+  int64_t vocab, run;               // entries of a warp
+};
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
+}
+__device__ __forceinline__ double peer_f64(const double* p, int rank) {
+  uint32_t at;
+  double v;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ double vd_value(float x) { return x; }
+__device__ __forceinline__ double vd_value(__half x) { return __half2float(x); }
+__device__ __forceinline__ double vd_value(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// What is left of entry v (p and q: the rows' entries) after m refusals at the node, with the sums in between and the tokens
+// that are `gone`.
+template <bool DRAFT>
+__device__ __forceinline__ double left_of(double p, double q, int64_t v, int m, const double* sums, const int64_t* gone) {
+  if (DRAFT) {
+    for (int j = 0; j < m; j++) {
+      p = (j ? (sums[j] > 0. ? p / sums[j] : 0.) : p) - q;
+      p = p < 0. ? 0. : p;  // NaN stays NaN
+    }
+  } else {
+    for (int j = 0; j < m; j++)
+      if (gone[j] == v) p = 0.;
+  }
+  return p;
+}
+
+template <typename T, bool DRAFT>
+__global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(const __grid_constant__ VdArgs a) {
+  extern __shared__ double vd_shared[];
+  double* p_of = vd_shared;                 // [nodes] target's entry of the node's token in its parent's row
+  double* q_of = p_of + a.nodes;            // [nodes] the draft's
+  double* sums = q_of + a.nodes;            // [nodes] Z_m at the present node
+  int64_t* token = reinterpret_cast<int64_t*>(sums + a.nodes);
+  int64_t* gone = token + a.nodes;          // tokens refused at the present node
+  float* uniform = reinterpret_cast<float*>(gone + a.nodes);
+  int* parent = reinterpret_cast<int*>(uniform + a.nodes);
+  int* path = parent + a.nodes;
+  __shared__ double own[2][VD_WARPS], all[16 * VD_WARPS];
+  __shared__ int s_node, s_m, s_i, s_count, s_owner;  // where the walk stands; whose run holds the drawn token
+  __shared__ double s_total, s_z, s_before;
+
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, n = a.nodes;
+  const int rank = (int)blockIdx.x % a.blocks;
+  const int64_t b = blockIdx.x / a.blocks;
+  const T* target = static_cast<const T*>(a.target) + b * a.ts[0];
+  const T* draft = static_cast<const T*>(a.draft) + (DRAFT ? b * a.ds[0] : 0);
+  for (int i = tid; i < n; i += VD_THREADS) {
+    const int64_t up = a.parents[b * a.parents_stride + i], t = a.tokens[b * n + i];
+    const bool known = i > 0 && up >= 0 && up < i && t >= 0 && t < a.vocab;
+    parent[i] = i > 0 && up >= 0 && up < i ? (int)up : -1;
+    token[i] = t;
+    uniform[i] = a.uniforms[b * n + i];
+    p_of[i] = known ? vd_value(target[up * a.ts[1] + t]) : 0.;
+    q_of[i] = known ? (DRAFT ? vd_value(draft[up * a.ds[1] + t]) : 1.) : 0.;
+  }
+  if (tid == 0) s_node = 0, s_m = 0, s_i = 1, s_count = 0, s_z = 1., sums[0] = 1., path[0] = 0;
+  __syncthreads();
+
+  const int64_t lo = min(a.vocab, ((int64_t)rank * VD_WARPS + warp) * a.run), hi = min(a.vocab, lo + a.run);
+  const int runs = a.blocks * VD_WARPS;
+  int round = 0;
+  // all[] = every warp's sum of what is left at `node` after m refusals, s_total = their sum: the same in all blocks
+  auto sum_up = [&](int node, int m) {
+    const T* p = target + (int64_t)node * a.ts[1];
+    const T* q = DRAFT ? draft + (int64_t)node * a.ds[1] : nullptr;
+    double sum = 0.;
+    for (int64_t v = lo + lane; v < hi; v += 32 * VD_LOADS) {
+      T pe[VD_LOADS], qe[VD_LOADS];
+#pragma unroll
+      for (int j = 0; j < VD_LOADS; j++)
+        if (v + j * 32 < hi) {
+          pe[j] = p[v + j * 32];
+          if (DRAFT && m) qe[j] = q[v + j * 32];
+        }
+#pragma unroll
+      for (int j = 0; j < VD_LOADS; j++)
+        if (v + j * 32 < hi)
+          sum += left_of<DRAFT>(vd_value(pe[j]), DRAFT && m ? vd_value(qe[j]) : 0., v + j * 32, m, sums, gone);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    // buffers alternate: one is written again behind a barrier that all its readers have passed
+    if (lane == 0) own[round & 1][warp] = sum;
+    cluster_sync();
+    if (tid < runs) all[tid] = peer_f64(&own[round & 1][tid % VD_WARPS], tid / VD_WARPS);
+    round++;
+    __syncthreads();
+    if (warp == 0) {
+      double t = 0.;
+      for (int i = lane; i < runs; i += 32) t += all[i];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+      if (lane == 0) {
+        s_total = t;
+        if (m) sums[m] = t;
+      }
+    }
+    __syncthreads();
+  };
+  for (int have_node = -1, have_m = -1;;) {
+    if (tid == 0) {
+      // on along the tree: to its end, or to a refusal whose sum has to be known first
+      int node = s_node, m = s_m, i = s_i, count = s_count;
+      double z = s_z;
+      for (bool stop = false; i < n && !stop; i++) {
+        if (parent[i] != node) continue;
+        const double r = left_of<DRAFT>(p_of[i], q_of[i], token[i], m, sums, gone);
+        if (DRAFT) z = m ? sums[m] : 1.;
+        if ((double)uniform[i] * q_of[i] * z < r) {
+          node = i, m = 0, z = 1., path[++count] = i;
+        } else if (DRAFT) {
+          m++, stop = true;
+        } else {
+          gone[m++] = token[i], z -= r;
+        }
+      }
+      s_node = node, s_m = m, s_i = i, s_count = count, s_z = z;
+    }
+    __syncthreads();
+    if (s_node != have_node || s_m != have_m) sum_up(s_node, s_m);
+    have_node = s_node, have_m = s_m;
+    if (s_i >= n) break;
+    __syncthreads();  // before thread 0 goes on
+  }
+  const int node = s_node;
+  int m = s_m;
+  if (m && s_total == 0.) {
+    __syncthreads();
+    sum_up(node, m = 0);
+  }
+  const double border = (double)uniform[0] * s_total;
+  if (warp == 0) {
+    // the first run that reaches beyond the border, else the last one with anything in it
+    const int per = (runs + 31) / 32, from = min(runs, lane * per), to = min(runs, from + per);
+    double sum = 0.;
+    for (int i = from; i < to; i++) sum += all[i];
+    double upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double below = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += below;
+    }
+    double before = upto - sum, before_last = 0., before_found = 0.;
+    int last = -1, found = runs;
+    for (int i = from; i < to; i++) {
+      if (all[i] > 0.) {
+        last = i, before_last = before;
+        if (found == runs && before + all[i] > border) found = i, before_found = before;
+      }
+      before += all[i];
+    }
+    const int first = __reduce_min_sync(0xffffffffu, found), final = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0) s_owner = first < runs ? first : final;
+    if (first < runs ? found == first : final >= 0 && last == final) s_before = first < runs ? before_found : before_last;
+  }
+  __syncthreads();
+  if (rank == 0) {
+    for (int i = tid; i < n; i += VD_THREADS) a.path[b * n + i] = i <= s_count ? path[i] : -1;
+    if (tid == 0) a.accepted[b] = s_count;
+  }
+  const bool fine = s_total > 0. && s_total < __longlong_as_double(0x7ff0000000000000ll);
+  if (!fine || s_owner < 0) {
+    if (rank == 0 && tid == 0) a.next[b] = -1;
+  } else if (s_owner == rank * VD_WARPS + warp) {
+    const T* p = target + (int64_t)node * a.ts[1];
+    const T* q = DRAFT ? draft + (int64_t)node * a.ds[1] : nullptr;
+    auto entry = [&](int64_t v) { return left_of<DRAFT>(vd_value(p[v]), DRAFT && m ? vd_value(q[v]) : 0., v, m, sums, gone); };
+    // a lane takes consecutive entries
+    const int64_t per = (hi - lo + 31) / 32, from = min(hi, lo + lane * per), to = min(hi, from + per);
+    double sum = 0.;
+    for (int64_t v = from; v < to; v++) sum += entry(v);
+    double upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double below = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += below;
+    }
+    double run = s_before + (upto - sum);
+    long long found = a.vocab, last = -1;
+    for (int64_t v = from; v < to; v++) {
+      const double r = entry(v);
+      run += r;
+      if (r > 0.) {
+        last = v;
+        if (run > border && found == a.vocab) found = v;
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      found = min(found, __shfl_xor_sync(0xffffffffu, found, o));
+      last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+    }
+    if (lane == 0) a.next[b] = found < a.vocab ? found : last;
+  }
+  cluster_sync();  // no block leaves while another reads its sums
+}
+
+template <typename T, bool DRAFT>
+int vd_run(VdArgs a, int64_t batch, cudaStream_t s) {
+  auto kernel = verify_draft_kernel<T, DRAFT>;
+  const int smem = a.nodes * (5 * 8 + 3 * 4);
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return 1;
+  // blocks per sequence: up to two per SM, no run of fewer than 128 entries
+  int blocks = 16;
+  while (blocks > 1 && (batch * blocks > 2 * std::max(1, sm_count()) || a.vocab < (int64_t)blocks * VD_WARPS * 128)) blocks /= 2;
+  if (blocks > 8) DYN_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  a.blocks = blocks;
+  a.run = ((a.vocab + blocks * VD_WARPS - 1) / (blocks * VD_WARPS) + 31) / 32 * 32;
+  DYN_CHECK(batch * blocks <= 0x7fffffff, "verify_draft: %lld sequences are too many for one call", (long long)batch);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(batch * blocks)), cfg.blockDim = dim3(VD_THREADS), cfg.dynamicSmemBytes = (size_t)smem, cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)blocks, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  DYN_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+  count_launch();
+  return 0;
+}
+
+template <typename T>
+int vd_type(const VdArgs& a, int64_t batch, cudaStream_t s) {
+  return a.draft ? vd_run<T, true>(a, batch, s) : vd_run<T, false>(a, batch, s);
+}
+
+}  // namespace
+
+int launch_verify_draft(const int64_t* tokens, const int64_t* parents, int64_t parents_stride, const void* target,
+                        const int64_t* target_strides, const void* draft, const int64_t* draft_strides, int type,
+                        const float* uniforms, int64_t batch, int64_t nodes, int64_t vocab, int64_t* accepted, int64_t* path,
+                        int64_t* next, cudaStream_t s) {
+  if (batch == 0) return 0;
+  VdArgs a{};
+  a.tokens = tokens, a.parents = parents, a.parents_stride = parents_stride, a.target = target, a.draft = draft;
+  a.ts[0] = target_strides[0], a.ts[1] = target_strides[1];
+  if (draft) a.ds[0] = draft_strides[0], a.ds[1] = draft_strides[1];
+  a.uniforms = uniforms, a.accepted = accepted, a.path = path, a.next = next, a.nodes = (int)nodes, a.vocab = vocab;
+  if (type == E_F32) return vd_type<float>(a, batch, s);
+  if (type == E_F16) return vd_type<__half>(a, batch, s);
+  return vd_type<__nv_bfloat16>(a, batch, s);
+}
+
+}  // namespace dyn

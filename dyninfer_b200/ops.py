@@ -7,6 +7,7 @@ these functions: without the library or without a GPU they raise.
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import numpy as np
 import torch
@@ -154,6 +155,279 @@ def argmax(v: torch.Tensor) -> int:
                           device=v.device)
     check(lib().dyninfer_cuda_argmax(_p(v), v.numel(), _p(out), _p(scratch), _stream()))
     return int(out.item())
+
+
+# ---- speculative decoding: a tree of drafted tokens over a cache -----------------------------------------------------
+
+_SCALED = {torch.int8: _lib.KV["q8"], torch.float8_e4m3fn: _lib.KV["e4m3"]}
+_KV = {**_SCALED, torch.float16: ENC["plain.f16"], torch.bfloat16: ENC["plain.bf16"]}
+
+
+def _strides(count, *tensors):
+    """The first `count` strides of every tensor; a dimension of one entry is never stepped along, whatever it says."""
+    return (C.c_int64 * (count * len(tensors)))(*[step if size > 1 else 0 for t in tensors
+                                                  for size, step in zip(t.shape[:count], t.stride())])
+
+
+def _on_device(call, *tensors):
+    """`call(stream)` on the device that all the tensors are on."""
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on different devices: {device} and {t.device}")
+    if device.type != "cuda":
+        raise ValueError(f"tensors are on {device}: this target runs on a CUDA device")
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return check(call(_stream()))
+    check(call(_stream()))
+
+
+def _dense_last(what, t):
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what}: the last dimension must be dense (stride 1), not {t.stride(-1)}")
+
+
+def _shape(what, t, *shape):
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {shape}")
+
+
+def _index(what, t):
+    """Positions, lengths and token ids: dense int64 (int32 is converted)."""
+    if t.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what} must be int64, not {t.dtype}")
+    return t.to(torch.int64).contiguous()
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, layout: str = "half",
+           magnitude: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions of x [..., heads, d] (f32, f16 or bf16, up to two leading dimensions, any strides with a dense last
+    dimension): pair i of the first 2 * len(frequencies) dimensions turns by positions[...] * frequencies[i] and is multiplied by
+    `magnitude`; the other dimensions are copied. `layout` is "half" (pairs i, i + r/2) or "interleaved" (2i, 2i + 1).
+    `frequencies` is a float64 tensor in host memory (`rotary_frequencies` makes one); angles are exact modulo a turn at any
+    position. `out` may be x itself: a view of the leading heads of fused [q | k | v] rows turns q and k where they lie."""
+    if x.dtype not in _WT:
+        raise TypeError(f"x must be float32, float16 or bfloat16, not {x.dtype}")
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"layout {layout!r} is neither 'half' nor 'interleaved'")
+    if x.dim() not in (3, 4):
+        raise ValueError(f"x must be [rows, heads, d] or [batch, rows, heads, d], not {tuple(x.shape)}")
+    if frequencies.device.type != "cpu" or frequencies.dtype != torch.float64 or frequencies.dim() != 1:
+        raise ValueError("frequencies must be a one-dimensional float64 tensor in host memory")
+    _dense_last("x", x)
+    _shape("positions", positions, *x.shape[:-2])
+    positions, frequencies = _index("positions", positions), frequencies.contiguous()
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    elif out.dtype != x.dtype or out.shape != x.shape:
+        raise ValueError("out must have x's type and shape")
+    _dense_last("out", out)
+    x4, o4 = (x, out) if x.dim() == 4 else (x.unsqueeze(0), out.unsqueeze(0))
+    batch, rows, heads, d = x4.shape
+    _on_device(lambda stream: lib().dyninfer_cuda_rotary(
+        x4.data_ptr(), _WT[x.dtype], _strides(3, x4), positions.data_ptr(), frequencies.data_ptr(),
+        2 * frequencies.numel(), layout == "interleaved", float(magnitude), batch, rows, heads, d,
+        o4.data_ptr(), _strides(3, o4), stream), x, positions, out)
+    return out
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = 1e6, scaling: str = "none", factor: float = 1.0,
+                       original_length: int | None = None, low: float | None = None, high: float | None = None):
+    """(frequencies, magnitude) for `rotary`: theta^(-2i / rotary_dim), lengthened by `factor` in one of these ways.
+
+    * "none"
+    * "linear": all frequencies / factor
+    * "ntk": theta * factor^(rotary_dim / (rotary_dim - 2)): the fastest stays, the slowest is divided by factor
+    * "yarn": dimensions that turn over `high` (32) times within original_length stay, those under `low` (1) times are divided,
+      linearly in between along the dimensions; the magnitude is 0.1 ln(factor) + 1
+    * "wavelength": as yarn with `low` = 1 and `high` = 4, linearly along the number of turns, magnitude 1
+    """
+    if rotary_dim <= 0 or rotary_dim % 2 or not theta > 0 or not factor > 0:
+        raise ValueError(f"rotary_dim {rotary_dim} must be even and above zero, theta and factor above zero")
+    i = torch.arange(rotary_dim // 2, dtype=torch.float64)
+    f = theta ** (-2 * i / rotary_dim)
+    if scaling == "none":
+        return f, 1.0
+    if scaling == "linear":
+        return f / factor, 1.0
+    if scaling == "ntk":
+        if rotary_dim == 2:
+            raise ValueError("ntk scaling needs more than one pair")
+        return (theta * factor ** (rotary_dim / (rotary_dim - 2))) ** (-2 * i / rotary_dim), 1.0
+    if scaling not in ("yarn", "wavelength"):
+        raise ValueError(f"scaling {scaling!r} is not one of none, linear, ntk, yarn, wavelength")
+    if not original_length or original_length <= 0:
+        raise ValueError(f"{scaling} scaling needs original_length")
+    low, high = 1.0 if low is None else low, (32.0 if scaling == "yarn" else 4.0) if high is None else high
+    if not 0 < low < high:
+        raise ValueError(f"low {low} must be above zero and below high {high}")
+    if scaling == "yarn":
+        def dimension(turns):
+            return rotary_dim * math.log(original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        first, last = max(math.floor(dimension(high)), 0), min(math.ceil(dimension(low)), rotary_dim - 1)
+        ramp = ((i - first) / max(last - first, 0.001)).clamp(0, 1)
+        return f * (1 - ramp) + f / factor * ramp, 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+    keep = ((original_length * f / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+    return (1 - keep) * f / factor + keep * f, 1.0
+
+
+def _scaled_cache(k_cache, v_cache, k_scale, v_scale):
+    """Checks of an 8-bit cache: codes [slots, kv_heads, capacity, d], scales [slots, kv_heads, capacity]."""
+    if k_cache.dtype not in _SCALED or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"an 8-bit cache is int8 or float8_e4m3fn, not {k_cache.dtype} and {v_cache.dtype}")
+    _cache(k_cache, v_cache)
+    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if s is None or s.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32")
+        _shape(name, s, *k_cache.shape[:3])
+        _dense_last(name, s)
+
+
+def _cache(k_cache, v_cache):
+    if k_cache.dim() != 4:
+        raise ValueError(f"a cache is [slots, kv_heads, capacity, d], not {tuple(k_cache.shape)}")
+    _shape("v_cache", v_cache, *k_cache.shape)
+    _dense_last("k_cache", k_cache)
+    _dense_last("v_cache", v_cache)
+
+
+def kv_write(k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+             k_scale: torch.Tensor, v_scale: torch.Tensor, counts: torch.Tensor | None = None) -> None:
+    """Quantises k and v [slots, rows, kv_heads, d] (f32, f16 or bf16) into an 8-bit cache [slots, kv_heads, capacity, d] of
+    int8 or float8_e4m3fn codes with f32 scales [slots, kv_heads, capacity]: row r of a slot goes to cache row starts[slot] + r,
+    for r < counts[slot] where counts are given. Rows outside the cache are left out, all others of the cache as they were."""
+    if k.dtype not in _WT or v.dtype != k.dtype:
+        raise TypeError(f"k and v must both be float32, float16 or bfloat16, not {k.dtype} and {v.dtype}")
+    _scaled_cache(k_cache, v_cache, k_scale, v_scale)
+    slots, heads, cap, d = k_cache.shape
+    if k.dim() != 4:
+        raise ValueError(f"k must be [slots, rows, kv_heads, d], not {tuple(k.shape)}")
+    rows = k.shape[1]
+    _shape("k", k, slots, rows, heads, d)
+    _shape("v", v, slots, rows, heads, d)
+    _dense_last("k", k)
+    _dense_last("v", v)
+    _shape("starts", starts, slots)
+    starts = _index("starts", starts)
+    if counts is not None:
+        _shape("counts", counts, slots)
+        counts = _index("counts", counts)
+    _on_device(lambda stream: lib().dyninfer_cuda_kv_write(
+        k.data_ptr(), v.data_ptr(), _WT[k.dtype], _strides(3, k, v), k_cache.data_ptr(), v_cache.data_ptr(),
+        _KV[k_cache.dtype], _strides(3, k_cache, v_cache), k_scale.data_ptr(), v_scale.data_ptr(),
+        _strides(2, k_scale, v_scale), starts.data_ptr(), _p(counts), slots, rows, heads, d, cap, stream),
+        k, v, starts, counts, k_cache, v_cache, k_scale, v_scale)
+
+
+def kv_read(starts: torch.Tensor, rows: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+            v_scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows starts[slot] .. starts[slot] + rows - 1 of an 8-bit cache as values (k, v), each [slots, rows, kv_heads, d] of
+    `dtype`: what `kv_write` takes. Zeros for rows outside the cache."""
+    if dtype not in _WT:
+        raise TypeError(f"dtype must be float32, float16 or bfloat16, not {dtype}")
+    if rows < 0:
+        raise ValueError(f"rows must be at least zero, not {rows}")
+    _scaled_cache(k_cache, v_cache, k_scale, v_scale)
+    slots, heads, cap, d = k_cache.shape
+    _shape("starts", starts, slots)
+    starts = _index("starts", starts)
+    k, v = (torch.empty((slots, rows, heads, d), dtype=dtype, device=k_cache.device) for _ in range(2))
+    _on_device(lambda stream: lib().dyninfer_cuda_kv_read(
+        k.data_ptr(), v.data_ptr(), _WT[dtype], _strides(3, k, v), k_cache.data_ptr(), v_cache.data_ptr(),
+        _KV[k_cache.dtype], _strides(3, k_cache, v_cache), k_scale.data_ptr(), v_scale.data_ptr(),
+        _strides(2, k_scale, v_scale), starts.data_ptr(), slots, rows, heads, d, cap, stream),
+        starts, k_cache, v_cache, k_scale, v_scale)
+    return k, v
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                   mask: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+                   v_scale: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """Attention of drafted rows q [slots, rows, heads, d] (f32, f16 or bf16) over caches [slots, kv_heads, capacity, d] of f16,
+    bf16, or 8-bit codes with their scales. Row r of a slot sees keys 0 .. lengths[slot] - 1, and of the rows' own keys, which
+    stand at lengths[slot] + j, those with mask[slot, r, j] (bool, [rows, rows] for all slots or [slots, rows, rows]); without a
+    mask, those with j <= r: a chain, or the plain decode step. A row that sees nothing, or whose length is below zero, gets
+    zeros. `scale` is 1 / sqrt(d) unless given. Returns [slots, rows, heads, d] of q's type."""
+    if q.dtype not in _WT:
+        raise TypeError(f"q must be float32, float16 or bfloat16, not {q.dtype}")
+    if k_cache.dtype not in _KV or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"caches must both be float16, bfloat16, int8 or float8_e4m3fn, not {k_cache.dtype} and {v_cache.dtype}")
+    scales = None
+    if k_cache.dtype in _SCALED:
+        _scaled_cache(k_cache, v_cache, k_scale, v_scale)
+        scales = _strides(2, k_scale, v_scale)
+    else:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError(f"a cache of {k_cache.dtype} has no scales")
+        _cache(k_cache, v_cache)
+    slots, kv_heads, cap, d = k_cache.shape
+    if q.dim() != 4:
+        raise ValueError(f"q must be [slots, rows, heads, d], not {tuple(q.shape)}")
+    rows, heads = q.shape[1:3]
+    _shape("q", q, slots, rows, heads, d)
+    _dense_last("q", q)
+    _shape("lengths", lengths, slots)
+    lengths = _index("lengths", lengths)
+    masked = None
+    if mask is not None:
+        if mask.dtype != torch.bool:
+            raise TypeError(f"mask must be bool, not {mask.dtype}")
+        if mask.dim() == 2:
+            mask = mask.unsqueeze(0).expand(slots, -1, -1)
+        _shape("mask", mask, slots, rows, rows)
+        if mask.stride(-1) != 1 and rows > 1:
+            mask = mask.contiguous()
+        masked = _strides(2, mask)
+    out = torch.empty((slots, rows, heads, d), dtype=q.dtype, device=q.device)
+    _on_device(lambda stream: lib().dyninfer_cuda_tree_attention(
+        q.data_ptr(), _WT[q.dtype], _strides(3, q), k_cache.data_ptr(), v_cache.data_ptr(), _KV[k_cache.dtype],
+        _strides(3, k_cache, v_cache), _p(k_scale), _p(v_scale), scales, lengths.data_ptr(), _p(mask),
+        masked, slots, rows, heads, kv_heads, d, cap, d ** -0.5 if scale is None else float(scale), out.data_ptr(), stream),
+        q, k_cache, v_cache, lengths, mask, k_scale, v_scale)
+    return out
+
+
+def verify_draft(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tensor, uniforms: torch.Tensor,
+                 draft: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which drafted tokens stand, and the token behind them: (accepted [slots], path [slots, nodes], next [slots]), int64.
+
+    Node 0 is the text's last token; node i > 0 carries tokens[:, i] behind node parents[:, i] < i ([nodes] for all slots or
+    [slots, nodes]; any other parent: no such node). target [slots, nodes, vocab] (f32, f16 or bf16) holds the probabilities of
+    the token behind each node, draft those that a node's children were drawn from independently; without it the children are
+    distinct tokens chosen without chance. uniforms [slots, nodes] are f32 in [0, 1): node i is tried with its own, and node 0's
+    draws the last token. From node 0 on the children of the node reached are tried in order; a refusal takes the draft's
+    probabilities (without a draft, the child's entry) from what the next child or the last token is drawn from. The
+    target's distribution is kept. next is -1 where a row has no finite positive sum."""
+    if target.dim() != 3:
+        raise ValueError(f"target must be [slots, nodes, vocab], not {tuple(target.shape)}")
+    if target.dtype not in _WT:
+        raise TypeError(f"target must be float32, float16 or bfloat16, not {target.dtype}")
+    slots, nodes, vocab = target.shape
+    _shape("tokens", tokens, slots, nodes)
+    if parents.dim() == 2:
+        _shape("parents", parents, slots, nodes)
+    else:
+        _shape("parents", parents, nodes)
+    _shape("uniforms", uniforms, slots, nodes)
+    if uniforms.dtype != torch.float32:
+        raise TypeError(f"uniforms must be float32, not {uniforms.dtype}")
+    _dense_last("target", target)
+    tokens, parents, uniforms = _index("tokens", tokens), _index("parents", parents), uniforms.contiguous()
+    drafted = None
+    if draft is not None:
+        if draft.dtype != target.dtype:
+            raise TypeError(f"draft must have the target's type {target.dtype}, not {draft.dtype}")
+        _shape("draft", draft, slots, nodes, vocab)
+        _dense_last("draft", draft)
+        drafted = _strides(2, draft)
+    accepted, following = (torch.empty(slots, dtype=torch.int64, device=target.device) for _ in range(2))
+    path = torch.empty((slots, nodes), dtype=torch.int64, device=target.device)
+    _on_device(lambda stream: lib().dyninfer_cuda_verify_draft(
+        tokens.data_ptr(), parents.data_ptr(), nodes if parents.dim() == 2 else 0, target.data_ptr(), _strides(2, target),
+        _p(draft), drafted, _WT[target.dtype], uniforms.data_ptr(), slots, nodes, vocab, accepted.data_ptr(), path.data_ptr(),
+        following.data_ptr(), stream), target, tokens, parents, uniforms, draft)
+    return accepted, path, following
 
 
 def check_device_error():

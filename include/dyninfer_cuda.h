@@ -145,6 +145,83 @@ int dyninfer_cuda_argmax(const float* v_dev, int64_t n, int64_t* out_index_dev, 
 int64_t dyninfer_cuda_argmax_static_max_n(void);
 int dyninfer_cuda_argmax_static(const float* v_dev, int64_t n, int64_t* out_index_dev, void* stream);
 
+/* ---- speculative decoding (extension: the reference decodes one token at a time) ------------
+ *
+ * A step over a tree of drafted tokens: its rows are rotated to their depths, written behind the
+ * cache's rows, attended to under the tree's mask, and verified against the target. Strides are
+ * host arrays that count elements (not bytes); the last dimension is always dense. `type` is
+ * DYNINFER_ENC_F32, _F16 or _BF16. Work is asynchronous on `stream`, nothing is allocated, and
+ * nothing is kept between calls, so all five may be captured into graphs. */
+
+/* cache types besides DYNINFER_ENC_F16 / _BF16: one byte per element and one f32 scale per row */
+enum {
+  DYNINFER_KV_Q8 = 32,  /* signed whole numbers, value = code * scale */
+  DYNINFER_KV_E4M3 = 33 /* e4m3, value = code * scale (a power of two); the NaN codes read as +-480 */
+};
+
+/* Rotary positions of x [batch, rows, heads, d] (strides: batch, row, head): pair i of the first
+ * rotary_dim dimensions -- (i, i + rotary_dim / 2), or (2i, 2i + 1) when `interleaved` -- turns by
+ * positions[batch, row] * frequencies[i] and is multiplied by `magnitude`; other dimensions are
+ * copied. `frequencies` (rotary_dim / 2 values) lies in host memory and is read before the call
+ * returns; angles are exact modulo a turn for any 64-bit position. y may be x itself with the same
+ * strides, but must not overlap it otherwise. d <= 256. */
+int dyninfer_cuda_rotary(const void* x_dev, int type, const int64_t* x_strides, const int64_t* positions_dev,
+                         const double* frequencies, int64_t rotary_dim, int interleaved, double magnitude,
+                         int64_t batch, int64_t rows, int64_t heads, int64_t d, void* y_dev,
+                         const int64_t* y_strides, void* stream);
+
+/* Quantises rows of k and v [batch, rows, kv_heads, d] into an 8-bit cache: row r of batch entry b
+ * goes to cache row starts[b] + r, for r < counts[b] (counts NULL: all); rows outside the cache are
+ * left out. x_strides: batch, row, head of k, then of v. Caches are [batch, kv_heads, kv_cap, d]
+ * bytes (cache_strides: batch, head, row of k, then of v; multiples of 16), scales
+ * [batch, kv_heads, kv_cap] floats (scale_strides: batch, head of k, then of v). A row whose largest
+ * magnitude is below 2^-100 becomes zeros; one with an infinity or NaN reads back as NaN. d is a
+ * multiple of 16 up to 256. */
+int dyninfer_cuda_kv_write(const void* k_dev, const void* v_dev, int type, const int64_t* x_strides,
+                           void* k_cache_dev, void* v_cache_dev, int kv_type, const int64_t* cache_strides,
+                           float* k_scale_dev, float* v_scale_dev, const int64_t* scale_strides,
+                           const int64_t* starts_dev, const int64_t* counts_dev, int64_t batch, int64_t rows,
+                           int64_t kv_heads, int64_t d, int64_t kv_cap, void* stream);
+
+/* The reverse: rows starts[b] + r as values of `type`; zeros for rows outside the cache. */
+int dyninfer_cuda_kv_read(void* k_dev, void* v_dev, int type, const int64_t* x_strides, const void* k_cache_dev,
+                          const void* v_cache_dev, int kv_type, const int64_t* cache_strides,
+                          const float* k_scale_dev, const float* v_scale_dev, const int64_t* scale_strides,
+                          const int64_t* starts_dev, int64_t batch, int64_t rows, int64_t kv_heads, int64_t d,
+                          int64_t kv_cap, void* stream);
+
+/* Attention of q [batch, rows, heads, d] over caches [batch, kv_heads, kv_cap, d]: row r of batch
+ * entry b sees keys 0 .. lengths[b] - 1, and key lengths[b] + j (the tree's row j) where
+ * mask[b, r, j] is not zero (strides: batch, row; a batch stride of 0 shares one mask); mask NULL:
+ * where j <= r. Keys from kv_cap on do not exist; a row that sees nothing gets zeros, and so do all
+ * rows of an entry whose length is below zero. ctx [batch, rows, heads, d] is dense, of q's type.
+ * kv_type F16, BF16, or an 8-bit type with its scales (as kv_write lays them out). d is a multiple
+ * of 16 up to 128. */
+int dyninfer_cuda_tree_attention(const void* q_dev, int q_type, const int64_t* q_strides, const void* k_cache_dev,
+                                 const void* v_cache_dev, int kv_type, const int64_t* cache_strides,
+                                 const float* k_scale_dev, const float* v_scale_dev, const int64_t* scale_strides,
+                                 const int64_t* lengths_dev, const uint8_t* mask_dev, const int64_t* mask_strides,
+                                 int64_t batch, int64_t rows, int64_t heads, int64_t kv_heads, int64_t d,
+                                 int64_t kv_cap, float scale, void* ctx_dev, void* stream);
+
+/* Which drafted tokens stand, and the token behind them. Node 0 is the text's last token, node i > 0
+ * carries tokens[b, i] behind node parents[b, i] < i (any other value: the node is not there;
+ * parents_stride 0 shares one tree). target[b, i] holds the probabilities of the token behind node
+ * i, draft[b, i] those that node i's children were drawn from independently (NULL: the children were
+ * chosen without chance, distinct tokens). From node 0 on the children of the node reached are tried
+ * in order, child c against uniforms[b, c] in [0, 1): taken if uniform * q(c) * Z < r(c), where r = p
+ * and Z = 1 at first and a refusal leaves r = max(r / Z - q, 0) (without a draft: q = 1 in the test,
+ * and r loses c's entry) and Z = its sum. The token behind is the first v at which the running sum
+ * of r passes uniforms[b, 0] times its total; where nothing is left, of the target's row; -1 where
+ * that has no finite positive sum. Tokens outside the vocabulary are refused. accepted [batch] = the
+ * number of tokens taken, path [batch, nodes] = the nodes from node 0 on, then -1, next [batch] =
+ * the token. Sums are in 64 bits. Up to 1024 nodes. */
+int dyninfer_cuda_verify_draft(const int64_t* tokens_dev, const int64_t* parents_dev, int64_t parents_stride,
+                               const void* target_dev, const int64_t* target_strides, const void* draft_dev,
+                               const int64_t* draft_strides, int type, const float* uniforms_dev, int64_t batch,
+                               int64_t nodes, int64_t vocab, int64_t* accepted_dev, int64_t* path_dev,
+                               int64_t* next_dev, void* stream);
+
 /* ---- session (paged-KV ABI) ----------------------------------------------- */
 
 typedef struct dyninfer_cuda_session_t dyninfer_cuda_session_t;
