@@ -45,7 +45,7 @@ class AllocatorStatistics(C.Structure):
 
 _P = C.c_void_p
 _I64 = C.c_int64
-_S = C.POINTER(C.c_int64)   # strides, in host memory
+_S = C.c_void_p            # strides: int64 values in host memory
 PROTOTYPES = {
     "dyninfer_cuda_abi_version": (C.c_int, []),
     "dyninfer_cuda_last_error": (C.c_char_p, []),

@@ -21,6 +21,15 @@ size_t type_bytes(int t) { return t == E_F32 ? 4 : 2; }
 // Counts whose products stay far inside 64 bits
 bool sane(int64_t n) { return n >= 0 && n <= (1ll << 31) - 1; }
 
+// Strides with those of dimensions of one entry as zero: nothing is stepped along there, whatever they say.
+template <int N>
+struct Steps {
+  int64_t v[N];
+  Steps(const int64_t* of, const int64_t* extents, int dims) {
+    for (int i = 0; i < N; i++) v[i] = of && extents[i % dims] > 1 ? of[i] : 0;
+  }
+};
+
 int kv_rows(const char* what, const void* k, const void* v, int type, const int64_t* x_strides, void* k_cache, void* v_cache,
             int kv_type, const int64_t* cache_strides, float* k_scale, float* v_scale, const int64_t* scale_strides,
             const int64_t* starts, const int64_t* counts, int64_t batch, int64_t rows, int64_t heads, int64_t d, int64_t cap,
@@ -35,15 +44,18 @@ int kv_rows(const char* what, const void* k, const void* v, int type, const int6
   DYN_CHECK(aligned(k, type_bytes(type)) && aligned(v, type_bytes(type)) && aligned(k_scale, 4) && aligned(v_scale, 4) &&
                 aligned(starts, 8) && aligned(counts, 8),
             "%s: a pointer is not aligned to its type", what);
+  const int64_t of_x[3] = {batch, rows, heads}, of_cache[3] = {batch, heads, cap};
+  const Steps<6> x_steps(x_strides, of_x, 3), cache_steps(cache_strides, of_cache, 3);
+  const Steps<4> scale_steps(scale_strides, of_cache, 2);
   bool even = aligned(k_cache, 16) && aligned(v_cache, 16);
-  for (int i = 0; i < 6; i++) even = even && cache_strides[i] % 16 == 0;
+  for (int64_t step : cache_steps.v) even = even && step % 16 == 0;
   DYN_CHECK(even, "%s: caches and their strides must be multiples of 16 bytes", what);
   if (have_device()) return 1;
   KvRows r{};
   // read-only when writing; the struct serves both directions
-  r.x[0] = const_cast<void*>(k), r.x[1] = const_cast<void*>(v), r.x_strides = x_strides;
-  r.codes[0] = k_cache, r.codes[1] = v_cache, r.code_strides = cache_strides;
-  r.scales[0] = k_scale, r.scales[1] = v_scale, r.scale_strides = scale_strides;
+  r.x[0] = const_cast<void*>(k), r.x[1] = const_cast<void*>(v), r.x_strides = x_steps.v;
+  r.codes[0] = k_cache, r.codes[1] = v_cache, r.code_strides = cache_steps.v;
+  r.scales[0] = k_scale, r.scales[1] = v_scale, r.scale_strides = scale_steps.v;
   r.starts = starts, r.counts = counts, r.batch = batch, r.rows = rows, r.heads = heads, r.d = d, r.cap = cap;
   r.type = type, r.e4m3 = kv_type == DYNINFER_KV_E4M3;
   return launch_kv_rows(r, write, (cudaStream_t)stream);
@@ -71,8 +83,10 @@ int dyninfer_cuda_rotary(const void* x_dev, int type, const int64_t* x_strides, 
             "rotary: a pointer is not aligned to its type");
   for (int64_t i = 0; i < rotary_dim / 2; i++) DYN_CHECK(isfinite(frequencies[i]), "rotary: frequency %lld is not finite", (long long)i);
   if (have_device()) return 1;
-  return launch_rotary(x_dev, type, batch, rows, heads, d, x_strides, positions_dev, frequencies, rotary_dim, interleaved != 0,
-                       magnitude, y_dev, y_strides, (cudaStream_t)stream);
+  const int64_t extents[3] = {batch, rows, heads};
+  const Steps<3> x_steps(x_strides, extents, 3), y_steps(y_strides, extents, 3);
+  return launch_rotary(x_dev, type, batch, rows, heads, d, x_steps.v, positions_dev, frequencies, rotary_dim, interleaved != 0,
+                       magnitude, y_dev, y_steps.v, (cudaStream_t)stream);
 }
 
 int dyninfer_cuda_kv_write(const void* k_dev, const void* v_dev, int type, const int64_t* x_strides, void* k_cache_dev,
@@ -114,19 +128,24 @@ int dyninfer_cuda_tree_attention(const void* q_dev, int q_type, const int64_t* q
   DYN_CHECK(aligned(q_dev, type_bytes(q_type)) && aligned(lengths_dev, 8) && aligned(k_scale_dev, 4) && aligned(v_scale_dev, 4),
             "tree_attention: a pointer is not aligned to its type");
   const int64_t size = wide ? 2 : 1;
+  const int64_t of_q[3] = {batch, rows, heads}, of_cache[3] = {batch, kv_heads, kv_cap};
+  const Steps<3> q_steps(q_strides, of_q, 3);
+  const Steps<6> cache_steps(cache_strides, of_cache, 3);
+  const Steps<4> scale_steps(scale_strides, of_cache, 2);
+  const Steps<2> mask_steps(mask_strides, of_q, 2);
   bool even = aligned(k_cache_dev, 16) && aligned(v_cache_dev, 16) && aligned(ctx_dev, 16);
-  for (int i = 0; i < 6; i++) even = even && cache_strides[i] * size % 16 == 0;
+  for (int64_t step : cache_steps.v) even = even && step * size % 16 == 0;
   DYN_CHECK(even, "tree_attention: caches, their strides and the output must be multiples of 16 bytes");
   if (have_device()) return 1;
   TreeArgs a{};
   a.q = q_dev, a.out = ctx_dev, a.k = static_cast<const uint8_t*>(k_cache_dev), a.v = static_cast<const uint8_t*>(v_cache_dev);
   a.lengths = lengths_dev, a.mask = mask_dev;
-  for (int i = 0; i < 3; i++) a.qs[i] = q_strides[i], a.kst[i] = cache_strides[i] * size, a.vst[i] = cache_strides[3 + i] * size;
+  for (int i = 0; i < 3; i++) a.qs[i] = q_steps.v[i], a.kst[i] = cache_steps.v[i] * size, a.vst[i] = cache_steps.v[3 + i] * size;
   if (!wide) {
     a.ks = k_scale_dev, a.vs = v_scale_dev;
-    for (int i = 0; i < 2; i++) a.kss[i] = scale_strides[i], a.vss[i] = scale_strides[2 + i];
+    for (int i = 0; i < 2; i++) a.kss[i] = scale_steps.v[i], a.vss[i] = scale_steps.v[2 + i];
   }
-  if (mask_dev) a.ms[0] = mask_strides[0], a.ms[1] = mask_strides[1];
+  a.ms[0] = mask_steps.v[0], a.ms[1] = mask_steps.v[1];
   a.batch = batch, a.cap = kv_cap, a.rows = (int)rows, a.heads = (int)heads, a.kv_heads = (int)kv_heads;
   a.group = (int)(heads / kv_heads), a.d = (int)d, a.scale = scale;
   const cudaStream_t s = (cudaStream_t)stream;

@@ -13,8 +13,8 @@
 // Whether a child is taken depends on single entries, which are fetched for all nodes at once; what costs is one pass over a
 // row of target (and draft) per refusal, about 1.2 MB for 150000 entries, so memory and latency bound it. A cluster of up to 16
 // blocks takes a sequence, every warp a run of entries; the warps' sums meet through shared memory, in one order everywhere, so
-// that all blocks walk the tree alike without asking one another. The sums are also what the draw searches: the warp
-// whose run holds the border looks through its own run once more, out of the caches.
+// that all blocks walk the tree alike without asking one another. The sums are also what the draw searches: the block
+// whose warp had the border in its run looks through that run once more, out of the caches.
 #include <algorithm>
 
 #include "common.cuh"
@@ -24,7 +24,7 @@ namespace dyn {
 
 namespace {
 
-constexpr int VD_THREADS = 512, VD_WARPS = VD_THREADS / 32, VD_LOADS = 8;
+constexpr int VD_THREADS = 512, VD_WARPS = VD_THREADS / 32;
 
 struct VdArgs {
   const int64_t *tokens, *parents;  // [batch][nodes]
@@ -52,16 +52,18 @@ __device__ __forceinline__ double vd_value(float x) { return x; }
 __device__ __forceinline__ double vd_value(__half x) { return __half2float(x); }
 __device__ __forceinline__ double vd_value(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// What is left of entry v (p and q: the rows' entries) after m refusals at the node, with the sums in between and the tokens
-// that are `gone`.
+// What is left of entry v (p and q: the rows' entries) after m refusals at the node, with `inv[j]` one over the sum behind the
+// j-th (0 where nothing was left) and the tokens that are `gone`.
 template <bool DRAFT>
-__device__ __forceinline__ double left_of(double p, double q, int64_t v, int m, const double* sums, const int64_t* gone) {
+__device__ __forceinline__ double left_of(double p, double q, int64_t v, int m, const double* inv, const int64_t* gone) {
   if (DRAFT) {
+#pragma unroll 1
     for (int j = 0; j < m; j++) {
-      p = (j ? (sums[j] > 0. ? p / sums[j] : 0.) : p) - q;
+      p = (j ? p * inv[j] : p) - q;
       p = p < 0. ? 0. : p;  // NaN stays NaN
     }
   } else {
+#pragma unroll 1
     for (int j = 0; j < m; j++)
       if (gone[j] == v) p = 0.;
   }
@@ -69,17 +71,18 @@ __device__ __forceinline__ double left_of(double p, double q, int64_t v, int m, 
 }
 
 template <typename T, bool DRAFT>
-__global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(const __grid_constant__ VdArgs a) {
+__global__ void __launch_bounds__(VD_THREADS, 2) verify_draft_kernel(const __grid_constant__ VdArgs a) {
   extern __shared__ double vd_shared[];
   double* p_of = vd_shared;                 // [nodes] target's entry of the node's token in its parent's row
   double* q_of = p_of + a.nodes;            // [nodes] the draft's
-  double* sums = q_of + a.nodes;            // [nodes] Z_m at the present node
-  int64_t* token = reinterpret_cast<int64_t*>(sums + a.nodes);
+  double* inv = q_of + a.nodes;             // [nodes] 1 / Z_m at the present node
+  int64_t* token = reinterpret_cast<int64_t*>(inv + a.nodes);
   int64_t* gone = token + a.nodes;          // tokens refused at the present node
   float* uniform = reinterpret_cast<float*>(gone + a.nodes);
   int* parent = reinterpret_cast<int*>(uniform + a.nodes);
   int* path = parent + a.nodes;
-  __shared__ double own[2][VD_WARPS], all[16 * VD_WARPS];
+  __shared__ double own[2][VD_WARPS], all[16 * VD_WARPS], part[VD_WARPS];
+  __shared__ long long s_found, s_last;
   __shared__ int s_node, s_m, s_i, s_count, s_owner;  // where the walk stands; whose run holds the drawn token
   __shared__ double s_total, s_z, s_before;
 
@@ -97,29 +100,77 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(const __grid_c
     p_of[i] = known ? vd_value(target[up * a.ts[1] + t]) : 0.;
     q_of[i] = known ? (DRAFT ? vd_value(draft[up * a.ds[1] + t]) : 1.) : 0.;
   }
-  if (tid == 0) s_node = 0, s_m = 0, s_i = 1, s_count = 0, s_z = 1., sums[0] = 1., path[0] = 0;
+  if (tid == 0) s_node = 0, s_m = 0, s_i = 1, s_count = 0, s_z = 1., path[0] = 0;
   __syncthreads();
 
   const int64_t lo = min(a.vocab, ((int64_t)rank * VD_WARPS + warp) * a.run), hi = min(a.vocab, lo + a.run);
   const int runs = a.blocks * VD_WARPS;
   int round = 0;
+  constexpr int N = 16 / sizeof(T), LOADS = 16 / N;
+  struct alignas(16) Piece {
+    T v[N];
+  };
+  // N entries' r after m refusals of drawn children
+  auto all_left = [&](const T* pv, const T* qv, int m, double* r) {
+#pragma unroll
+    for (int e = 0; e < N; e++) r[e] = vd_value(pv[e]);
+    for (int j = 0; j < m; j++) {
+      const double by = j ? inv[j] : 1.;
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        r[e] = r[e] * by - vd_value(qv[e]);
+        r[e] = r[e] < 0. ? 0. : r[e];  // NaN stays NaN
+      }
+    }
+  };
   // all[] = every warp's sum of what is left at `node` after m refusals, s_total = their sum: the same in all blocks
   auto sum_up = [&](int node, int m) {
     const T* p = target + (int64_t)node * a.ts[1];
     const T* q = DRAFT ? draft + (int64_t)node * a.ds[1] : nullptr;
     double sum = 0.;
-    for (int64_t v = lo + lane; v < hi; v += 32 * VD_LOADS) {
-      T pe[VD_LOADS], qe[VD_LOADS];
+    // 16 bytes at a time from the boundary below the run's first entry on; what lies outside the run, and q where it is not
+    // aligned as p is, by single entries
+    const int64_t base = lo - (int64_t)(reinterpret_cast<uintptr_t>(p + lo) % 16 / sizeof(T));
+    bool touched = false;  // without a draft: one of the refused tokens is this warp's
+    for (int j = 0; !DRAFT && j < m; j++) touched = touched || (gone[j] >= lo && gone[j] < hi);
+    const bool alike = !DRAFT || (reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(q)) % 16 == 0;
+    for (int64_t v0 = base + lane * N; v0 < hi; v0 += 32 * N * LOADS) {
+      Piece pe[LOADS] = {}, qe[LOADS] = {};
 #pragma unroll
-      for (int j = 0; j < VD_LOADS; j++)
-        if (v + j * 32 < hi) {
-          pe[j] = p[v + j * 32];
-          if (DRAFT && m) qe[j] = q[v + j * 32];
+      for (int j = 0; j < LOADS; j++) {
+        const int64_t v = v0 + j * 32 * N;
+        if (v >= lo && v + N <= hi) {
+          pe[j] = *reinterpret_cast<const Piece*>(p + v);
+          if (DRAFT && m && alike) qe[j] = *reinterpret_cast<const Piece*>(q + v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; e++)
+            if (v + e >= lo && v + e < hi) {
+              pe[j].v[e] = p[v + e];
+              if (DRAFT && m && alike) qe[j].v[e] = q[v + e];
+            }
         }
+        if (DRAFT && m && !alike) {
 #pragma unroll
-      for (int j = 0; j < VD_LOADS; j++)
-        if (v + j * 32 < hi)
-          sum += left_of<DRAFT>(vd_value(pe[j]), DRAFT && m ? vd_value(qe[j]) : 0., v + j * 32, m, sums, gone);
+          for (int e = 0; e < N; e++)
+            if (v + e >= lo && v + e < hi) qe[j].v[e] = q[v + e];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < LOADS; j++) {
+        if (!DRAFT && touched) {
+          for (int g = 0; g < m; g++) {
+            const int64_t at = gone[g] - (v0 + j * 32 * N);
+#pragma unroll
+            for (int e = 0; e < N; e++)
+              if (at == e) pe[j].v[e] = T(0.f);
+          }
+        }
+        double r[N];
+        all_left(pe[j].v, qe[j].v, DRAFT ? m : 0, r);
+#pragma unroll
+        for (int e = 0; e < N; e++) sum += r[e];
+      }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -136,35 +187,45 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(const __grid_c
       for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
       if (lane == 0) {
         s_total = t;
-        if (m) sums[m] = t;
+        if (m) inv[m] = t > 0. ? 1. / t : 0., s_z = t;
       }
     }
     __syncthreads();
   };
   for (int have_node = -1, have_m = -1;;) {
-    if (tid == 0) {
-      // on along the tree: to its end, or to a refusal whose sum has to be known first
+    if (warp == 0) {
+      // on along the tree: to its end, or to a refusal whose sum has to be known first. 32 nodes at a time are looked through
+      // for children of the one reached; all lanes try the same child
       int node = s_node, m = s_m, i = s_i, count = s_count;
       double z = s_z;
-      for (bool stop = false; i < n && !stop; i++) {
-        if (parent[i] != node) continue;
-        const double r = left_of<DRAFT>(p_of[i], q_of[i], token[i], m, sums, gone);
-        if (DRAFT) z = m ? sums[m] : 1.;
-        if ((double)uniform[i] * q_of[i] * z < r) {
-          node = i, m = 0, z = 1., path[++count] = i;
+      for (bool stop = false; i < n && !stop;) {
+        const int at = (i & ~31) + lane;
+        const uint32_t children = __ballot_sync(0xffffffffu, at >= i && at < n && parent[at] == node);
+        if (!children) {
+          i = (i & ~31) + 32;
+          continue;
+        }
+        const int c = (i & ~31) + __ffs(children) - 1;
+        i = c + 1;
+        const double r = left_of<DRAFT>(p_of[c], q_of[c], token[c], m, inv, gone);
+        if ((double)uniform[c] * q_of[c] * z < r) {
+          node = c, m = 0, z = 1., count++;
+          if (lane == 0) path[count] = c;
         } else if (DRAFT) {
           m++, stop = true;
         } else {
-          gone[m++] = token[i], z -= r;
+          if (lane == 0) gone[m] = token[c];
+          __syncwarp();
+          m++, z -= r;
         }
       }
-      s_node = node, s_m = m, s_i = i, s_count = count, s_z = z;
+      if (lane == 0) s_node = node, s_m = m, s_i = i, s_count = count, s_z = z;
     }
     __syncthreads();
     if (s_node != have_node || s_m != have_m) sum_up(s_node, s_m);
     have_node = s_node, have_m = s_m;
     if (s_i >= n) break;
-    __syncthreads();  // before thread 0 goes on
+    __syncthreads();  // before the first warp goes on
   }
   const int node = s_node;
   int m = s_m;
@@ -205,28 +266,56 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(const __grid_c
   const bool fine = s_total > 0. && s_total < __longlong_as_double(0x7ff0000000000000ll);
   if (!fine || s_owner < 0) {
     if (rank == 0 && tid == 0) a.next[b] = -1;
-  } else if (s_owner == rank * VD_WARPS + warp) {
+  } else if (s_owner / VD_WARPS == rank) {
+    // the run's entries once more, over all warps of its block; a lane takes consecutive ones
     const T* p = target + (int64_t)node * a.ts[1];
     const T* q = DRAFT ? draft + (int64_t)node * a.ds[1] : nullptr;
-    auto entry = [&](int64_t v) { return left_of<DRAFT>(vd_value(p[v]), DRAFT && m ? vd_value(q[v]) : 0., v, m, sums, gone); };
-    // a lane takes consecutive entries
-    const int64_t per = (hi - lo + 31) / 32, from = min(hi, lo + lane * per), to = min(hi, from + per);
+    const int64_t begin = min(a.vocab, (int64_t)s_owner * a.run), end = min(a.vocab, begin + a.run);
+    const int64_t per = (end - begin + VD_THREADS - 1) / VD_THREADS, from = min(end, begin + tid * per), to = min(end, from + per);
+    auto entries = [&](int64_t v, double* r) {  // of v .. v + N - 1, zero from `to` on
+      T pv[N] = {}, qv[N] = {};
+#pragma unroll
+      for (int e = 0; e < N; e++)
+        if (v + e < to) {
+          pv[e] = p[v + e];
+          if (DRAFT && m) qv[e] = q[v + e];
+        }
+      for (int g = 0; !DRAFT && g < m; g++) {
+#pragma unroll
+        for (int e = 0; e < N; e++)
+          if (gone[g] - v == e) pv[e] = T(0.f);
+      }
+      all_left(pv, qv, DRAFT ? m : 0, r);
+    };
     double sum = 0.;
-    for (int64_t v = from; v < to; v++) sum += entry(v);
+    for (int64_t v = from; v < to; v += N) {
+      double r[N];
+      entries(v, r);
+#pragma unroll
+      for (int e = 0; e < N; e++) sum += r[e];
+    }
     double upto = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double below = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += below;
     }
+    if (lane == 31) part[warp] = upto;
+    if (tid == 0) s_found = a.vocab, s_last = -1;
+    __syncthreads();
     double run = s_before + (upto - sum);
+    for (int w = 0; w < warp; w++) run += part[w];
     long long found = a.vocab, last = -1;
-    for (int64_t v = from; v < to; v++) {
-      const double r = entry(v);
-      run += r;
-      if (r > 0.) {
-        last = v;
-        if (run > border && found == a.vocab) found = v;
+    for (int64_t v = from; v < to; v += N) {
+      double r[N];
+      entries(v, r);
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        run += r[e];
+        if (r[e] > 0.) {
+          last = v + e;
+          if (run > border && found == a.vocab) found = v + e;
+        }
       }
     }
 #pragma unroll
@@ -234,7 +323,9 @@ __global__ void __launch_bounds__(VD_THREADS) verify_draft_kernel(const __grid_c
       found = min(found, __shfl_xor_sync(0xffffffffu, found, o));
       last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
     }
-    if (lane == 0) a.next[b] = found < a.vocab ? found : last;
+    if (lane == 0) atomicMin(&s_found, found), atomicMax(&s_last, last);
+    __syncthreads();
+    if (tid == 0) a.next[b] = s_found < a.vocab ? s_found : s_last;  // rounding may leave the border beyond the last sum
   }
   cluster_sync();  // no block leaves while another reads its sums
 }

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
 import numpy as np
 import torch
@@ -163,39 +164,51 @@ _SCALED = {torch.int8: _lib.KV["q8"], torch.float8_e4m3fn: _lib.KV["e4m3"]}
 _KV = {**_SCALED, torch.float16: ENC["plain.f16"], torch.bfloat16: ENC["plain.bf16"]}
 
 
-def _strides(count, *tensors):
-    """The first `count` strides of every tensor; a dimension of one entry is never stepped along, whatever it says."""
-    return (C.c_int64 * (count * len(tensors)))(*[step if size > 1 else 0 for t in tensors
-                                                  for size, step in zip(t.shape[:count], t.stride())])
+# Host-side work is most of a small call's time, so the checks below keep to plain comparisons: strides travel as packed
+# bytes (0.3 us; a ctypes array is 1.2), devices are compared by index, dense int64 tensors are not touched.
+_pack2, _pack3, _pack4, _pack6 = (struct.Struct(f"{n}q").pack for n in (2, 3, 4, 6))
 
 
-def _on_device(call, *tensors):
-    """`call(stream)` on the device that all the tensors are on."""
-    device = tensors[0].device
+def _devices(*tensors):
+    """The device that all the tensors are on."""
+    at = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors on different devices: {device} and {t.device}")
-    if device.type != "cuda":
-        raise ValueError(f"tensors are on {device}: this target runs on a CUDA device")
-    if device.index != torch.cuda.current_device():
+        if t is not None and t.get_device() != at:
+            raise ValueError(f"tensors on different devices: {tensors[0].device} and {t.device}")
+    if at < 0:
+        raise ValueError(f"tensors are on {tensors[0].device}: this target runs on a CUDA device")
+    return at
+
+
+def _here():
+    return _raw_device() if _raw_device is not None else torch.cuda.current_device()
+
+
+def _run(device, call, *args):
+    """call(*args, stream) on a device, which may be another than the current one."""
+    if device == _here():
+        if call(*args, _stream()):
+            check(1)
+    else:
         with torch.cuda.device(device):
-            return check(call(_stream()))
-    check(call(_stream()))
+            check(call(*args, _stream()))
 
 
 def _dense_last(what, t):
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{what}: the last dimension must be dense (stride 1), not {t.stride(-1)}")
 
 
-def _shape(what, t, *shape):
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {shape}")
+def _shape(what, t, shape):
+    if t.shape != shape:
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
 
 
 def _index(what, t):
     """Positions, lengths and token ids: dense int64 (int32 is converted)."""
-    if t.dtype not in (torch.int64, torch.int32):
+    if t.dtype is torch.int64:
+        return t if t.is_contiguous() else t.contiguous()
+    if t.dtype is not torch.int32:
         raise TypeError(f"{what} must be int64, not {t.dtype}")
     return t.to(torch.int64).contiguous()
 
@@ -207,28 +220,36 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     `magnitude`; the other dimensions are copied. `layout` is "half" (pairs i, i + r/2) or "interleaved" (2i, 2i + 1).
     `frequencies` is a float64 tensor in host memory (`rotary_frequencies` makes one); angles are exact modulo a turn at any
     position. `out` may be x itself: a view of the leading heads of fused [q | k | v] rows turns q and k where they lie."""
-    if x.dtype not in _WT:
+    kind = _WT.get(x.dtype)
+    if kind is None:
         raise TypeError(f"x must be float32, float16 or bfloat16, not {x.dtype}")
-    if layout not in ("half", "interleaved"):
+    if layout != "half" and layout != "interleaved":
         raise ValueError(f"layout {layout!r} is neither 'half' nor 'interleaved'")
-    if x.dim() not in (3, 4):
-        raise ValueError(f"x must be [rows, heads, d] or [batch, rows, heads, d], not {tuple(x.shape)}")
-    if frequencies.device.type != "cpu" or frequencies.dtype != torch.float64 or frequencies.dim() != 1:
+    shape = x.shape
+    if len(shape) == 3:
+        (rows, heads, d), batch = shape, 1
+    elif len(shape) == 4:
+        batch, rows, heads, d = shape
+    else:
+        raise ValueError(f"x must be [rows, heads, d] or [batch, rows, heads, d], not {tuple(shape)}")
+    if frequencies.is_cuda or frequencies.dtype is not torch.float64 or frequencies.dim() != 1:
         raise ValueError("frequencies must be a one-dimensional float64 tensor in host memory")
     _dense_last("x", x)
-    _shape("positions", positions, *x.shape[:-2])
-    positions, frequencies = _index("positions", positions), frequencies.contiguous()
+    _shape("positions", positions, shape[:-2])
+    positions = _index("positions", positions)
+    if not frequencies.is_contiguous():
+        frequencies = frequencies.contiguous()
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif out.dtype != x.dtype or out.shape != x.shape:
+        out = x.new_empty(shape)
+    elif out.dtype != x.dtype or out.shape != shape:
         raise ValueError("out must have x's type and shape")
     _dense_last("out", out)
-    x4, o4 = (x, out) if x.dim() == 4 else (x.unsqueeze(0), out.unsqueeze(0))
-    batch, rows, heads, d = x4.shape
-    _on_device(lambda stream: lib().dyninfer_cuda_rotary(
-        x4.data_ptr(), _WT[x.dtype], _strides(3, x4), positions.data_ptr(), frequencies.data_ptr(),
-        2 * frequencies.numel(), layout == "interleaved", float(magnitude), batch, rows, heads, d,
-        o4.data_ptr(), _strides(3, o4), stream), x, positions, out)
+    sx, so = x.stride(), out.stride()
+    if batch == 1:      # a dimension of one entry is not stepped along, whatever its stride says
+        sx, so = (0, *sx[-3:]), (0, *so[-3:])
+    _run(_devices(x, positions, out), lib().dyninfer_cuda_rotary, x.data_ptr(), kind, _pack3(sx[0], sx[1], sx[2]),
+         positions.data_ptr(), frequencies.data_ptr(), 2 * frequencies.numel(), layout == "interleaved", magnitude, batch, rows,
+         heads, d, out.data_ptr(), _pack3(so[0], so[1], so[2]))
     return out
 
 
@@ -272,24 +293,33 @@ def rotary_frequencies(rotary_dim: int, theta: float = 1e6, scaling: str = "none
     return (1 - keep) * f / factor + keep * f, 1.0
 
 
-def _scaled_cache(k_cache, v_cache, k_scale, v_scale):
-    """Checks of an 8-bit cache: codes [slots, kv_heads, capacity, d], scales [slots, kv_heads, capacity]."""
-    if k_cache.dtype not in _SCALED or v_cache.dtype != k_cache.dtype:
-        raise TypeError(f"an 8-bit cache is int8 or float8_e4m3fn, not {k_cache.dtype} and {v_cache.dtype}")
-    _cache(k_cache, v_cache)
-    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if s is None or s.dtype != torch.float32:
-            raise TypeError(f"{name} must be float32")
-        _shape(name, s, *k_cache.shape[:3])
-        _dense_last(name, s)
-
-
 def _cache(k_cache, v_cache):
     if k_cache.dim() != 4:
         raise ValueError(f"a cache is [slots, kv_heads, capacity, d], not {tuple(k_cache.shape)}")
-    _shape("v_cache", v_cache, *k_cache.shape)
+    _shape("v_cache", v_cache, k_cache.shape)
     _dense_last("k_cache", k_cache)
     _dense_last("v_cache", v_cache)
+    k, v = k_cache.stride(), v_cache.stride()
+    return _pack6(k[0], k[1], k[2], v[0], v[1], v[2])
+
+
+def _scales(k_cache, k_scale, v_scale):
+    """Scales [slots, kv_heads, capacity] of an 8-bit cache's rows."""
+    shape = k_cache.shape[:3]
+    for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if scale is None or scale.dtype is not torch.float32:
+            raise TypeError(f"{name} must be float32")
+        _shape(name, scale, shape)
+        _dense_last(name, scale)
+    k, v = k_scale.stride(), v_scale.stride()
+    return _pack4(k[0], k[1], v[0], v[1])
+
+
+def _scaled_kind(k_cache, v_cache):
+    kind = _SCALED.get(k_cache.dtype)
+    if kind is None or v_cache.dtype != k_cache.dtype:
+        raise TypeError(f"an 8-bit cache is int8 or float8_e4m3fn, not {k_cache.dtype} and {v_cache.dtype}")
+    return kind
 
 
 def kv_write(k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -297,47 +327,49 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, k_cache: to
     """Quantises k and v [slots, rows, kv_heads, d] (f32, f16 or bf16) into an 8-bit cache [slots, kv_heads, capacity, d] of
     int8 or float8_e4m3fn codes with f32 scales [slots, kv_heads, capacity]: row r of a slot goes to cache row starts[slot] + r,
     for r < counts[slot] where counts are given. Rows outside the cache are left out, all others of the cache as they were."""
-    if k.dtype not in _WT or v.dtype != k.dtype:
+    kind = _WT.get(k.dtype)
+    if kind is None or v.dtype != k.dtype:
         raise TypeError(f"k and v must both be float32, float16 or bfloat16, not {k.dtype} and {v.dtype}")
-    _scaled_cache(k_cache, v_cache, k_scale, v_scale)
+    cache = _scaled_kind(k_cache, v_cache)
+    steps, scale_steps = _cache(k_cache, v_cache), _scales(k_cache, k_scale, v_scale)
     slots, heads, cap, d = k_cache.shape
     if k.dim() != 4:
         raise ValueError(f"k must be [slots, rows, kv_heads, d], not {tuple(k.shape)}")
     rows = k.shape[1]
-    _shape("k", k, slots, rows, heads, d)
-    _shape("v", v, slots, rows, heads, d)
+    _shape("k", k, (slots, rows, heads, d))
+    _shape("v", v, k.shape)
     _dense_last("k", k)
     _dense_last("v", v)
-    _shape("starts", starts, slots)
+    _shape("starts", starts, (slots,))
     starts = _index("starts", starts)
     if counts is not None:
-        _shape("counts", counts, slots)
+        _shape("counts", counts, (slots,))
         counts = _index("counts", counts)
-    _on_device(lambda stream: lib().dyninfer_cuda_kv_write(
-        k.data_ptr(), v.data_ptr(), _WT[k.dtype], _strides(3, k, v), k_cache.data_ptr(), v_cache.data_ptr(),
-        _KV[k_cache.dtype], _strides(3, k_cache, v_cache), k_scale.data_ptr(), v_scale.data_ptr(),
-        _strides(2, k_scale, v_scale), starts.data_ptr(), _p(counts), slots, rows, heads, d, cap, stream),
-        k, v, starts, counts, k_cache, v_cache, k_scale, v_scale)
+    sk, sv = k.stride(), v.stride()
+    _run(_devices(k, v, starts, counts, k_cache, v_cache, k_scale, v_scale), lib().dyninfer_cuda_kv_write, k.data_ptr(), v.data_ptr(),
+         kind, _pack6(sk[0], sk[1], sk[2], sv[0], sv[1], sv[2]), k_cache.data_ptr(), v_cache.data_ptr(), cache, steps,
+         k_scale.data_ptr(), v_scale.data_ptr(), scale_steps, starts.data_ptr(), _p(counts), slots, rows, heads, d, cap)
 
 
 def kv_read(starts: torch.Tensor, rows: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
             v_scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows starts[slot] .. starts[slot] + rows - 1 of an 8-bit cache as values (k, v), each [slots, rows, kv_heads, d] of
     `dtype`: what `kv_write` takes. Zeros for rows outside the cache."""
-    if dtype not in _WT:
+    kind = _WT.get(dtype)
+    if kind is None:
         raise TypeError(f"dtype must be float32, float16 or bfloat16, not {dtype}")
     if rows < 0:
         raise ValueError(f"rows must be at least zero, not {rows}")
-    _scaled_cache(k_cache, v_cache, k_scale, v_scale)
+    cache = _scaled_kind(k_cache, v_cache)
+    steps, scale_steps = _cache(k_cache, v_cache), _scales(k_cache, k_scale, v_scale)
     slots, heads, cap, d = k_cache.shape
-    _shape("starts", starts, slots)
+    _shape("starts", starts, (slots,))
     starts = _index("starts", starts)
-    k, v = (torch.empty((slots, rows, heads, d), dtype=dtype, device=k_cache.device) for _ in range(2))
-    _on_device(lambda stream: lib().dyninfer_cuda_kv_read(
-        k.data_ptr(), v.data_ptr(), _WT[dtype], _strides(3, k, v), k_cache.data_ptr(), v_cache.data_ptr(),
-        _KV[k_cache.dtype], _strides(3, k_cache, v_cache), k_scale.data_ptr(), v_scale.data_ptr(),
-        _strides(2, k_scale, v_scale), starts.data_ptr(), slots, rows, heads, d, cap, stream),
-        starts, k_cache, v_cache, k_scale, v_scale)
+    k, v = k_cache.new_empty((2, slots, rows, heads, d), dtype=dtype).unbind(0)
+    sk = rows * heads * d, heads * d, d
+    _run(_devices(k, starts, k_cache, v_cache, k_scale, v_scale), lib().dyninfer_cuda_kv_read, k.data_ptr(), v.data_ptr(), kind,
+         _pack6(*sk, *sk), k_cache.data_ptr(), v_cache.data_ptr(), cache, steps, k_scale.data_ptr(), v_scale.data_ptr(), scale_steps,
+         starts.data_ptr(), slots, rows, heads, d, cap)
     return k, v
 
 
@@ -349,42 +381,40 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     stand at lengths[slot] + j, those with mask[slot, r, j] (bool, [rows, rows] for all slots or [slots, rows, rows]); without a
     mask, those with j <= r: a chain, or the plain decode step. A row that sees nothing, or whose length is below zero, gets
     zeros. `scale` is 1 / sqrt(d) unless given. Returns [slots, rows, heads, d] of q's type."""
-    if q.dtype not in _WT:
+    kind, cache = _WT.get(q.dtype), _KV.get(k_cache.dtype)
+    if kind is None:
         raise TypeError(f"q must be float32, float16 or bfloat16, not {q.dtype}")
-    if k_cache.dtype not in _KV or v_cache.dtype != k_cache.dtype:
+    if cache is None or v_cache.dtype != k_cache.dtype:
         raise TypeError(f"caches must both be float16, bfloat16, int8 or float8_e4m3fn, not {k_cache.dtype} and {v_cache.dtype}")
-    scales = None
-    if k_cache.dtype in _SCALED:
-        _scaled_cache(k_cache, v_cache, k_scale, v_scale)
-        scales = _strides(2, k_scale, v_scale)
-    else:
-        if k_scale is not None or v_scale is not None:
-            raise ValueError(f"a cache of {k_cache.dtype} has no scales")
-        _cache(k_cache, v_cache)
+    steps, scale_steps = _cache(k_cache, v_cache), None
+    if cache >= _lib.KV["q8"]:
+        scale_steps = _scales(k_cache, k_scale, v_scale)
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError(f"a cache of {k_cache.dtype} has no scales")
     slots, kv_heads, cap, d = k_cache.shape
     if q.dim() != 4:
         raise ValueError(f"q must be [slots, rows, heads, d], not {tuple(q.shape)}")
-    rows, heads = q.shape[1:3]
-    _shape("q", q, slots, rows, heads, d)
+    shape = q.shape
+    _, rows, heads, _ = shape
+    _shape("q", q, (slots, rows, heads, d))
     _dense_last("q", q)
-    _shape("lengths", lengths, slots)
+    _shape("lengths", lengths, (slots,))
     lengths = _index("lengths", lengths)
     masked = None
     if mask is not None:
-        if mask.dtype != torch.bool:
+        if mask.dtype is not torch.bool:
             raise TypeError(f"mask must be bool, not {mask.dtype}")
-        if mask.dim() == 2:
-            mask = mask.unsqueeze(0).expand(slots, -1, -1)
-        _shape("mask", mask, slots, rows, rows)
+        shared = mask.dim() == 2
+        _shape("mask", mask, (rows, rows) if shared else (slots, rows, rows))
         if mask.stride(-1) != 1 and rows > 1:
             mask = mask.contiguous()
-        masked = _strides(2, mask)
-    out = torch.empty((slots, rows, heads, d), dtype=q.dtype, device=q.device)
-    _on_device(lambda stream: lib().dyninfer_cuda_tree_attention(
-        q.data_ptr(), _WT[q.dtype], _strides(3, q), k_cache.data_ptr(), v_cache.data_ptr(), _KV[k_cache.dtype],
-        _strides(3, k_cache, v_cache), _p(k_scale), _p(v_scale), scales, lengths.data_ptr(), _p(mask),
-        masked, slots, rows, heads, kv_heads, d, cap, d ** -0.5 if scale is None else float(scale), out.data_ptr(), stream),
-        q, k_cache, v_cache, lengths, mask, k_scale, v_scale)
+        masked = _pack2(0 if shared else mask.stride(0), mask.stride(-2))
+    out = q.new_empty(shape)
+    sq = q.stride()
+    _run(_devices(q, k_cache, v_cache, lengths, mask, k_scale, v_scale), lib().dyninfer_cuda_tree_attention, q.data_ptr(), kind,
+         _pack3(sq[0], sq[1], sq[2]), k_cache.data_ptr(), v_cache.data_ptr(), cache, steps, _p(k_scale), _p(v_scale), scale_steps,
+         lengths.data_ptr(), _p(mask), masked, slots, rows, heads, kv_heads, d, cap, d ** -0.5 if scale is None else scale,
+         out.data_ptr())
     return out
 
 
@@ -401,32 +431,33 @@ def verify_draft(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tens
     target's distribution is kept. next is -1 where a row has no finite positive sum."""
     if target.dim() != 3:
         raise ValueError(f"target must be [slots, nodes, vocab], not {tuple(target.shape)}")
-    if target.dtype not in _WT:
+    kind = _WT.get(target.dtype)
+    if kind is None:
         raise TypeError(f"target must be float32, float16 or bfloat16, not {target.dtype}")
     slots, nodes, vocab = target.shape
-    _shape("tokens", tokens, slots, nodes)
-    if parents.dim() == 2:
-        _shape("parents", parents, slots, nodes)
-    else:
-        _shape("parents", parents, nodes)
-    _shape("uniforms", uniforms, slots, nodes)
-    if uniforms.dtype != torch.float32:
+    each = (slots, nodes)
+    _shape("tokens", tokens, each)
+    shared = parents.dim() == 1
+    _shape("parents", parents, (nodes,) if shared else each)
+    _shape("uniforms", uniforms, each)
+    if uniforms.dtype is not torch.float32:
         raise TypeError(f"uniforms must be float32, not {uniforms.dtype}")
     _dense_last("target", target)
-    tokens, parents, uniforms = _index("tokens", tokens), _index("parents", parents), uniforms.contiguous()
+    tokens, parents = _index("tokens", tokens), _index("parents", parents)
+    if not uniforms.is_contiguous():
+        uniforms = uniforms.contiguous()
     drafted = None
     if draft is not None:
         if draft.dtype != target.dtype:
             raise TypeError(f"draft must have the target's type {target.dtype}, not {draft.dtype}")
-        _shape("draft", draft, slots, nodes, vocab)
+        _shape("draft", draft, (slots, nodes, vocab))
         _dense_last("draft", draft)
-        drafted = _strides(2, draft)
-    accepted, following = (torch.empty(slots, dtype=torch.int64, device=target.device) for _ in range(2))
-    path = torch.empty((slots, nodes), dtype=torch.int64, device=target.device)
-    _on_device(lambda stream: lib().dyninfer_cuda_verify_draft(
-        tokens.data_ptr(), parents.data_ptr(), nodes if parents.dim() == 2 else 0, target.data_ptr(), _strides(2, target),
-        _p(draft), drafted, _WT[target.dtype], uniforms.data_ptr(), slots, nodes, vocab, accepted.data_ptr(), path.data_ptr(),
-        following.data_ptr(), stream), target, tokens, parents, uniforms, draft)
+        drafted = _pack2(draft.stride(0), draft.stride(1))
+    path = tokens.new_empty(each)
+    accepted, following = tokens.new_empty(slots), tokens.new_empty(slots)
+    _run(_devices(target, tokens, parents, uniforms, draft), lib().dyninfer_cuda_verify_draft, tokens.data_ptr(), parents.data_ptr(),
+         0 if shared else nodes, target.data_ptr(), _pack2(target.stride(0), target.stride(1)), _p(draft), drafted, kind,
+         uniforms.data_ptr(), slots, nodes, vocab, accepted.data_ptr(), path.data_ptr(), following.data_ptr())
     return accepted, path, following
 
 

@@ -120,7 +120,7 @@ def test_native_cache_refusals(native_lib):
     native_refusal("kv_write", "NULL", *write(scale=None))
     native_refusal("kv_write", "aligned", *write(x=AT + 2))
     native_refusal("kv_write", "multiples of 16", *write(codes=AT + 8))
-    native_refusal("kv_write", "multiples of 16", *write(strides=(C.c_int64 * 6)(16, 16, 16, 16, 16, 24)))
+    native_refusal("kv_write", "multiples of 16", *write(strides=(C.c_int64 * 6)(16, 16, 16, 16, 16, 24), cap=2))
     assert native_lib.dyninfer_cuda_kv_write(*write(x=None, rows=0)) == 0
     read = (AT, AT, 0, S6, AT, AT, 32, S6, AT, AT, S4, AT, 1, 1, 1, 24, 1, None)
     native_refusal("kv_read", "kv_read: head dim 24", *read)
