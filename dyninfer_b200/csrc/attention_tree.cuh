@@ -7,14 +7,15 @@
 // The T * G rows that share a kv head (G query heads) are one block of rows, so that a key or value is fetched once for all of
 // them. Work on a (sequence, kv head) is split over the keys: over the key groups of a block and over the blocks of a cluster,
 // each with a running (maximum, sum, output) of its own; the states meet in a fixed order, in shared memory.
-//   S = Q K^T  mma.sync m16n8k16. The order of the head's dimensions inside the product is free, so 8-bit keys are read 16
-//              bytes per lane as they lie and become exact f16 numbers in a register; the key's scale multiplies the score.
+//   S = Q K^T  mma.sync. The order of the head's dimensions inside the product is free, so 8-bit keys are read 16 bytes per lane
+//              as they lie; the key's scale multiplies the score. q8 keys enter whole-number products (m16n8k32) unconverted,
+//              others become f16 in a register (m16n8k16).
 //   O += P V   the accumulators of S are the A operand of P. 8-bit values are read 16 bytes of one key per lane, and two keys'
 //              bytes are interleaved on the way to f16; the value's scale goes into P. 2-byte values come by ldmatrix.trans.
 // Precision. Operands are f16 (bf16 for bf16 caches); what does not fit goes as two or three terms (an f32 query: 22 or 24
 // bits). A row of Q enters times a power of two that brings its largest element to 2^8 .. 2^9 (f16 has five bits of
-// exponent), P as p 2^14 scaled by the tile's largest value scale. An mma truncates where it adds to its accumulator, always
-// toward zero, so a tile's P V starts from zero and joins the running output by a rounded fma.
+// exponent) or, for whole-number products, as 24-bit numbers; P relative to the largest value scale so far. An mma truncates where
+// it adds to its accumulator, always toward zero, so a tile's P V starts from zero and joins the running output by rounded adds.
 #pragma once
 
 #include <algorithm>
@@ -129,11 +130,17 @@ __device__ __forceinline__ float lds4(uint32_t addr) {
   return v;
 }
 
-// Four codes of one word as two f16 pairs, in order. q8: whole numbers; e4m3: the value times 2^-8.
+// Two e4m3 codes as an f16 pair.
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t codes) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)codes));
+  return r;
+}
+// Four codes of one word as two f16 pairs, in order (q8: whole numbers).
 template <bool E4M3>
 __device__ __forceinline__ void widen(uint32_t w, uint32_t* lo, uint32_t* hi) {
   if (E4M3) {
-    *lo = kv_e4m3_to_half2(prmt(w, 0, 0x1404)), *hi = kv_e4m3_to_half2(prmt(w, 0, 0x3424));
+    *lo = e4m3_pair(w), *hi = e4m3_pair(w >> 16);
   } else {
     w ^= 0x80808080u;
     *lo = kv_q8_to_half2(prmt(w, 0x64646464u, 0x4140)), *hi = kv_q8_to_half2(prmt(w, 0x64646464u, 0x4342));
@@ -142,33 +149,69 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t* lo, uint32_t* hi) {
 // Entry i (0 .. 3) of two words, interleaved: (x_i, y_i) as an f16 pair; r[i].
 template <bool E4M3>
 __device__ __forceinline__ void widen_pairs(uint32_t x, uint32_t y, uint32_t (&r)[4]) {
+  uint32_t lo = prmt(x, y, 0x5140), hi = prmt(x, y, 0x7362);
   if (E4M3) {
-    r[0] = kv_e4m3_to_half2(prmt(x, y, 0x4000)), r[1] = kv_e4m3_to_half2(prmt(x, y, 0x5010));
-    r[2] = kv_e4m3_to_half2(prmt(x, y, 0x6020)), r[3] = kv_e4m3_to_half2(prmt(x, y, 0x7030));
+    r[0] = e4m3_pair(lo), r[1] = e4m3_pair(lo >> 16), r[2] = e4m3_pair(hi), r[3] = e4m3_pair(hi >> 16);
   } else {
-    const uint32_t lo = prmt(x, y, 0x5140) ^ 0x80808080u, hi = prmt(x, y, 0x7362) ^ 0x80808080u;
+    lo ^= 0x80808080u, hi ^= 0x80808080u;
     r[0] = kv_q8_to_half2(prmt(lo, 0x64646464u, 0x4140)), r[1] = kv_q8_to_half2(prmt(lo, 0x64646464u, 0x4342));
     r[2] = kv_q8_to_half2(prmt(hi, 0x64646464u, 0x4140)), r[3] = kv_q8_to_half2(prmt(hi, 0x64646464u, 0x4342));
   }
 }
+// Bytes that are e4m3's NaN become zeros; says whether there were any.
+__device__ __forceinline__ bool without_nan(uint32_t& w) {
+  const uint32_t some = (((w & 0x7f7f7f7fu) ^ 0x7f7f7f7fu) + 0x7f7f7f7fu) & 0x80808080u;
+  const uint32_t none = some ^ 0x80808080u;
+  w &= ~((none >> 7) * 0xffu);
+  return none != 0;
+}
+// 2-byte entries that are not finite become zeros; says whether there were any.
+template <bool BF>
+__device__ __forceinline__ bool without_odd(uint32_t& w) {
+  const uint32_t odd = BF ? ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u : ((w & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+  w &= ~((odd >> 15) * 0xffffu);
+  return odd != 0;
+}
+__device__ __forceinline__ void mma_s8(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// (x, y) += (u, v), two sums per instruction
+__device__ __forceinline__ void add2(float& x, float& y, float u, float v) {
+  asm("{\n\t.reg .b64 o, w;\n\tmov.b64 o, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\tadd.rn.f32x2 o, o, w;\n\tmov.b64 {%0, %1}, o;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(u), "f"(v));
+}
 
 // CT: cache; TQ: type of q and out; D: head dimensions, d filled up with zeros; MT: 16-row tiles per warp; WR: warps along the
-// rows; WK: key groups.
+// rows; WK: key groups. MT = 0: up to eight rows, an operand's leading terms in rows 0 .. 7 of a tile and its second ones in rows
+// 8 .. 15, so that one mma takes both and a thread has scores and outputs of one row instead of two.
 template <int CT, typename TQ, int D_, int MT_, int WR_, int WK_>
 struct Cfg {
-  static constexpr int D = D_, MT = MT_, WR = WR_, WK = WK_;
+  static constexpr bool HALF = MT_ == 0;
+  static constexpr int D = D_, MT = HALF ? 1 : MT_, WR = WR_, WK = WK_, H = HALF ? 1 : 2;   // H: rows of a thread in a tile
   static constexpr bool BF = CT == TREE_BF16, WIDE = CT == TREE_BF16 || CT == TREE_F16, E4M3 = CT == TREE_E4M3;
   static constexpr int ES = WIDE ? 2 : 1;
   static constexpr bool QF = std::is_same<TQ, float>::value, QB = std::is_same<TQ, __nv_bfloat16>::value;
-  static constexpr int QT = BF ? (QB ? 1 : QF ? 3 : 2) : (QF ? 2 : 1);   // terms of Q
+  // q8 keys of few rows are operands as they are, of whole-number products; Q is three signed bytes of its row's largest element
+  static constexpr bool I8 = CT == TREE_Q8 && MT_ <= 1;
+  static constexpr int QT = I8 ? 3 : BF ? (QB ? 1 : QF ? 3 : 2) : (QF ? 2 : 1);   // terms of Q
   static constexpr int PT = BF ? (QF ? 3 : 2) : (QB ? 1 : 2);            // terms of P
-  static constexpr int RB = 16 * MT * WR;                                // rows of a block
+  static constexpr int NQ = HALF ? (QT + 1) / 2 : QT, NP = HALF ? (PT + 1) / 2 : PT;   // operands of Q and P
+  static constexpr int RB = 8 * H * MT * WR;                             // rows of a block
   static constexpr int THREADS = 32 * WR * WK;
-  static constexpr int KT = (WIDE ? 16 : 32) * (WR >= 2 ? 2 : 1);        // keys of a tile
-  static constexpr int STAGES = 3;
+  static constexpr int KT = (WIDE || HALF ? 16 : 32) * (WR >= 2 ? 2 : 1); // keys of a tile
+  static constexpr int STAGES = HALF && !WIDE ? 4 : 3;
+  static constexpr int BLOCKS = HALF ? (WIDE ? 2 : 3) : 1;               // of an SM, as far as registers go
   static constexpr int TILE = KT * D * ES;
   static constexpr int STAGE = 2 * TILE + (WIDE ? 0 : 2 * KT * 4);
   static constexpr int RING = STAGE * STAGES * WK;
+  static constexpr int QS = I8 ? D / 32 : D / 16;                        // steps of the products over the dimensions
+  // a row's reference maximum may lie this far below its maximum (in powers of two): outputs are rescaled less often. f32 results
+  // keep the weights' bits instead
+  static constexpr float SLACK = QF ? 0.f : 8.f;
+  static constexpr int PEXP = QF ? 13 : 5;                               // f16 weights enter times 2^PEXP
   static constexpr bool QREG = MT == 1;                                  // Q stays in registers, else in shared memory
   static constexpr int QSM = QREG ? 0 : RB * D * 2 * QT;
   static constexpr int STATE = WK * RB * (D + 2) * 4;                    // (output, maximum, sum) of every key group
@@ -194,11 +237,11 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int64_t b, int row, int6
   return a.mask ? a.mask[b * a.ms[0] + row * a.ms[1] + j] != 0 : j <= row;
 }
 
-template <int CT, typename TQ, int D, int MT, int WR, int WK>
-__global__ void __launch_bounds__(32 * WR * WK) tree_attention_kernel(const __grid_constant__ TreeArgs a) {
-  using C = Cfg<CT, TQ, D, MT, WR, WK>;
+template <int CT, typename TQ, int D, int MT_, int WR, int WK>
+__global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLOCKS) tree_attention_kernel(const __grid_constant__ TreeArgs a) {
+  using C = Cfg<CT, TQ, D, MT_, WR, WK>;
   using O = Op<C::BF>;
-  constexpr int KT = C::KT, NT = D / 8, KS = D / 16, NK = KT / 8;
+  constexpr int KT = C::KT, NT = D / 8, KS = D / 16, NK = KT / 8, MT = C::MT, H = C::H, NE = 2 * H;  // NE: a thread's entries of an n8 tile
   extern __shared__ __align__(128) uint8_t tree_shared[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int wr = warp % WR, wk = warp / WR;
@@ -220,30 +263,41 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attention_kernel(const __gr
   const float* vsb = C::WIDE ? nullptr : a.vs + b * a.vss[0] + kvh * a.vss[1];
 
   // ---- tiles: the group takes every (splits * WK)-th one ----
-  const int64_t tiles = (keys + KT - 1) / KT;
-  const int64_t first = (int64_t)split * WK + wk, step = (int64_t)a.splits * WK;
+  const int tiles = (int)((keys + KT - 1) / KT);
+  const int first = split * WK + wk, step = a.splits * WK;
   const uint32_t ring = smem_u32(tree_shared) + (uint32_t)(wk * C::STAGES * C::STAGE);
   const int gtid = wr * 32 + lane;
-  const int chunks = a.d * C::ES / 16;
-  auto fetch = [&](int64_t tile, int stage) {
+  constexpr int PER = D * C::ES / 16, ROWS = 32 * WR / PER, COPIES = KT / ROWS;  // a thread's copies lie ROWS keys apart
+  const int my_key = gtid / PER, my_chunk = gtid % PER;
+  const bool my_dims = my_chunk < a.d * C::ES / 16;
+  const uint8_t* const kp = kb + my_key * a.kst[2] + my_chunk * 16;
+  const uint8_t* const vp = vb + my_key * a.vst[2] + my_chunk * 16;
+  auto fetch = [&](int tile, int stage) {
     if (tile < tiles) {
       const uint32_t at = ring + (uint32_t)(stage * C::STAGE);
-      const int64_t key0 = tile * KT;
-      constexpr int PER = D * C::ES / 16;
+      const int64_t key0 = (int64_t)tile * KT;
+      const uint8_t *ks = kp + key0 * a.kst[2], *vs = vp + key0 * a.vst[2];
+      if (key0 + KT <= keys) {
 #pragma unroll
-      for (int i = 0; i < KT * PER / (32 * WR); i++) {
-        const int u = i * 32 * WR + gtid, key = u / PER, c = u % PER;
-        const int64_t kk = key0 + key;
-        const bool live = kk < keys && c < chunks;
-        cp16(at + k_chunk<C>(key, c), live ? kb + kk * a.kst[2] + c * 16 : kb, live);
-        cp16(at + C::TILE + v_chunk<C>(key, c), live ? vb + kk * a.vst[2] + c * 16 : vb, live);
+        for (int i = 0; i < COPIES; i++) {
+          cp16(at + k_chunk<C>(my_key + i * ROWS, my_chunk), my_dims ? ks : kb, my_dims);
+          cp16(at + C::TILE + v_chunk<C>(my_key + i * ROWS, my_chunk), my_dims ? vs : vb, my_dims);
+          ks += ROWS * a.kst[2], vs += ROWS * a.vst[2];
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < COPIES; i++) {
+          const bool live = my_dims && key0 + my_key + i * ROWS < keys;
+          cp16(at + k_chunk<C>(my_key + i * ROWS, my_chunk), live ? ks + i * ROWS * a.kst[2] : kb, live);
+          cp16(at + C::TILE + v_chunk<C>(my_key + i * ROWS, my_chunk), live ? vs + i * ROWS * a.vst[2] : vb, live);
+        }
       }
       if (!C::WIDE) {
-        for (int u = gtid; u < KT; u += 32 * WR) {
-          const int64_t kk = key0 + u;
-          const bool live = kk < keys;
-          cp4(at + 2 * C::TILE + u * 4, live ? ksb + kk : ksb, live);
-          cp4(at + 2 * C::TILE + (KT + u) * 4, live ? vsb + kk : vsb, live);
+#pragma unroll
+        for (int u = gtid; u < 2 * KT; u += 32 * WR) {  // the keys' scales, then the values'
+          const int64_t kk = key0 + (u & (KT - 1));
+          const float* const of = u < KT ? ksb : vsb;
+          cp4(at + 2 * C::TILE + u * 4, kk < keys ? of + kk : of, kk < keys);
         }
       }
     }
@@ -257,396 +311,462 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attention_kernel(const __gr
 
   // ---- Q: this warp's rows, in the order in which keys' dimensions come out ----
   // element e (0 .. 3) of k16 step s at lane quarter t: 2-byte keys 16 s + 2 t + {0, 1, 8, 9}; 8-bit keys lie 16 bytes per lane
-  uint32_t qf[C::QREG ? C::QT : 1][C::QREG ? KS : 1][4];
+  uint32_t qf[C::QREG ? C::NQ : 1][C::QREG ? C::QS : 1][4];
   uint8_t* qs = tree_shared + C::BODY;
-  float mult[MT][2];  // what a row's scores are multiplied with: log2(e) * scale / the row's power of two
+  float mult[MT][H];  // what a row's scores are multiplied with: log2(e) * scale / the row's factor
 #pragma unroll
   for (int m = 0; m < MT; m++) {
-    float x[2][KS][4];
+    float x[H][KS][4];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int h = 0; h < H; h++) {
       const int r = row0 + (wr * MT + m) * 16 + g + 8 * h;
       const bool live = r < total_rows;
       const int tr = live ? r / a.group : 0, gh = live ? r - tr * a.group : 0;
       const TQ* src = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
-      float top = 0.f;
+      float most = 0.f, odd = 0.f;
 #pragma unroll
       for (int s = 0; s < KS; s++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int dim = C::WIDE ? 16 * s + 2 * t + (e & 1) + 8 * (e >> 1) : s / 4 * 64 + t * 16 + s % 4 * 4 + e;
           x[h][s][e] = live && dim < a.d ? kv_float(src[dim]) : 0.f;
-          top = fmaxf(top, fabsf(x[h][s][e]));
+          most = fmaxf(most, fabsf(x[h][s][e]));
+          odd = fmaf(x[h][s][e], 0.f, odd);
         }
       float mul = 1.f, inv = 1.f;
       if (!C::BF) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the row's largest element to 2^8 .. 2^9; zeros, infinities and extremes of f32 keep a bounded factor
-        int ex = (int)((__float_as_uint(top) >> 23) & 0xff);
-        ex = ex < 20 ? 20 : ex > 250 ? 250 : ex;
-        mul = __uint_as_float((uint32_t)(262 - ex) << 23), inv = __uint_as_float((uint32_t)(ex - 8) << 23);
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        if (C::I8) {
+          // the largest element to 127 * 2^16: three signed bytes. A row that is not finite gets scores that are not numbers
+          odd += __shfl_xor_sync(0xffffffffu, odd, 1);
+          odd += __shfl_xor_sync(0xffffffffu, odd, 2);
+          most = fminf(fmaxf(most, 1e-31f), 3e38f);
+          mul = odd == 0.f ? 8323072.f / most : 0.f, inv = odd == 0.f ? most / 8323072.f : __uint_as_float(0x7fc00000u);
+        } else {
+          // the row's largest element to 2^8 .. 2^9; zeros, infinities and extremes of f32 keep a bounded factor
+          int ex = (int)((__float_as_uint(most) >> 23) & 0xff);
+          ex = ex < 20 ? 20 : ex > 250 ? 250 : ex;
+          mul = __uint_as_float((uint32_t)(262 - ex) << 23), inv = __uint_as_float((uint32_t)(ex - 8) << 23);
+        }
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
           for (int e = 0; e < 4; e++) x[h][s][e] *= mul;
       }
-      mult[m][h] = a.scale * LOG2E * inv * (C::E4M3 ? 256.f : 1.f);
+      mult[m][h] = a.scale * LOG2E * inv;
     }
+    auto keep = [&](int n, int s, const uint32_t (&f)[4]) {
+      if (C::QREG) {
 #pragma unroll
-    for (int s = 0; s < KS; s++)
-#pragma unroll
-      for (int n = 0; n < C::QT; n++) {
-        uint32_t f[4];
-        f[0] = O::take(x[0][s][0], x[0][s][1]), f[1] = O::take(x[1][s][0], x[1][s][1]);
-        f[2] = O::take(x[0][s][2], x[0][s][3]), f[3] = O::take(x[1][s][2], x[1][s][3]);
-        if (C::QREG) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) qf[C::QREG ? n : 0][C::QREG ? s : 0][i] = f[i];
-        } else if (wk == 0) {
-          *reinterpret_cast<uint4*>(qs + ((((wr * MT + m) * C::QT + n) * KS + s) * 32 + lane) * 16) = make_uint4(f[0], f[1], f[2], f[3]);
-        }
+        for (int i = 0; i < 4; i++) qf[C::QREG ? n : 0][C::QREG ? s : 0][i] = f[i];
+      } else if (wk == 0) {
+        *reinterpret_cast<uint4*>(qs + ((((wr * MT + m) * C::NQ + n) * C::QS + s) * 32 + lane) * 16) = make_uint4(f[0], f[1], f[2], f[3]);
       }
-  }
-  if (!C::QREG) __syncthreads();
-  const uint32_t qaddr = smem_u32(qs) + (uint32_t)(wr * MT * C::QT * KS * 512 + lane * 16);
-
-  // ---- the running state ----
-  float out[MT][NT][4], top[MT][2], sum[MT][2];
-  // 2-byte values that are not finite: weight 0, or a weight's zero second term, times one is not a number. Where a result is
-  // not finite the keys are gone through once more, with such entries left out of the products and added one by one.
-  for (bool careful = false;; careful = true) {
+    };
+    if (C::I8) {
 #pragma unroll
-  for (int m = 0; m < MT; m++) {
+      for (int s = 0; s < C::QS; s++) {
+        uint32_t term[3][H][2] = {};  // [leading to last][row][step of four dimensions]
 #pragma unroll
-    for (int n = 0; n < NT; n++)
+        for (int h = 0; h < H; h++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) out[m][n][e] = 0.f;
-    top[m][0] = top[m][1] = -INFINITY, sum[m][0] = sum[m][1] = 0.f;
-  }
-
-  int stage = 0;
-  for (int64_t tile = first; tile < tiles; tile += step) {
-    cp_wait<C::STAGES - 2>();
-    if (WR > 1)
-      asm volatile("bar.sync %0, %1;" ::"r"(wk + 1), "n"(32 * WR) : "memory");
-    else
-      __syncwarp();
-    {
-      int ahead = stage + C::STAGES - 1;
-      if (ahead >= C::STAGES) ahead -= C::STAGES;
-      fetch(tile + (C::STAGES - 1) * step, ahead);
-    }
-    const uint32_t kt = ring + (uint32_t)(stage * C::STAGE), vt = kt + C::TILE, st = vt + C::TILE;
-    if (++stage == C::STAGES) stage = 0;
-
-    // S
-    float sc[MT][NK][4];
+          for (int w = 0; w < 2; w++)
 #pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-      for (int j = 0; j < NK; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) sc[m][j][e] = 0.f;
-    if (C::WIDE) {
-#pragma unroll
-      for (int s = 0; s < KS; s++) {
-        uint32_t kf[NK][2];
-#pragma unroll
-        for (int j = 0; j < NK; j += 2) {
-          uint32_t r[4];
-          const int key = j * 8 + (lane & 7) + ((lane >> 4) << 3);
-          ldsm4(r, kt + k_chunk<C>(key, 2 * s + ((lane >> 3) & 1)));
-          kf[j][0] = r[0], kf[j][1] = r[1], kf[j + 1][0] = r[2], kf[j + 1][1] = r[3];
-        }
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-          for (int n = C::QT - 1; n >= 0; n--) {
-            uint32_t f[4];
-            if (C::QREG) {
-#pragma unroll
-              for (int i = 0; i < 4; i++) f[i] = qf[C::QREG ? n : 0][C::QREG ? s : 0][i];
-            } else {
-              const uint4 w = lds16(qaddr + (uint32_t)(((m * C::QT + n) * KS + s) * 512));
-              f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
+            for (int e = 0; e < 4; e++) {
+              const int v = __float2int_rn(x[h][(2 * s + w) % KS][e]);
+              const int low = (int)(signed char)v, above = (v - low) >> 8, mid = (int)(signed char)above, top = (above - mid) >> 8;
+              term[0][h][w] |= (uint32_t)(top & 0xff) << (8 * e), term[1][h][w] |= (uint32_t)(mid & 0xff) << (8 * e);
+              term[2][h][w] |= (uint32_t)(low & 0xff) << (8 * e);
             }
+        if (C::HALF) {
+          keep(0, s, {term[0][0][0], term[1][0][0], term[0][0][1], term[1][0][1]});
+          keep(1 % C::NQ, s, {term[2][0][0], 0u, term[2][0][1], 0u});
+        } else {
 #pragma unroll
-            for (int j = 0; j < NK; j++) O::mma(sc[m][j], f, kf[j][0], kf[j][1]);
-          }
+          for (int n = 0; n < 3; n++) keep(n % C::NQ, s, {term[n][0][0], term[n][H - 1][0], term[n][0][1], term[n][H - 1][1]});
+        }
       }
     } else {
 #pragma unroll
-      for (int h = 0; h < D / 64; h++) {
-        uint4 raw[NK];
+      for (int s = 0; s < KS; s++)
 #pragma unroll
-        for (int j = 0; j < NK; j++) raw[j] = lds16(kt + k_chunk<C>(j * 8 + g, h * 4 + t));
+        for (int n = 0; n < C::NQ; n++) {
+          uint32_t f[4] = {};
+          f[0] = O::take(x[0][s][0], x[0][s][1]), f[2] = O::take(x[0][s][2], x[0][s][3]);
+          if (!C::HALF || 2 * n + 1 < C::QT) f[1] = O::take(x[H - 1][s][0], x[H - 1][s][1]), f[3] = O::take(x[H - 1][s][2], x[H - 1][s][3]);
+          keep(n, s % C::QS, f);
+        }
+    }
+  }
+  if (!C::QREG) __syncthreads();
+  const uint32_t qaddr = smem_u32(qs) + (uint32_t)(wr * MT * C::NQ * C::QS * 512 + lane * 16);
+  auto query = [&](int m, int n, int s, uint32_t (&f)[4]) {
+    if (C::QREG) {
 #pragma unroll
-        for (int s4 = 0; s4 < 4; s4++) {
-          const int s = h * 4 + s4;
+      for (int i = 0; i < 4; i++) f[i] = qf[C::QREG ? n : 0][C::QREG ? s : 0][i];
+    } else {
+      const uint4 w = lds16(qaddr + (uint32_t)(((m * C::NQ + n) * C::QS + s) * 512));
+      f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
+    }
+  };
+
+  // ---- the running state ----
+  float out[MT][NT][NE], top[MT][H], sum[MT][H];
+  int vex = 30;  // 8-bit: exponent that the values' scales are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
+  // Values that are not finite: weight 0, or a weight's zero second term, times one is not a number. Where a result is not finite
+  // the keys are gone through once more, with such entries left out of the products and added one by one. (Codes of q8 are finite.)
+  constexpr bool ODD = CT != TREE_Q8;
+  for (bool careful = false;; careful = true) {
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < NE; e++) out[m][n][e] = 0.f;
+#pragma unroll
+      for (int h = 0; h < H; h++) top[m][h] = -INFINITY, sum[m][h] = 0.f;
+    }
+    vex = 30;
+    int stage = 0;
+    for (int tile = first; tile < tiles; tile += step) {
+      cp_wait<C::STAGES - 2>();
+      if (WR > 1)
+        asm volatile("bar.sync %0, %1;" ::"r"(wk + 1), "n"(32 * WR) : "memory");
+      else
+        __syncwarp();
+      {
+        int ahead = stage + C::STAGES - 1;
+        if (ahead >= C::STAGES) ahead -= C::STAGES;
+        fetch(tile + (C::STAGES - 1) * step, ahead);
+      }
+      const uint32_t kt = ring + (uint32_t)(stage * C::STAGE), vt = kt + C::TILE, st = vt + C::TILE;
+      if (++stage == C::STAGES) stage = 0;
+
+      // S
+      float sc[MT][NK][NE];
+      if constexpr (C::I8) {
+        int acc[3][NK][4] = {};  // leading, second (not HALF: HALF has both in one), last terms
+        uint4 raw[NK][D / 64];
+#pragma unroll
+        for (int j = 0; j < NK; j++)
+#pragma unroll
+          for (int h = 0; h < D / 64; h++) raw[j][h] = lds16(kt + k_chunk<C>(j * 8 + g, h * 4 + t));
+#pragma unroll
+        for (int s = 0; s < C::QS; s++)
+#pragma unroll
+          for (int n = 0; n < C::NQ; n++) {
+            uint32_t f[4];
+            query(0, n, s, f);
+#pragma unroll
+            for (int j = 0; j < NK; j++) {
+              const uint4 w = raw[j][s / 2];
+              mma_s8(acc[n][j], f, s & 1 ? w.z : w.x, s & 1 ? w.w : w.y);
+            }
+          }
+#pragma unroll
+        for (int j = 0; j < NK; j++)
+#pragma unroll
+          for (int e = 0; e < NE; e++) {
+            const int lead = acc[0][j][e], mid = C::HALF ? acc[0][j][(e + 2) & 3] : acc[1][j][e], low = acc[C::NQ - 1][j][e];
+            sc[0][j][e] = fmaf((float)lead, 65536.f, (float)(mid * 256 + low));
+          }
+      } else {
+        float acc[MT][NK][4] = {};
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
           uint32_t kf[NK][2];
+          if (C::WIDE) {
 #pragma unroll
-          for (int j = 0; j < NK; j++)
-            widen<C::E4M3>(s4 == 0 ? raw[j].x : s4 == 1 ? raw[j].y : s4 == 2 ? raw[j].z : raw[j].w, &kf[j][0], &kf[j][1]);
+            for (int j = 0; j < NK; j += 2) {
+              uint32_t r[4];
+              const int key = j * 8 + (lane & 7) + ((lane >> 4) << 3);
+              ldsm4(r, kt + k_chunk<C>(key, 2 * s + ((lane >> 3) & 1)));
+              kf[j][0] = r[0], kf[j][1] = r[1], kf[j + 1][0] = r[2], kf[j + 1][1] = r[3];
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < NK; j++) {
+              uint32_t w;
+              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(kt + k_chunk<C>(j * 8 + g, s / 4 * 4 + t) + s % 4 * 4));
+              widen<C::E4M3>(w, &kf[j][0], &kf[j][1]);
+            }
+          }
 #pragma unroll
           for (int m = 0; m < MT; m++)
 #pragma unroll
-            for (int n = C::QT - 1; n >= 0; n--) {
+            for (int n = C::NQ - 1; n >= 0; n--) {
               uint32_t f[4];
-              if (C::QREG) {
+              query(m, n, s % C::QS, f);
 #pragma unroll
-                for (int i = 0; i < 4; i++) f[i] = qf[C::QREG ? n : 0][C::QREG ? s : 0][i];
-              } else {
-                const uint4 w = lds16(qaddr + (uint32_t)(((m * C::QT + n) * KS + s) * 512));
-                f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
-              }
-#pragma unroll
-              for (int j = 0; j < NK; j++) O::mma(sc[m][j], f, kf[j][0], kf[j][1]);
+              for (int j = 0; j < NK; j++) O::mma(acc[m][j], f, kf[j][0], kf[j][1]);
             }
         }
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int j = 0; j < NK; j++)
+#pragma unroll
+            for (int e = 0; e < NE; e++) sc[m][j][e] = C::HALF ? acc[m][j][e] + acc[m][j][e + 4 - NE] : acc[m][j][e];
       }
-    }
 
-    // scores in powers of two, masked
-    const int64_t key0 = tile * KT;
-    float vscale[C::WIDE ? 1 : NK][2];
-    float pmul = C::BF ? 1.f : 16384.f, punit = C::BF ? 1.f : 0x1p-14f;
-    if (!C::WIDE) {
-      float most = 0.f;
+      // scores in powers of two, masked
+      const int64_t key0 = (int64_t)tile * KT;
+      float vscale[C::WIDE ? 1 : NK][2];
+      float grow = 1.f;  // 8-bit: what the units of `out` change by
+      if (!C::WIDE) {
+        float most = 0.f;
 #pragma unroll
-      for (int j = 0; j < NK; j++)
+        for (int j = 0; j < NK; j++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          vscale[C::WIDE ? 0 : j][e] = lds4(st + (uint32_t)(KT + j * 8 + 2 * t + e) * 4);
-          most = fmaxf(most, vscale[C::WIDE ? 0 : j][e]);
-          const float kscale = lds4(st + (uint32_t)(j * 8 + 2 * t + e) * 4);
+          for (int e = 0; e < 2; e++) {
+            vscale[C::WIDE ? 0 : j][e] = lds4(st + (uint32_t)(KT + j * 8 + 2 * t + e) * 4);
+            most = fmaxf(most, vscale[C::WIDE ? 0 : j][e]);
+            const float kscale = lds4(st + (uint32_t)(j * 8 + 2 * t + e) * 4);
 #pragma unroll
-          for (int m = 0; m < MT; m++) sc[m][j][e] *= kscale, sc[m][j][e + 2] *= kscale;
-        }
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      int ex = (int)(__float_as_uint(most) >> 23);
-      ex = ex < 30 ? 30 : ex > 240 ? 240 : ex;
-      pmul = __uint_as_float((uint32_t)(254 + 13 - ex) << 23);   // the tile's largest value scale to 2^13 .. 2^14
-      punit = __uint_as_float((uint32_t)(ex - 13 + (C::E4M3 ? 8 : 0)) << 23);
-    }
-    const bool tail = key0 + KT > len;
-    uint32_t vis[MT][2];
+            for (int m = 0; m < MT; m++)
 #pragma unroll
-    for (int m = 0; m < MT; m++) vis[m][0] = vis[m][1] = 0xffffffffu;
-    if (tail) {
+              for (int h = 0; h < H; h++) sc[m][j][2 * h + e] *= kscale;
+          }
+        int ex = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23);
+        ex = ex < 30 ? 30 : ex > 240 ? 240 : ex;
+        if (ex > vex) grow = ex2((float)(vex - ex)), vex = ex;
+      }
+      const float pmul = C::BF ? 1.f : C::WIDE ? (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(254 + C::PEXP - vex) << 23);
+      const bool tail = key0 + KT > len;
+      uint32_t vis[MT][H];
 #pragma unroll
       for (int m = 0; m < MT; m++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const int r = row0 + (wr * MT + m) * 16 + g + 8 * h;
-          const int tr = r < total_rows ? r / a.group : 0;
-          uint32_t bits = 0;
+        for (int h = 0; h < H; h++) vis[m][h] = 0xffffffffu;
+      if (tail) {
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int h = 0; h < H; h++) {
+            const int r = row0 + (wr * MT + m) * 16 + g + 8 * h;
+            const int tr = r < total_rows ? r / a.group : 0;
+            uint32_t bits = 0;
+#pragma unroll 1
+            for (int i = 0; i < 2 * NK; i++) {
+              const int64_t key = key0 + (i >> 1) * 8 + 2 * t + (i & 1);
+              if (key < keys && sees(a, b, tr, key - len)) bits |= 1u << i;
+            }
+            vis[m][h] = bits;
+          }
+      }
+      float decay[MT][H];
+      bool change = grow != 1.f;
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+          // the maximum in powers of two; a score and its reference go through one fma, so that the score is not rounded before
+          // the difference. Masked entries are -infinity by a choice, not by a product with a factor that may be zero
+          float best = -INFINITY;
 #pragma unroll
           for (int j = 0; j < NK; j++)
 #pragma unroll
-            for (int e = 0; e < 2; e++)
-              if (key0 + j * 8 + 2 * t + e < keys && sees(a, b, tr, key0 + j * 8 + 2 * t + e - len)) bits |= 1u << (2 * j + e);
-          vis[m][h] = bits;
-        }
-    }
-    float decay[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        // the maximum in powers of two; a score and its maximum go through one fma, so that the score is not rounded before
-        // the difference. Masked entries are -infinity by a choice, not by a product with a factor that may be zero
-        float best = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < NK; j++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const float s = sc[m][j][2 * h + e] * mult[m][h];
-            best = fmaxf(best, !tail || vis[m][h] >> (2 * j + e) & 1 ? s : -INFINITY);
-          }
-        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
-        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-        best = fmaxf(best, top[m][h]);
-        const float base = best == -INFINITY ? 0.f : best;
-        decay[m][h] = ex2(top[m][h] - base);
-        top[m][h] = best;
-        float part = 0.f;
-#pragma unroll
-        for (int j = 0; j < NK; j++)
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            float p = ex2(fmaf(sc[m][j][2 * h + e], mult[m][h], -base));
-            if (tail && !(vis[m][h] >> (2 * j + e) & 1)) p = 0.f;
-            sc[m][j][2 * h + e] = p;
-            part += p;
-          }
-        sum[m][h] = sum[m][h] * decay[m][h] + part;
-      }
-    // weights as operands
-    uint32_t pf[MT][C::PT][NK / 2][4];
-#pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
-      for (int j = 0; j < NK; j++) {
-        float w[4];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          w[e] = sc[m][j][e] * pmul;
-          if (!C::WIDE) {
-            w[e] *= vscale[C::WIDE ? 0 : j][e & 1];
-            if (tail && !(vis[m][e >> 1] >> (2 * j + (e & 1)) & 1)) w[e] = 0.f;  // the scale of a key that is not seen
-          }
-        }
-#pragma unroll
-        for (int n = 0; n < C::PT; n++) {
-          pf[m][n][j / 2][(j & 1) * 2] = O::take(w[0], w[1]);
-          pf[m][n][j / 2][(j & 1) * 2 + 1] = O::take(w[2], w[3]);
-        }
-      }
-    bool odd = false;
-    if (C::WIDE && careful) {
-      constexpr int PER = D * C::ES / 16;
-      for (int u = lane; u < KT * PER; u += 32) {
-        const uint4 w = lds16(vt + (uint32_t)u * 16);
-        const uint32_t mask = C::BF ? 0x7f807f80u : 0x7c007c00u, x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          odd |= ((x[i] & mask & 0xffffu) == (mask & 0xffffu)) || ((x[i] & mask & 0xffff0000u) == (mask & 0xffff0000u));
-      }
-      odd = __any_sync(0xffffffffu, odd);
-    }
-    // O = O * decay + P V
-#pragma unroll
-    for (int nb = 0; nb < NT / 2; nb++) {
-      // two n8 tiles at a time (2-byte), or four (8-bit: a word of four dimensions)
-      if (C::WIDE) {
-        float u[MT][2][4];
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-          for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) u[m][i][e] = 0.f;
-#pragma unroll
-        for (int kk = 0; kk < NK / 2; kk++) {
-          uint32_t r[4];
-          const int key = kk * 16 + (lane & 15);
-          ldsm4t(r, vt + v_chunk<C>(key, 2 * nb + (lane >> 4)));
-          if (odd) {
-            const uint32_t mask = C::BF ? 0x7f80u : 0x7c00u;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              if ((r[i] & mask) == mask) r[i] &= 0xffff0000u;
-              if ((r[i] >> 16 & mask) == mask) r[i] &= 0xffffu;
+            for (int e = 0; e < 2; e++) {
+              const float s = sc[m][j][2 * h + e] * mult[m][h];
+              best = fmaxf(best, !tail || vis[m][h] >> (2 * j + e) & 1 ? s : -INFINITY);
             }
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+          decay[m][h] = grow;
+          if (best > top[m][h] + C::SLACK || top[m][h] == -INFINITY) {
+            if (best > -INFINITY) decay[m][h] *= ex2(top[m][h] - best), change = true;
+            sum[m][h] *= ex2(top[m][h] - (best == -INFINITY ? 0.f : best));
+            top[m][h] = best;
           }
+          const float base = top[m][h] == -INFINITY ? 0.f : top[m][h];
+          float part = 0.f;
 #pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int n = C::PT - 1; n >= 0; n--) {
-              O::mma(u[m][0], pf[m][n][kk], r[0], r[1]);
-              O::mma(u[m][1], pf[m][n][kk], r[2], r[3]);
-            }
-        }
-#pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
-          for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) out[m][2 * nb + i][e] = out[m][2 * nb + i][e] * decay[m][e >> 1] + u[m][i][e] * punit;
-      }
-    }
-    if (C::WIDE && odd) {
-      // the entries left out, to the rows that see their keys
-#pragma unroll 1
-      for (int key = 0; key < KT; key++) {
-        const int j = key / 8, from = (lane & ~3) + (key & 7) / 2;
-#pragma unroll
-        for (int m = 0; m < MT; m++) {
-          // which of the two columns is a matter of the key: picked without indexing registers
-          float p0 = 0.f, p1 = 0.f;
-          uint32_t s0 = 0, s1 = 0;
-#pragma unroll
-          for (int jj = 0; jj < NK; jj++)
-            if (jj == j) {
-              p0 = key & 1 ? sc[m][jj][1] : sc[m][jj][0], p1 = key & 1 ? sc[m][jj][3] : sc[m][jj][2];
-              s0 = vis[m][0] >> (2 * jj + (key & 1)) & 1, s1 = vis[m][1] >> (2 * jj + (key & 1)) & 1;
-            }
-          p0 = __shfl_sync(0xffffffffu, p0, from), p1 = __shfl_sync(0xffffffffu, p1, from);
-          s0 = __shfl_sync(0xffffffffu, s0, from), s1 = __shfl_sync(0xffffffffu, s1, from);
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-            uint32_t w;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(vt + v_chunk<C>(key, n) + 4 * t));
+          for (int j = 0; j < NK; j++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const uint32_t half = e ? w >> 16 : w & 0xffffu, mask = C::BF ? 0x7f80u : 0x7c00u;
-              if ((half & mask) == mask) {
-                const float val = C::BF ? __bfloat162float(__ushort_as_bfloat16((unsigned short)half)) : __half2float(__ushort_as_half((unsigned short)half));
-                if (s0) out[m][n][e] += p0 * val;
-                if (s1) out[m][n][e + 2] += p1 * val;
-              }
+              float p = ex2(fmaf(sc[m][j][2 * h + e], mult[m][h], -base));
+              if (tail && !(vis[m][h] >> (2 * j + e) & 1)) p = 0.f;
+              sc[m][j][2 * h + e] = p;
+              part += p;
             }
-          }
+          sum[m][h] += part;
         }
-      }
-    }
-    if (!C::WIDE) {
-      // lane g has D / 8 consecutive dimensions of a key: n8 tile i is dimension g * D / 8 + i
-      constexpr int WORDS = D / 32;  // words of a key per lane
-#pragma unroll
-      for (int w4 = 0; w4 < WORDS; w4++) {
-        float u[MT][4][4];
+      if (__any_sync(0xffffffffu, change)) {
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
-          for (int i = 0; i < 4; i++)
+          for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) u[m][i][e] = 0.f;
+            for (int e = 0; e < NE; e++) out[m][n][e] *= decay[m][e >> 1];
+      }
+      // weights as operands
+      uint32_t pf[MT][C::NP][NK / 2][4];
 #pragma unroll
-        for (int kk = 0; kk < NK / 2; kk++) {
-          uint32_t x[4];
+      for (int m = 0; m < MT; m++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int key = kk * 16 + 2 * t + (i & 1) + 8 * (i >> 1), at = g * (D / 8) + w4 * 4;
-            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x[i]) : "r"(vt + v_chunk<C>(key, at / 16) + (uint32_t)(at % 16)));
+        for (int j = 0; j < NK; j++) {
+          float w[NE];
+#pragma unroll
+          for (int e = 0; e < NE; e++) {
+            w[e] = sc[m][j][e] * pmul;
+            if (!C::WIDE) {
+              w[e] *= vscale[C::WIDE ? 0 : j][e & 1];
+              if (tail && !(vis[m][e >> 1] >> (2 * j + (e & 1)) & 1)) w[e] = 0.f;  // the scale of a key that is not seen
+            }
           }
-          uint32_t r0[4], r1[4];
-          widen_pairs<C::E4M3>(x[0], x[1], r0);
-          widen_pairs<C::E4M3>(x[2], x[3], r1);
+#pragma unroll
+          for (int n = 0; n < C::NP; n++) {
+            pf[m][n][j / 2][(j & 1) * 2] = O::take(w[0], w[1]);
+            pf[m][n][j / 2][(j & 1) * 2 + 1] = !C::HALF || 2 * n + 1 < C::PT ? O::take(w[NE - 2], w[NE - 1]) : 0u;
+          }
+        }
+      bool odd = false;
+      if (ODD && careful) {
+        for (int u = lane; u < KT * PER; u += 32) {
+          const uint4 w = lds16(vt + (uint32_t)u * 16);
+          uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 4; i++) odd |= C::WIDE ? without_odd<C::BF>(x[i]) : without_nan(x[i]);
+        }
+        odd = __any_sync(0xffffffffu, odd);
+      }
+      // O += P V: products of the tile start from zero
+      auto fold = [&](int m, int n, const float (&u)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) add2(out[m][n][e % NE], out[m][n][e % NE + 1], u[e], u[e + 1]);
+      };
+      if (C::WIDE) {
+#pragma unroll
+        for (int nb = 0; nb < NT / 2; nb++) {
+          float u[MT][2][4] = {};
+#pragma unroll
+          for (int kk = 0; kk < NK / 2; kk++) {
+            uint32_t r[4];
+            const int key = kk * 16 + (lane & 15);
+            ldsm4t(r, vt + v_chunk<C>(key, 2 * nb + (lane >> 4)));
+            if (odd) {
+#pragma unroll
+              for (int i = 0; i < 4; i++) without_odd<C::BF>(r[i]);
+            }
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+              for (int n = C::NP - 1; n >= 0; n--) {
+                O::mma(u[m][0], pf[m][n][kk], r[0], r[1]);
+                O::mma(u[m][1], pf[m][n][kk], r[2], r[3]);
+              }
+          }
 #pragma unroll
           for (int m = 0; m < MT; m++)
 #pragma unroll
-            for (int n = C::PT - 1; n >= 0; n--)
-#pragma unroll
-              for (int i = 0; i < 4; i++) O::mma(u[m][i], pf[m][n][kk], r0[i], r1[i]);
+            for (int i = 0; i < 2; i++) fold(m, 2 * nb + i, u[m][i]);
         }
+      } else {
+        // lane g has D / 8 consecutive dimensions of a key: n8 tile i is dimension g * D / 8 + i
+        constexpr int WORDS = D / 32;  // words of a key per lane
+        uint32_t x[NK / 2][4][WORDS];
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int kk = 0; kk < NK / 2; kk++)
 #pragma unroll
-          for (int i = 0; i < 4; i++)
+          for (int i = 0; i < 4; i++) {
+            const int key = kk * 16 + 2 * t + (i & 1) + 8 * (i >> 1);
+            if (WORDS == 4) {
+              const uint4 w = lds16(vt + v_chunk<C>(key, g));
+              x[kk][i][0] = w.x, x[kk][i][1] = w.y, x[kk][i][2 % WORDS] = w.z, x[kk][i][3 % WORDS] = w.w;
+            } else {
+              const uint2 w = lds8(vt + v_chunk<C>(key, g / 2) + (uint32_t)(g % 2 * 8));
+              x[kk][i][0] = w.x, x[kk][i][1] = w.y;
+            }
+            if (ODD && odd) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) out[m][w4 * 4 + i][e] = out[m][w4 * 4 + i][e] * decay[m][e >> 1] + u[m][i][e] * punit;
+              for (int w = 0; w < WORDS; w++) without_nan(x[kk][i][w]);
+            }
+          }
+#pragma unroll
+        for (int w = 0; w < WORDS; w++) {
+          float u[MT][4][4] = {};
+#pragma unroll
+          for (int kk = 0; kk < NK / 2; kk++) {
+            uint32_t r0[4], r1[4];
+            widen_pairs<C::E4M3>(x[kk][0][w], x[kk][1][w], r0);
+            widen_pairs<C::E4M3>(x[kk][2][w], x[kk][3][w], r1);
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+              for (int n = C::NP - 1; n >= 0; n--)
+#pragma unroll
+                for (int i = 0; i < 4; i++) O::mma(u[m][i], pf[m][n][kk], r0[i], r1[i]);
+          }
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) fold(m, w * 4 + i, u[m][i]);
+        }
+      }
+      if (ODD && odd) {
+        // the entries left out, to the rows that see their keys
+#pragma unroll 1
+        for (int key = 0; key < KT; key++) {
+          const int j = key / 8, from = (lane & ~3) + (key & 7) / 2;
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+              // which of the two columns is a matter of the key: picked without indexing registers
+              float p = 0.f;
+              uint32_t seen = 0;
+#pragma unroll
+              for (int jj = 0; jj < NK; jj++)
+                if (jj == j) p = key & 1 ? sc[m][jj][2 * h + 1] : sc[m][jj][2 * h], seen = vis[m][h] >> (2 * jj + (key & 1)) & 1;
+              p = __shfl_sync(0xffffffffu, p, from), seen = __shfl_sync(0xffffffffu, seen, from);
+#pragma unroll
+              for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                  const int dim = C::WIDE ? n * 8 + 2 * t + e : (2 * t + e) * (D / 8) + n;
+                  const uint32_t at = vt + v_chunk<C>(key, dim * C::ES / 16) + (uint32_t)(dim * C::ES % 16);
+                  float val = 0.f;
+                  if (C::WIDE) {
+                    unsigned short bits;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(at));
+                    if ((bits & (C::BF ? 0x7f80u : 0x7c00u)) == (C::BF ? 0x7f80u : 0x7c00u))
+                      val = C::BF ? __bfloat162float(__ushort_as_bfloat16(bits)) : __half2float(__ushort_as_half(bits));
+                  } else {
+                    uint32_t bits;
+                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bits) : "r"(at));
+                    if ((bits & 0x7fu) == 0x7fu) val = __uint_as_float(0x7fc00000u);
+                  }
+                  if (seen && val != 0.f) out[m][n][2 * h + e] += p * val;
+                }
+            }
+        }
       }
     }
+    cp_wait<0>();
+    if (!ODD || careful) break;
+    bool finite = true;
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int e = 0; e < NE; e++) finite = finite && fabsf(out[m][n][e]) < INFINITY;
+    if (!__syncthreads_or(!finite)) break;
+    begin();
   }
-  cp_wait<0>();
-  if (!C::WIDE || careful) break;
-  bool finite = true;
+  // out in its own units again
+  const float unit = C::BF ? 1.f : C::WIDE ? 1.f / (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(vex - C::PEXP) << 23);
 #pragma unroll
   for (int m = 0; m < MT; m++)
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) finite = finite && fabsf(out[m][n][e]) < INFINITY;
-  if (!__syncthreads_or(!finite)) break;
-  begin();
-  }
+      for (int e = 0; e < NE; e++) out[m][n][e] *= unit;
 #pragma unroll
   for (int m = 0; m < MT; m++)
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int h = 0; h < H; h++) {
       sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 1);
       sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 2);
     }
@@ -658,7 +778,7 @@ __global__ void __launch_bounds__(32 * WR * WK) tree_attention_kernel(const __gr
 #pragma unroll
   for (int m = 0; m < MT; m++)
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int h = 0; h < H; h++) {
       const int r = (wr * MT + m) * 16 + g + 8 * h;
       float* to = so + (wk * C::RB + r) * D;
       if (C::WIDE) {
@@ -746,9 +866,10 @@ int run(TreeArgs a, cudaStream_t s) {
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), C::SMEM)) return 1;
   const int64_t pairs = a.batch * a.kv_heads;
   a.row_blocks = (int)(((int64_t)a.rows * a.group + C::RB - 1) / C::RB);
-  // blocks of a cluster: as many as two per SM leave room for, at least two tiles for each key group at full capacity
+  // blocks of a cluster: as many as there is room for at once, at least two tiles for each key group at full capacity
+  const int64_t room = (int64_t)std::max(1, sm_count()) * std::max(1, std::min(std::max(2, C::BLOCKS), (227 << 10) / (C::SMEM + 1024)));
   int splits = 16;
-  while (splits > 1 && (pairs * a.row_blocks * splits > 2 * std::max(1, sm_count()) || a.cap < (int64_t)splits * WK * C::KT * 2)) splits /= 2;
+  while (splits > 1 && (pairs * a.row_blocks * splits > room || a.cap < (int64_t)splits * WK * C::KT * 2)) splits--;
   if (splits > 8) DYN_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   a.splits = splits;
   DYN_CHECK(pairs * splits <= 0x7fffffff && a.row_blocks <= 65535, "tree_attention: too many sequences or rows for one call");
@@ -767,6 +888,7 @@ int run(TreeArgs a, cudaStream_t s) {
 template <int CT, typename TQ, int D>
 int by_rows(const TreeArgs& a, cudaStream_t s) {
   const int64_t rows = (int64_t)a.rows * a.group;
+  if (rows <= 8) return run<CT, TQ, D, 0, 1, 4>(a, s);
   if (rows <= 16) return run<CT, TQ, D, 1, 1, 4>(a, s);
   if (rows <= 32) return run<CT, TQ, D, 2, 1, 4>(a, s);
   if (rows <= 64) return run<CT, TQ, D, 2, 2, 2>(a, s);

@@ -49,11 +49,6 @@ __device__ __forceinline__ uint2 kv_encode8(const float (&v)[8], float inv) {
   return make_uint2(w[0], w[1]);
 }
 
-// Two e4m3 codes, one in each half's upper byte, as f16 of their value times 2^-8: exponents differ by eight between the
-// formats, subnormals included. The format's NaN encodings, which no write makes, come out as +-480.
-__device__ __forceinline__ uint32_t kv_e4m3_to_half2(uint32_t bytes) {
-  return (bytes & 0x80008000u) | ((bytes >> 1) & 0x3f803f80u);
-}
 // Two q8 codes with 128 added, one in each half's lower byte: 0x6400 | u is the f16 number 1024 + u.
 __device__ __forceinline__ uint32_t kv_q8_to_half2(uint32_t bytes) {
   const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&bytes), __half2half2(__ushort_as_half(0x6480)));  // 1152
@@ -65,8 +60,7 @@ __device__ __forceinline__ void kv_decode8(uint2 raw, float scale, float (&v)[8]
 #pragma unroll
   for (int i = 0; i < 8; i++) {
     const uint32_t byte = ((i < 4 ? raw.x : raw.y) >> (i % 4 * 8)) & 0xffu;
-    // powers of two leave the e4m3 value exact: the one rounding is the product's
-    const float code = E4M3 ? __half2float(__ushort_as_half((unsigned short)kv_e4m3_to_half2(byte << 8))) * 256.f
+    const float code = E4M3 ? __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)))
                             : (float)(int)(signed char)byte;
     v[i] = code * scale;
   }

@@ -156,7 +156,7 @@ int dyninfer_cuda_argmax_static(const float* v_dev, int64_t n, int64_t* out_inde
 /* cache types besides DYNINFER_ENC_F16 / _BF16: one byte per element and one f32 scale per row */
 enum {
   DYNINFER_KV_Q8 = 32,  /* signed whole numbers, value = code * scale */
-  DYNINFER_KV_E4M3 = 33 /* e4m3, value = code * scale (a power of two); the NaN codes read as +-480 */
+  DYNINFER_KV_E4M3 = 33 /* e4m3, value = code * scale (a power of two) */
 };
 
 /* Rotary positions of x [batch, rows, heads, d] (strides: batch, row, head): pair i of the first
