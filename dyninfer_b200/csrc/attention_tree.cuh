@@ -885,27 +885,5 @@ int run(TreeArgs a, cudaStream_t s) {
   return 0;
 }
 
-template <int CT, typename TQ, int D>
-int by_rows(const TreeArgs& a, cudaStream_t s) {
-  const int64_t rows = (int64_t)a.rows * a.group;
-  if (rows <= 8) return run<CT, TQ, D, 0, 1, 4>(a, s);
-  if (rows <= 16) return run<CT, TQ, D, 1, 1, 4>(a, s);
-  if (rows <= 32) return run<CT, TQ, D, 2, 1, 4>(a, s);
-  if (rows <= 64) return run<CT, TQ, D, 2, 2, 2>(a, s);
-  return run<CT, TQ, D, 2, 4, 1>(a, s);
-}
-
-template <int CT>
-int by_type(const TreeArgs& a, int q_type, cudaStream_t s) {
-  if (a.d <= 64) {
-    if (q_type == E_F32) return by_rows<CT, float, 64>(a, s);
-    if (q_type == E_F16) return by_rows<CT, __half, 64>(a, s);
-    return by_rows<CT, __nv_bfloat16, 64>(a, s);
-  }
-  if (q_type == E_F32) return by_rows<CT, float, 128>(a, s);
-  if (q_type == E_F16) return by_rows<CT, __half, 128>(a, s);
-  return by_rows<CT, __nv_bfloat16, 128>(a, s);
-}
-
 }  // namespace tree
 }  // namespace dyn

@@ -1,5 +1,5 @@
 // Tree attention over e4m3 caches.
-#include "attention_tree.cuh"
+#include "attention_tree_wide.cuh"
 
 namespace dyn {
 

@@ -1,5 +1,5 @@
 // Tree attention over f16 caches.
-#include "attention_tree.cuh"
+#include "attention_tree_wide.cuh"
 
 namespace dyn {
 

@@ -1,0 +1,566 @@
+// Tree attention of many rows (attention_tree.cuh states the operator) on the 5th-generation tensor cores.
+//
+// One block = 128 rows (tokens x query heads of one kv head), the 128 lanes of tensor memory, and a share of the keys in tiles of
+// 64; the blocks of a cluster take the tiles in turn and merge their states through shared memory. Roles:
+//   8 softmax warps   two threads share a row: each has half of a tile's scores and half of the output's dimensions. They turn S
+//                     into P (terms side by side, in place of S) and add the product before, U, to 64 f32 sums.
+//   4 filling warps   bring keys and values into shared memory as swizzled 16-bit tiles: 2-byte caches by asynchronous copies
+//                     straight to their places, 8-bit ones by way of a ring of raw tiles, converted on the way.
+//   1 issuing warp    S(i+1) = Q K^T while the softmax warps are at tile i, U(i) = P V while they are at tile i + 1; S has two
+//                     places in tensor memory, Q (up to three terms) lies there as well.
+// Scores, references, slack, terms and units are those of attention_tree.cuh. Where a result is not finite (weight 0 times
+// an infinity in a key that a row does not see), the block's rows are computed once more one by one, without tensor cores.
+// All waits are bounded; one that runs out leaves a code in the device's error word.
+#pragma once
+
+#include "attention_tree.cuh"
+#include "umma.cuh"
+
+namespace dyn {
+namespace tree {
+
+constexpr int W_ROWS = 128, W_KEYS = 64, W_SOFTMAX = 256, W_FILL = 128, W_THREADS = W_SOFTMAX + W_FILL + 32;
+constexpr int W_BOX = W_KEYS * 128;  // bytes of 64 keys x 64 two-byte dimensions
+
+template <int CT, typename TQ, int D_>
+struct Wide {
+  static constexpr int D = D_;
+  static constexpr bool BF = CT == TREE_BF16, WIDE = CT == TREE_BF16 || CT == TREE_F16, E4M3 = CT == TREE_E4M3;
+  static constexpr bool QF = std::is_same<TQ, float>::value, QB = std::is_same<TQ, __nv_bfloat16>::value;
+  static constexpr int QT = BF ? (QB ? 1 : QF ? 3 : 2) : (QF ? 2 : 1), PT = BF ? (QF ? 3 : 2) : (QB ? 1 : 2);
+  static constexpr float SLACK = QF ? 0.f : 8.f;
+  static constexpr int PEXP = QF ? 13 : 5;
+  // tensor memory columns
+  static constexpr int S_COLS = PT == 3 ? 96 : 64, U_COL = 2 * S_COLS, Q_COL = U_COL + D;
+  static_assert(Q_COL + QT * (D / 2) <= 512, "tensor memory has 512 columns");
+  // shared memory: tiles (keys, then values), the values' and keys' scales, raw tiles
+  static constexpr int TILE = 2 * D * W_KEYS * 2, TILES = WIDE ? 5 : 4;
+  static constexpr int RAW = WIDE ? 0 : 2 * D * W_KEYS + 2 * W_KEYS * 4, RAWS = 3;
+  static constexpr int PITCH = D + 4;  // floats of a row's final state
+  static constexpr int BODY = TILE * TILES + RAW * RAWS;
+  static_assert(W_ROWS * PITCH * 4 <= BODY, "the final states take the tiles' place");
+  // A block waits for its columns of tensor memory and then for its cluster, so no two blocks of that kind may share an SM: this
+  // much shared memory leaves no room for another one of this kernel, nor for one of the other kernels that do both (77 KB and more)
+  static constexpr int SMEM = BODY + 1024 > 152 * 1024 ? BODY + 1024 : 152 * 1024;
+  static_assert(SMEM + 1024 + 78 * 1024 > 228 * 1024 && SMEM <= 220 * 1024, "see above");
+};
+
+// kind::f16, M = 128, N = n; BF: bf16 operands; mn: B contiguous along N
+__device__ __forceinline__ uint32_t wide_idesc(int n, bool bf, bool mn) {
+  return umma_idesc(n) | (bf ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u);
+}
+// B operand contiguous along N, 128-byte swizzle: a 128-byte row per K element with 64 elements of N; the next 64 a box further
+__device__ __forceinline__ uint64_t wide_desc_mn(uint32_t at) {
+  return (uint64_t)((at >> 4) & 0x3fff) | ((uint64_t)(W_BOX >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void wide_st8(uint32_t addr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ uint32_t box_chunk(int key, int chunk) {  // a 16-byte chunk (8 dimensions) of a key in a tile
+  return (uint32_t)((chunk >> 3) * W_BOX + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
+}
+
+template <int CT>
+__device__ __forceinline__ float cached(const uint8_t* row, const float* scale, int dim) {  // one entry as a number
+  if (CT == TREE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[dim]);
+  if (CT == TREE_F16) return __half2float(reinterpret_cast<const __half*>(row)[dim]);
+  if (CT == TREE_Q8) return (float)(int)(signed char)row[dim] * *scale;
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)row[dim], __NV_E4M3))) * *scale;
+}
+
+template <int CT, typename TQ, int D>
+__global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const __grid_constant__ TreeArgs a, int* error) {
+  using C = Wide<CT, TQ, D>;
+  using O = Op<C::BF>;
+  extern __shared__ uint8_t wide_shared[];
+  __shared__ uint64_t kv_full[C::TILES], kv_free[C::TILES], s_full[2], p_full[2], u_full, u_free;
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int s_abort;
+  __shared__ __align__(16) float kscale[C::WIDE ? 1 : C::TILES][W_KEYS], vscale[C::WIDE ? 1 : C::TILES][W_KEYS];  // read by fours
+  __shared__ int vexp[C::TILES][4];               // exponents of the tile's largest value scale, of four filling warps
+  __shared__ float s_most[2][2][W_ROWS];          // [parity][half][row]
+  __shared__ __align__(16) float s_sum[W_ROWS][2];  // read by twos
+  __shared__ float s_top[W_ROWS];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wide_shared) + 1023) & ~uintptr_t(1023));
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int split = (int)blockIdx.x % a.splits;
+  const int64_t pair = blockIdx.x / a.splits;
+  const int64_t b = pair / a.kv_heads;
+  const int kvh = (int)(pair - b * a.kv_heads);
+  const int row0 = blockIdx.y * W_ROWS, live_rows = min(W_ROWS, a.rows * a.group - row0);
+  const int live_warps = 2 * ((live_rows + 31) / 32);
+
+  int64_t len = a.lengths[b], keys = 0;
+  if (len >= 0) {
+    len = len < a.cap ? len : a.cap;
+    keys = len + a.rows < a.cap ? len + a.rows : a.cap;
+  }
+  const uint8_t* const kb = a.k + b * a.kst[0] + kvh * a.kst[1];
+  const uint8_t* const vb = a.v + b * a.vst[0] + kvh * a.vst[1];
+  const float* const ksb = C::WIDE ? nullptr : a.ks + b * a.kss[0] + kvh * a.kss[1];
+  const float* const vsb = C::WIDE ? nullptr : a.vs + b * a.vss[0] + kvh * a.vss[1];
+  const int tiles = (int)((keys + W_KEYS - 1) / W_KEYS);
+  const int mine = split < tiles ? (tiles - split + a.splits - 1) / a.splits : 0;
+
+  if (tid == 0) {
+    s_abort = 0;
+    for (int i = 0; i < C::TILES; i++) mbar_init(kv_full + i, W_FILL), mbar_init(kv_free + i, 1);
+    for (int i = 0; i < 2; i++) mbar_init(s_full + i, 1), mbar_init(p_full + i, live_warps);
+    mbar_init(&u_full, 1), mbar_init(&u_free, live_warps);
+    mbar_fence_init();
+  }
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+  auto wait = [&](uint64_t* bar, unsigned parity, int code) {
+    if (!mbar_wait_bounded(bar, parity, TG_SPINS, &s_abort) && !s_abort) s_abort = code;
+  };
+
+  const int row = (warp & 3) * 32 + lane, part = (warp >> 2) & 1;   // of a softmax thread
+  const bool working = warp < 8 && (warp & 3) * 32 < live_rows;
+  const uint32_t tlane = (uint32_t)((warp & 3) * 32) << 16;
+  const int row_index = row0 + min(row, live_rows - 1), tr = row_index / a.group, gh = row_index - tr * a.group;
+  const TQ* const query = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
+  float out[D / 2], top = -INFINITY, sum = 0.f, mult = 0.f;
+  int vex = 30;  // 8-bit: exponent that value scales are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
+#pragma unroll
+  for (int d = 0; d < D / 2; d++) out[d] = 0.f;
+
+  if (working && mine) {
+    // ---- Q into tensor memory: this thread's half of the row ----
+    float mul = 1.f, inv = 1.f;
+    if (!C::BF) {
+      float most = 0.f;
+#pragma unroll 8
+      for (int d = 0; d < D / 2; d++)
+        if (part * (D / 2) + d < a.d) most = fmaxf(most, fabsf(kv_float(query[part * (D / 2) + d])));
+      s_most[0][part][row] = most;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+      most = fmaxf(most, s_most[0][part ^ 1][row]);
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+      int ex = (int)((__float_as_uint(most) >> 23) & 0xff);
+      ex = ex < 20 ? 20 : ex > 250 ? 250 : ex;
+      mul = __uint_as_float((uint32_t)(262 - ex) << 23), inv = __uint_as_float((uint32_t)(ex - 8) << 23);
+    }
+    mult = a.scale * LOG2E * inv;
+#pragma unroll 1
+    for (int s = 0; s < D / 32; s++) {
+      float x[16];
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        const int dim = part * (D / 2) + s * 16 + e;
+        x[e] = dim < a.d ? kv_float(query[dim]) * mul : 0.f;
+      }
+#pragma unroll
+      for (int n = 0; n < C::QT; n++) {
+        uint32_t f[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = O::take(x[2 * e], x[2 * e + 1]);
+        __syncwarp();
+        wide_st8(tmem + tlane + C::Q_COL + n * (D / 2) + part * (D / 4) + s * 8, f);
+      }
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  __syncthreads();  // Q is complete
+  tc_fence_after();
+
+  if (working) {
+    // ---- softmax ----
+    const uint32_t u_at = tmem + tlane + C::U_COL + (uint32_t)part * (D / 2);
+    bool changed = false;  // for the whole warp
+    float decay = 1.f;
+    auto fold = [&](int i) {  // U of tile i; then what tile i + 1 did to the reference
+      wait(&u_full, i & 1, 3);
+      __syncwarp();
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < D / 32; c++) {
+        uint32_t u[16];
+        tmem_ld16(u_at + 16u * c, u);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) add2(out[16 * c + e], out[16 * c + e + 1], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&u_free);
+    };
+    int buf = 0;
+    unsigned phase = 0;
+#pragma unroll 1
+    for (int i = 0; i < mine; i++) {
+      const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS + part * 32;
+      const uint32_t s_at = tmem + tlane + (uint32_t)((i & 1) * C::S_COLS);
+      wait(s_full + (i & 1), (i >> 1) & 1, 1);
+      if (!C::WIDE) wait(kv_full + buf, phase, 2);  // for the scales
+      __syncwarp();
+      tc_fence_after();
+      uint32_t x[32];
+      tmem_ld16(s_at + 32u * part, reinterpret_cast<uint32_t(&)[16]>(x[0]));
+      tmem_ld16(s_at + 32u * part + 16u, reinterpret_cast<uint32_t(&)[16]>(x[16]));
+      float grow = 1.f;
+      if (!C::WIDE) {
+        const int ex = max(max(vexp[buf][0], vexp[buf][1]), max(vexp[buf][2], vexp[buf][3]));
+        if (ex > vex) grow = ex2((float)(vex - ex)), vex = ex;
+      }
+      const float pmul = C::BF ? 1.f : C::WIDE ? (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(254 + C::PEXP - vex) << 23);
+      uint32_t vis = 0xffffffffu;
+      if (key0 + 32 > len) {
+        vis = 0;
+#pragma unroll 1
+        for (int e = 0; e < 32; e++)
+          if (key0 + e < keys && sees(a, b, tr, key0 + e - len)) vis |= 1u << e;
+      }
+      __syncwarp();
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      float best = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 32; e += 4) {
+        float s[4];
+        if (C::WIDE) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) s[j] = __uint_as_float(x[e + j]);
+        } else {
+          const float4 k4 = *reinterpret_cast<const float4*>(&kscale[C::WIDE ? 0 : buf][part * 32 + e]);
+          s[0] = __uint_as_float(x[e]) * k4.x, s[1] = __uint_as_float(x[e + 1]) * k4.y;
+          s[2] = __uint_as_float(x[e + 2]) * k4.z, s[3] = __uint_as_float(x[e + 3]) * k4.w;
+#pragma unroll
+          for (int j = 0; j < 4; j++) x[e + j] = __float_as_uint(s[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) best = fmaxf(best, vis >> (e + j) & 1 ? s[j] * mult : -INFINITY);
+      }
+      s_most[i & 1][part][row] = best;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+      best = fmaxf(best, s_most[i & 1][part ^ 1][row]);
+      decay = grow;
+      if (best > top + C::SLACK || top == -INFINITY) {
+        const float f = ex2(top - (best == -INFINITY ? 0.f : best));
+        decay *= f, sum *= f, top = best;
+      }
+      changed = __any_sync(0xffffffffu, decay != 1.f);
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        float w[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          float p = ex2(fmaf(__uint_as_float(x[16 * c + e]), mult, -base));
+          if (!(vis >> (16 * c + e) & 1)) p = 0.f;
+          w[e] = p;
+        }
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) s0 += w[e], s1 += w[e + 1];
+        sum += s0 + s1;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          if (C::WIDE) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[e + j] *= pmul;
+          } else {
+            const float4 v4 = *reinterpret_cast<const float4*>(&vscale[C::WIDE ? 0 : buf][part * 32 + 16 * c + e]);
+            w[e] *= pmul * v4.x, w[e + 1] *= pmul * v4.y, w[e + 2] *= pmul * v4.z, w[e + 3] *= pmul * v4.w;
+            if (vis != 0xffffffffu) {  // the scale of a key that is not seen
+#pragma unroll
+              for (int j = 0; j < 4; j++)
+                if (!(vis >> (16 * c + e + j) & 1)) w[e + j] = 0.f;
+            }
+          }
+        }
+        const uint32_t at = s_at + 32u * part + 16u * c;
+        __syncwarp();
+#pragma unroll
+        for (int n = 0; n < C::PT; n++) {
+          uint32_t f[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) f[e] = O::take(w[2 * e], w[2 * e + 1]);
+          wide_st8(n < 2 ? at + 8u * n : s_at + 64u + 16u * part + 8u * c, f);
+        }
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + (i & 1));
+      if (i) fold(i - 1);
+      if (changed) {
+#pragma unroll
+        for (int d = 0; d < D / 2; d++) out[d] *= decay;
+      }
+      if (++buf == C::TILES) buf = 0, phase ^= 1u;
+    }
+    if (mine) fold(mine - 1);
+    const float unit = C::BF ? 1.f : C::WIDE ? 1.f / (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(vex - C::PEXP) << 23);
+#pragma unroll
+    for (int d = 0; d < D / 2; d++) out[d] *= unit;
+  } else if (warp >= 8 && warp < 12) {
+    // ---- filling ----
+    const int ft = tid - W_SOFTMAX, fw = warp - 8;
+    constexpr int PER = C::WIDE ? D / 8 : D / 16;  // 16-byte pieces of a cached row
+    constexpr int COPIES = W_KEYS * PER / W_FILL, ROWS = W_FILL / PER;
+    const int key_l = ft / PER, piece = ft % PER;
+    const bool my_dims = piece * 16 < a.d * (C::WIDE ? 2 : 1);
+    auto copy = [&](int i) {  // tile i of this block's: into its place, or into the raw ring
+      if (i < mine) {
+        const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS;
+        const uint32_t at = smem_u32(smem) + (uint32_t)(C::WIDE ? i % C::TILES * C::TILE : C::TILES * C::TILE + i % C::RAWS * C::RAW);
+#pragma unroll
+        for (int j = 0; j < COPIES; j++) {
+          const int key = key_l + j * ROWS;
+          const bool live = my_dims && key0 + key < keys;
+          const uint32_t to = C::WIDE ? box_chunk(key, piece) : (uint32_t)(key * D + (D == 128 ? (piece ^ (key & 7)) : piece) * 16);
+          cp16(at + to, live ? kb + (key0 + key) * a.kst[2] + piece * 16 : kb, live);
+          cp16(at + (C::WIDE ? C::TILE / 2 : D * W_KEYS) + to, live ? vb + (key0 + key) * a.vst[2] + piece * 16 : vb, live);
+        }
+        if (!C::WIDE) {
+          const int64_t kk = key0 + (ft & (W_KEYS - 1));
+          const float* const of = ft < W_KEYS ? ksb : vsb;
+          cp4(at + 2 * D * W_KEYS + ft * 4, kk < keys ? of + kk : of, kk < keys);
+        }
+      }
+      cp_commit();
+    };
+    constexpr int AHEAD = C::WIDE ? C::TILES - 2 : C::RAWS - 1;  // copies under way
+    // a place is free when the products of the tile before in it are done
+    auto free_place = [&](int i) {
+      if (i >= C::TILES && i < mine) wait(kv_free + i % C::TILES, ((i / C::TILES) - 1) & 1, 4);
+    };
+    for (int i = 0; i < AHEAD; i++) copy(i);
+#pragma unroll 1
+    for (int i = 0; i < mine; i++) {
+      if (C::WIDE) {
+        free_place(i + AHEAD);
+        copy(i + AHEAD);
+        cp_wait<AHEAD>();
+      } else {
+        cp_wait<AHEAD - 1>();
+        asm volatile("bar.sync 5, %0;" ::"n"(W_FILL) : "memory");  // everybody's copies are there, and the oldest raw tile is done with
+        copy(i + AHEAD);
+        free_place(i);
+        const int to = i % C::TILES;
+        uint8_t* const tile = smem + to * C::TILE;
+        const uint32_t raw = smem_u32(smem) + (uint32_t)(C::TILES * C::TILE + i % C::RAWS * C::RAW);
+#pragma unroll
+        for (int j = 0; j < 2 * COPIES; j++) {
+          const int key = key_l + j % COPIES * ROWS, at = j / COPIES * D * W_KEYS + key * D + (D == 128 ? (piece ^ (key & 7)) : piece) * 16;
+          const uint4 w = lds16(raw + at);
+          uint4 f[2];
+          widen<C::E4M3>(w.x, &f[0].x, &f[0].y), widen<C::E4M3>(w.y, &f[0].z, &f[0].w);
+          widen<C::E4M3>(w.z, &f[1].x, &f[1].y), widen<C::E4M3>(w.w, &f[1].z, &f[1].w);
+          uint8_t* const half = tile + j / COPIES * (C::TILE / 2);
+          // pieces 4 .. 7 lie a box further, in the same banks as 0 .. 3: they store their halves the other way round
+          const bool turn = piece & 4;
+          *reinterpret_cast<uint4*>(half + box_chunk(key, 2 * piece + turn)) = turn ? f[1] : f[0];
+          *reinterpret_cast<uint4*>(half + box_chunk(key, 2 * piece + !turn)) = turn ? f[0] : f[1];
+        }
+        const float scale = lds4(raw + 2 * D * W_KEYS + ft * 4);
+        if (ft < W_KEYS) kscale[C::WIDE ? 0 : to][ft] = scale;
+        else vscale[C::WIDE ? 0 : to][ft - W_KEYS] = scale;
+        int ex = (int)(__reduce_max_sync(0xffffffffu, scale > 0.f ? __float_as_uint(scale) : 0u) >> 23);  // NaN compares false
+        ex = ex < 30 ? 30 : ex > 240 ? 240 : ex;
+        if (lane == 0) vexp[to][fw] = fw < 2 ? 30 : ex;
+      }
+      fence_async_smem();
+      mbar_arrive(kv_full + i % C::TILES);
+    }
+    cp_wait<0>();
+  } else if (warp == 12 && mine) {
+    // ---- issuing ----
+    const uint32_t id_s = wide_idesc(W_KEYS, C::BF, false), id_u = wide_idesc(D, C::BF, true);
+    const uint64_t k_desc = umma_desc(smem_u32(smem)), v_desc = wide_desc_mn(smem_u32(smem) + C::TILE / 2);
+    auto scores = [&](int i) {
+      const int buf = i % C::TILES;
+      wait(kv_full + buf, (i / C::TILES) & 1, 5);
+      if (i >= 2) wait(&u_full, (i - 2) & 1, 6);  // P of tile i - 2 has been read
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t k = k_desc + (uint64_t)(buf * (C::TILE >> 4));
+        const uint32_t to = tmem + (uint32_t)((i & 1) * C::S_COLS);
+        bool more = false;
+#pragma unroll
+        for (int n = C::QT - 1; n >= 0; n--)  // the small terms first
+#pragma unroll
+          for (int s = 0; s < D / 16; s++) {
+            umma_f16_ts(to, tmem + C::Q_COL + n * (D / 2) + 8u * s, k + (uint64_t)((s >> 2) * (W_BOX >> 4) + 2 * (s & 3)), id_s, more ? 1u : 0u);
+            more = true;
+          }
+        umma_commit(s_full + (i & 1));
+      }
+      __syncwarp();
+    };
+    scores(0);
+#pragma unroll 1
+    for (int i = 0; i < mine; i++) {
+      if (i + 1 < mine) scores(i + 1);
+      wait(p_full + (i & 1), (i >> 1) & 1, 7);
+      if (i) wait(&u_free, (i - 1) & 1, 8);
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t v = v_desc + (uint64_t)(i % C::TILES * (C::TILE >> 4));
+        const uint32_t p = tmem + (uint32_t)((i & 1) * C::S_COLS);
+        bool more = false;
+#pragma unroll
+        for (int n = C::PT - 1; n >= 0; n--)
+#pragma unroll
+          for (int s = 0; s < W_KEYS / 16; s++) {
+            umma_f16_ts(tmem + C::U_COL, n < 2 ? p + 16u * s + 8u * n : p + 64u + 8u * s, v + (uint64_t)(s * (2048 >> 4)), id_u, more ? 1u : 0u);
+            more = true;
+          }
+        umma_commit(&u_full);
+        umma_commit(kv_free + i % C::TILES);
+      }
+      __syncwarp();
+    }
+  }
+  if (s_abort) {
+    // products still under way land before their memory is used again
+    const long long t0 = clock64();
+    while (clock64() - t0 < (1LL << 22)) {
+    }
+  }
+  bool fine = true;
+#pragma unroll
+  for (int d = 0; d < D / 2; d++) fine = fine && fabsf(out[d]) < INFINITY;
+  __syncwarp();
+  if (__syncthreads_or(working && row < live_rows && !fine) && working) {
+    // ---- one by one: this thread's row and half of the dimensions, over this block's keys ----
+    top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int d = 0; d < D / 2; d++) out[d] = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < mine; i++) {
+      const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS;
+#pragma unroll 1
+      for (int e = 0; e < W_KEYS && key0 + e < keys; e++) {
+        if (!sees(a, b, tr, key0 + e - len)) continue;
+        const uint8_t *const k = kb + (key0 + e) * a.kst[2], *const v = vb + (key0 + e) * a.vst[2];
+        float s = 0.f;
+#pragma unroll 4
+        for (int d = 0; d < a.d; d++) s = fmaf(kv_float(query[d]), cached<CT>(k, ksb + key0 + e, d), s);
+        s *= a.scale * LOG2E;
+        if (!(s <= top)) {  // the maximum moves (or the score is not a number)
+          const float f = s > -INFINITY ? ex2(top - s) : 1.f;
+          sum *= f;
+#pragma unroll
+          for (int d = 0; d < D / 2; d++) out[d] *= f;
+          top = fmaxf(top, s);
+        }
+        const float p = ex2(s - (top == -INFINITY ? 0.f : top));
+        if (part == 0) sum += p;
+#pragma unroll
+        for (int d = 0; d < D / 2; d++) {
+          const int dim = part * (D / 2) + d;
+          if (dim < a.d) out[d] = fmaf(p, cached<CT>(v, vsb + key0 + e, dim), out[d]);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  __syncthreads();  // nobody reads tiles any more
+  float* const so = reinterpret_cast<float*>(smem);
+  if (working) {
+    float* const to = so + row * C::PITCH + part * (D / 2);
+#pragma unroll
+    for (int d = 0; d < D / 2; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(out[d], out[d + 1], out[d + 2], out[d + 3]);
+    s_sum[row][part] = sum;
+    if (part == 0) s_top[row] = top;
+  }
+  __syncwarp();
+  if (a.splits > 1)
+    asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
+  else
+    __syncthreads();
+  const uint32_t so_at = smem_u32(so), top_at = smem_u32(s_top), sum_at = smem_u32(&s_sum[0][0]);
+  for (int i = split * W_THREADS + tid; i < live_rows * (D / 4); i += a.splits * W_THREADS) {
+    const int r = i / (D / 4), c = i % (D / 4) * 4;
+    float m = -INFINITY, l = 0.f, o[4] = {};
+    for (int p = 0; p < a.splits; p++) {
+      uint32_t at_m, at_l, at_o;
+      float pm, l0, l1, x[4];
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_m) : "r"(top_at + (uint32_t)r * 4), "r"(p));
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_l) : "r"(sum_at + (uint32_t)r * 8), "r"(p));
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_o) : "r"(so_at + (uint32_t)(r * C::PITCH + c) * 4), "r"(p));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pm) : "r"(at_m) : "memory");
+      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(l0), "=f"(l1) : "r"(at_l) : "memory");
+      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(at_o) : "memory");
+      const float next = fmaxf(m, pm), base = next == -INFINITY ? 0.f : next;
+      const float fa = ex2(m - base), fb = ex2(pm - base);
+      l = l * fa + (l0 + l1) * fb;
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] = o[e] * fa + x[e] * fb;
+      m = next;
+    }
+    const int t2 = (row0 + r) / a.group, g2 = row0 + r - t2 * a.group;
+    TQ* to = static_cast<TQ*>(a.out) + ((b * a.rows + t2) * a.heads + (int64_t)kvh * a.group + g2) * a.d + c;
+    const float over = l == 0.f ? 0.f : 1.f / l;
+    if (c < a.d) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) kv_store(o[e] * over, to + e);
+    }
+  }
+  __syncwarp();
+  if (a.splits > 1)
+    asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");  // others read this block's states
+  tc_fence_after();
+  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  if (tid == 0 && s_abort) report_wait_expired(error, DEV_ERR_GEMM_PIPE);
+}
+
+template <int CT, typename TQ, int D>
+int run_wide(TreeArgs a, cudaStream_t s) {
+  using C = Wide<CT, TQ, D>;
+  auto kernel = tree_attention_wide_kernel<CT, TQ, D>;
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), C::SMEM)) return 1;
+  int* const error = device_error_word();
+  if (!error) return 1;
+  const int64_t pairs = a.batch * a.kv_heads;
+  a.row_blocks = (int)(((int64_t)a.rows * a.group + W_ROWS - 1) / W_ROWS);
+  // blocks of a cluster: as many as fit the SMs at once (a block takes an SM), at least two tiles each at full capacity
+  int splits = 8;
+  while (splits > 1 && (pairs * a.row_blocks * splits > std::max(1, sm_count()) || a.cap < (int64_t)splits * W_KEYS * 2)) splits--;
+  a.splits = splits;
+  DYN_CHECK(pairs * splits <= 0x7fffffff && a.row_blocks <= 65535, "tree_attention: too many sequences or rows for one call");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(pairs * splits), (unsigned)a.row_blocks), cfg.blockDim = dim3(W_THREADS);
+  cfg.dynamicSmemBytes = C::SMEM, cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  DYN_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, error));
+  count_launch();
+  return 0;
+}
+
+template <int CT, typename TQ, int D>
+int by_rows(const TreeArgs& a, cudaStream_t s) {
+  const int64_t rows = (int64_t)a.rows * a.group;
+  if (rows <= 8) return run<CT, TQ, D, 0, 1, 4>(a, s);
+  if (rows <= 16) return run<CT, TQ, D, 1, 1, 4>(a, s);
+  if (rows <= 32) return run<CT, TQ, D, 2, 1, 4>(a, s);
+  return run_wide<CT, TQ, D>(a, s);
+}
+
+template <int CT>
+int by_type(const TreeArgs& a, int q_type, cudaStream_t s) {
+  if (a.d <= 64) {
+    if (q_type == E_F32) return by_rows<CT, float, 64>(a, s);
+    if (q_type == E_F16) return by_rows<CT, __half, 64>(a, s);
+    return by_rows<CT, __nv_bfloat16, 64>(a, s);
+  }
+  if (q_type == E_F32) return by_rows<CT, float, 128>(a, s);
+  if (q_type == E_F16) return by_rows<CT, __half, 128>(a, s);
+  return by_rows<CT, __nv_bfloat16, 128>(a, s);
+}
+
+}  // namespace tree
+}  // namespace dyn
