@@ -120,7 +120,7 @@ int dyninfer_cuda_tree_attention(const void* q_dev, int q_type, const int64_t* q
   DYN_CHECK(heads <= 65536 && rows * heads <= (1ll << 30) && heads % kv_heads == 0, "tree_attention: heads %lld not a multiple of kv heads %lld (or too many)",
             (long long)heads, (long long)kv_heads);
   DYN_CHECK(d > 0 && d % 16 == 0 && d <= 128, "tree_attention: head dim %lld unsupported (a multiple of 16 up to 128)", (long long)d);
-  DYN_CHECK(isfinite(scale), "tree_attention: the scale is not finite");
+  DYN_CHECK(isfinite(scale) && scale > 0, "tree_attention: the scale must be above zero and finite");
   if (batch == 0 || rows == 0) return 0;
   DYN_CHECK(q_dev && q_strides && k_cache_dev && v_cache_dev && cache_strides && lengths_dev && ctx_dev, "tree_attention: NULL pointer");
   DYN_CHECK(wide || (k_scale_dev && v_scale_dev && scale_strides), "tree_attention: an 8-bit cache needs its scales");

@@ -13,13 +13,19 @@
 // All waits are bounded; one that runs out leaves a code in the device's error word.
 #pragma once
 
+#include <atomic>
+
 #include "attention_tree.cuh"
 #include "umma.cuh"
 
 namespace dyn {
 namespace tree {
 
-constexpr int W_ROWS = 128, W_KEYS = 64, W_SOFTMAX = 256, W_FILL = 128, W_THREADS = W_SOFTMAX + W_FILL + 32;
+constexpr int W_ROWS = 128, W_KEYS = 64, W_SOFTMAX = 256, W_FILL = 128;
+constexpr int W_THREADS = W_SOFTMAX + W_FILL + 128;  // whole warpgroups, because registers are dealt out per group
+// 512 threads start with 128 registers each; 256 x 168 + 256 x 88 is the same
+constexpr int W_MANY = 168, W_FEW = 88;
+static_assert(W_SOFTMAX * W_MANY + (W_THREADS - W_SOFTMAX) * W_FEW <= W_THREADS * 128, "the groups' shares come out of the launch's registers");
 constexpr int W_BOX = W_KEYS * 128;  // bytes of 64 keys x 64 two-byte dimensions
 
 template <int CT, typename TQ, int D_>
@@ -57,6 +63,17 @@ __device__ __forceinline__ void wide_st8(uint32_t addr, const uint32_t (&v)[8]) 
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
                "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
+}
+// (x, y) * (u, v), (x, y) * (u, u) - (v, v): two per instruction
+__device__ __forceinline__ void mul2(float& x, float& y, float u, float v) {
+  asm("{\n\t.reg .b64 o, w;\n\tmov.b64 o, {%0, %1};\n\tmov.b64 w, {%2, %3};\n\tmul.rn.f32x2 o, o, w;\n\tmov.b64 {%0, %1}, o;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(u), "f"(v));
+}
+__device__ __forceinline__ void fms2(float& x, float& y, float u, float v) {
+  asm("{\n\t.reg .b64 o, w, z;\n\tmov.b64 o, {%0, %1};\n\tmov.b64 w, {%2, %2};\n\tmov.b64 z, {%3, %3};\n\tfma.rn.f32x2 o, o, w, z;\n\tmov.b64 {%0, %1}, o;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(u), "f"(-v));
 }
 __device__ __forceinline__ uint32_t box_chunk(int key, int chunk) {  // a 16-byte chunk (8 dimensions) of a key in a tile
   return (uint32_t)((chunk >> 3) * W_BOX + key * 128 + (((chunk & 7) ^ (key & 7)) << 4));
@@ -128,10 +145,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
   const uint32_t tlane = (uint32_t)((warp & 3) * 32) << 16;
   const int row_index = row0 + min(row, live_rows - 1), tr = row_index / a.group, gh = row_index - tr * a.group;
   const TQ* const query = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
-  float out[D / 2], top = -INFINITY, sum = 0.f, mult = 0.f;
-  int vex = 30;  // 8-bit: exponent that value scales are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
-#pragma unroll
-  for (int d = 0; d < D / 2; d++) out[d] = 0.f;
+  float* const so = reinterpret_cast<float*>(smem);  // the final states, in the tiles' place
+  float mult = 0.f;
 
   if (working && mine) {
     // ---- Q into tensor memory: this thread's half of the row ----
@@ -149,7 +164,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
       ex = ex < 20 ? 20 : ex > 250 ? 250 : ex;
       mul = __uint_as_float((uint32_t)(262 - ex) << 23), inv = __uint_as_float((uint32_t)(ex - 8) << 23);
     }
-    mult = a.scale * LOG2E * inv;
+    mult = fmaxf(a.scale * LOG2E * inv, 1.2e-38f);  // above zero: -infinity stays itself
 #pragma unroll 1
     for (int s = 0; s < D / 32; s++) {
       float x[16];
@@ -173,22 +188,27 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
   __syncthreads();  // Q is complete
   tc_fence_after();
 
-  if (working) {
+  if (warp < 8) {
     // ---- softmax ----
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(W_MANY));
+    float out[D / 2], top = -INFINITY, sum = 0.f;
+    int vex = 30;  // 8-bit: exponent that value scales are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
+#pragma unroll
+    for (int d = 0; d < D / 2; d++) out[d] = 0.f;
     const uint32_t u_at = tmem + tlane + C::U_COL + (uint32_t)part * (D / 2);
-    bool changed = false;  // for the whole warp
-    float decay = 1.f;
-    auto fold = [&](int i) {  // U of tile i; then what tile i + 1 did to the reference
+    auto fold = [&](int i) {  // U of tile i
       wait(&u_full, i & 1, 3);
       __syncwarp();
       tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < D / 32; c++) {
-        uint32_t u[16];
-        tmem_ld16(u_at + 16u * c, u);
+      for (int c = 0; c < D / 32; c += 2) {
+        uint32_t u[2][16];
+        tmem_ld16(u_at + 16u * c, u[0]);
+        if (c + 1 < D / 32) tmem_ld16(u_at + 16u * c + 16u, u[1]);
         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) add2(out[16 * c + e], out[16 * c + e + 1], __uint_as_float(u[e]), __uint_as_float(u[e + 1]));
+        for (int e = 0; e < 32 && 16 * c + e < D / 2; e += 2)
+          add2(out[16 * c + e], out[16 * c + e + 1], __uint_as_float(u[e >> 4][e & 15]), __uint_as_float(u[e >> 4][(e & 15) + 1]));
       }
       tc_fence_before();
       __syncwarp();
@@ -197,22 +217,9 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
     int buf = 0;
     unsigned phase = 0;
 #pragma unroll 1
-    for (int i = 0; i < mine; i++) {
+    for (int i = 0; i < mine && working; i++) {
       const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS + part * 32;
       const uint32_t s_at = tmem + tlane + (uint32_t)((i & 1) * C::S_COLS);
-      wait(s_full + (i & 1), (i >> 1) & 1, 1);
-      if (!C::WIDE) wait(kv_full + buf, phase, 2);  // for the scales
-      __syncwarp();
-      tc_fence_after();
-      uint32_t x[32];
-      tmem_ld16(s_at + 32u * part, reinterpret_cast<uint32_t(&)[16]>(x[0]));
-      tmem_ld16(s_at + 32u * part + 16u, reinterpret_cast<uint32_t(&)[16]>(x[16]));
-      float grow = 1.f;
-      if (!C::WIDE) {
-        const int ex = max(max(vexp[buf][0], vexp[buf][1]), max(vexp[buf][2], vexp[buf][3]));
-        if (ex > vex) grow = ex2((float)(vex - ex)), vex = ex;
-      }
-      const float pmul = C::BF ? 1.f : C::WIDE ? (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(254 + C::PEXP - vex) << 23);
       uint32_t vis = 0xffffffffu;
       if (key0 + 32 > len) {
         vis = 0;
@@ -220,62 +227,76 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
         for (int e = 0; e < 32; e++)
           if (key0 + e < keys && sees(a, b, tr, key0 + e - len)) vis |= 1u << e;
       }
+      wait(s_full + (i & 1), (i >> 1) & 1, 1);
+      if (!C::WIDE) wait(kv_full + buf, phase, 2);  // for the scales
       __syncwarp();
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      float best = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        float s[4];
-        if (C::WIDE) {
-#pragma unroll
-          for (int j = 0; j < 4; j++) s[j] = __uint_as_float(x[e + j]);
-        } else {
-          const float4 k4 = *reinterpret_cast<const float4*>(&kscale[C::WIDE ? 0 : buf][part * 32 + e]);
-          s[0] = __uint_as_float(x[e]) * k4.x, s[1] = __uint_as_float(x[e + 1]) * k4.y;
-          s[2] = __uint_as_float(x[e + 2]) * k4.z, s[3] = __uint_as_float(x[e + 3]) * k4.w;
-#pragma unroll
-          for (int j = 0; j < 4; j++) x[e + j] = __float_as_uint(s[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++) best = fmaxf(best, vis >> (e + j) & 1 ? s[j] * mult : -INFINITY);
+      tc_fence_after();
+      uint32_t raw[2][16];
+      tmem_ld16(s_at + 32u * part, raw[0]);
+      tmem_ld16(s_at + 32u * part + 16u, raw[1]);
+      float grow = 1.f;
+      if (!C::WIDE) {
+        const int ex = max(vexp[buf][2], vexp[buf][3]);
+        if (ex > vex) grow = ex2((float)(vex - ex)), vex = ex;
       }
+      const float pmul = C::BF ? 1.f : C::WIDE ? (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(254 + C::PEXP - vex) << 23);
+      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      float x[32];
+#pragma unroll
+      for (int e = 0; e < 32; e++) x[e] = __uint_as_float(raw[e >> 4][e & 15]);
+      if (!C::WIDE) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          const float4 k4 = *reinterpret_cast<const float4*>(&kscale[C::WIDE ? 0 : buf][part * 32 + e]);
+          mul2(x[e], x[e + 1], k4.x, k4.y);
+          mul2(x[e + 2], x[e + 3], k4.z, k4.w);
+        }
+      }
+      if (vis != 0xffffffffu) {
+#pragma unroll
+        for (int e = 0; e < 32; e++)
+          if (!(vis >> e & 1)) x[e] = -INFINITY;
+      }
+      float best = x[0], other = x[1];
+#pragma unroll
+      for (int e = 2; e < 32; e += 2) best = fmaxf(best, x[e]), other = fmaxf(other, x[e + 1]);
+      best = fmaxf(fmaxf(best, other), -INFINITY) * mult;  // the factor is above zero
       s_most[i & 1][part][row] = best;
       asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
       best = fmaxf(best, s_most[i & 1][part ^ 1][row]);
-      decay = grow;
+      float decay = grow;
       if (best > top + C::SLACK || top == -INFINITY) {
         const float f = ex2(top - (best == -INFINITY ? 0.f : best));
         decay *= f, sum *= f, top = best;
       }
-      changed = __any_sync(0xffffffffu, decay != 1.f);
+      const bool changed = __any_sync(0xffffffffu, decay != 1.f);
       const float base = top == -INFINITY ? 0.f : top;
+      float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        float w[16];
+        float* const w = x + 16 * c;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-          float p = ex2(fmaf(__uint_as_float(x[16 * c + e]), mult, -base));
-          if (!(vis >> (16 * c + e) & 1)) p = 0.f;
-          w[e] = p;
+        for (int e = 0; e < 16; e += 2) {
+          fms2(w[e], w[e + 1], mult, base);
+          w[e] = ex2(w[e]), w[e + 1] = ex2(w[e + 1]);
+          add2(s0, s1, w[e], w[e + 1]);
         }
-        float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) s0 += w[e], s1 += w[e + 1];
-        sum += s0 + s1;
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           if (C::WIDE) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) w[e + j] *= pmul;
+            if (!C::BF) mul2(w[e], w[e + 1], pmul, pmul), mul2(w[e + 2], w[e + 3], pmul, pmul);
           } else {
-            const float4 v4 = *reinterpret_cast<const float4*>(&vscale[C::WIDE ? 0 : buf][part * 32 + 16 * c + e]);
-            w[e] *= pmul * v4.x, w[e + 1] *= pmul * v4.y, w[e + 2] *= pmul * v4.z, w[e + 3] *= pmul * v4.w;
-            if (vis != 0xffffffffu) {  // the scale of a key that is not seen
-#pragma unroll
-              for (int j = 0; j < 4; j++)
-                if (!(vis >> (16 * c + e + j) & 1)) w[e + j] = 0.f;
-            }
+            float4 v4 = *reinterpret_cast<const float4*>(&vscale[C::WIDE ? 0 : buf][part * 32 + 16 * c + e]);
+            mul2(v4.x, v4.y, pmul, pmul);
+            mul2(v4.z, v4.w, pmul, pmul);
+            mul2(w[e], w[e + 1], v4.x, v4.y);
+            mul2(w[e + 2], w[e + 3], v4.z, v4.w);
           }
+        }
+        if (!C::WIDE && vis != 0xffffffffu) {  // the scale of a key that is not seen may be anything
+#pragma unroll
+          for (int e = 0; e < 16; e++)
+            if (!(vis >> (16 * c + e) & 1)) w[e] = 0.f;
         }
         const uint32_t at = s_at + 32u * part + 16u * c;
         __syncwarp();
@@ -287,6 +308,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
           wide_st8(n < 2 ? at + 8u * n : s_at + 64u + 16u * part + 8u * c, f);
         }
       }
+      sum += s0 + s1;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
       __syncwarp();
@@ -294,20 +316,79 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
       if (i) fold(i - 1);
       if (changed) {
 #pragma unroll
-        for (int d = 0; d < D / 2; d++) out[d] *= decay;
+        for (int d = 0; d < D / 2; d += 2) mul2(out[d], out[d + 1], decay, decay);
       }
       if (++buf == C::TILES) buf = 0, phase ^= 1u;
     }
-    if (mine) fold(mine - 1);
-    const float unit = C::BF ? 1.f : C::WIDE ? 1.f / (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(vex - C::PEXP) << 23);
+    bool fine = true;
+    if (working) {
+      if (mine) fold(mine - 1);
+      const float unit = C::BF ? 1.f : C::WIDE ? 1.f / (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(vex - C::PEXP) << 23);
 #pragma unroll
-    for (int d = 0; d < D / 2; d++) out[d] *= unit;
-  } else if (warp >= 8 && warp < 12) {
+      for (int d = 0; d < D / 2; d++) {
+        out[d] *= unit;
+        fine = fine && fabsf(out[d]) < INFINITY;
+      }
+      fine = fine || row >= live_rows;
+    }
+    __syncwarp();
+    if (__syncthreads_or(!fine) && working) {
+      // ---- one by one: this thread's row and half of the dimensions, over this block's keys ----
+      top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int d = 0; d < D / 2; d++) out[d] = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < mine; i++) {
+        const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS;
+#pragma unroll 1
+        for (int e = 0; e < W_KEYS && key0 + e < keys; e++) {
+          if (!sees(a, b, tr, key0 + e - len)) continue;
+          const uint8_t *const k = kb + (key0 + e) * a.kst[2], *const v = vb + (key0 + e) * a.vst[2];
+          float s = 0.f;
+#pragma unroll 4
+          for (int d = 0; d < a.d; d++) s = fmaf(kv_float(query[d]), cached<CT>(k, ksb + key0 + e, d), s);
+          s *= a.scale * LOG2E;
+          if (!(s <= top)) {  // the maximum moves (or the score is not a number)
+            const float f = s > -INFINITY ? ex2(top - s) : 1.f;
+            sum *= f;
+#pragma unroll
+            for (int d = 0; d < D / 2; d++) out[d] *= f;
+            top = fmaxf(top, s);
+          }
+          const float p = ex2(s - (top == -INFINITY ? 0.f : top));
+          if (part == 0) sum += p;
+#pragma unroll
+          for (int d = 0; d < D / 2; d++) {
+            const int dim = part * (D / 2) + d;
+            if (dim < a.d) out[d] = fmaf(p, cached<CT>(v, vsb + key0 + e, dim), out[d]);
+          }
+        }
+      }
+    }
+    if (s_abort) {  // products still under way land before their memory is used again
+      const long long t0 = clock64();
+      while (clock64() - t0 < (1LL << 22)) {
+      }
+    }
+    __syncwarp();
+    // (all tiles have been read: the last U was awaited, and what is read above is the cache itself)
+    if (working) {
+      float* const to = so + row * C::PITCH + part * (D / 2);
+#pragma unroll
+      for (int d = 0; d < D / 2; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(out[d], out[d + 1], out[d + 2], out[d + 3]);
+      s_sum[row][part] = sum;
+      if (part == 0) s_top[row] = top;
+    }
+    __syncwarp();
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W_FEW));
+  } else if (warp < 12) {
     // ---- filling ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W_FEW));
     const int ft = tid - W_SOFTMAX, fw = warp - 8;
     constexpr int PER = C::WIDE ? D / 8 : D / 16;  // 16-byte pieces of a cached row
     constexpr int COPIES = W_KEYS * PER / W_FILL, ROWS = W_FILL / PER;
-    const int key_l = ft / PER, piece = ft % PER;
+    // 8-bit: eight lanes have four pieces of two keys, whose places in a tile are in different banks
+    const int key_l = C::WIDE || D == 64 ? ft / PER : ft / 16 * 2 + (ft >> 2 & 1), piece = C::WIDE || D == 64 ? ft % PER : (ft & 3) + (ft >> 1 & 4);
     const bool my_dims = piece * 16 < a.d * (C::WIDE ? 2 : 1);
     auto copy = [&](int i) {  // tile i of this block's: into its place, or into the raw ring
       if (i < mine) {
@@ -317,7 +398,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
         for (int j = 0; j < COPIES; j++) {
           const int key = key_l + j * ROWS;
           const bool live = my_dims && key0 + key < keys;
-          const uint32_t to = C::WIDE ? box_chunk(key, piece) : (uint32_t)(key * D + (D == 128 ? (piece ^ (key & 7)) : piece) * 16);
+          const uint32_t to = C::WIDE ? box_chunk(key, piece) : (uint32_t)(key * D + (D == 128 ? piece ^ (key & 1) << 2 : piece) * 16);
           cp16(at + to, live ? kb + (key0 + key) * a.kst[2] + piece * 16 : kb, live);
           cp16(at + (C::WIDE ? C::TILE / 2 : D * W_KEYS) + to, live ? vb + (key0 + key) * a.vst[2] + piece * 16 : vb, live);
         }
@@ -351,16 +432,14 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
         const uint32_t raw = smem_u32(smem) + (uint32_t)(C::TILES * C::TILE + i % C::RAWS * C::RAW);
 #pragma unroll
         for (int j = 0; j < 2 * COPIES; j++) {
-          const int key = key_l + j % COPIES * ROWS, at = j / COPIES * D * W_KEYS + key * D + (D == 128 ? (piece ^ (key & 7)) : piece) * 16;
+          const int key = key_l + j % COPIES * ROWS, at = j / COPIES * D * W_KEYS + key * D + (D == 128 ? piece ^ (key & 1) << 2 : piece) * 16;
           const uint4 w = lds16(raw + at);
           uint4 f[2];
           widen<C::E4M3>(w.x, &f[0].x, &f[0].y), widen<C::E4M3>(w.y, &f[0].z, &f[0].w);
           widen<C::E4M3>(w.z, &f[1].x, &f[1].y), widen<C::E4M3>(w.w, &f[1].z, &f[1].w);
           uint8_t* const half = tile + j / COPIES * (C::TILE / 2);
-          // pieces 4 .. 7 lie a box further, in the same banks as 0 .. 3: they store their halves the other way round
-          const bool turn = piece & 4;
-          *reinterpret_cast<uint4*>(half + box_chunk(key, 2 * piece + turn)) = turn ? f[1] : f[0];
-          *reinterpret_cast<uint4*>(half + box_chunk(key, 2 * piece + !turn)) = turn ? f[0] : f[1];
+          *reinterpret_cast<uint4*>(half + box_chunk(key, 2 * piece)) = f[0];
+          *reinterpret_cast<uint4*>(half + box_chunk(key, 2 * piece + 1)) = f[1];
         }
         const float scale = lds4(raw + 2 * D * W_KEYS + ft * 4);
         if (ft < W_KEYS) kscale[C::WIDE ? 0 : to][ft] = scale;
@@ -373,8 +452,10 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
       mbar_arrive(kv_full + i % C::TILES);
     }
     cp_wait<0>();
-  } else if (warp == 12 && mine) {
+    __syncthreads_or(0);
+  } else {
     // ---- issuing ----
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W_FEW));
     const uint32_t id_s = wide_idesc(W_KEYS, C::BF, false), id_u = wide_idesc(D, C::BF, true);
     const uint64_t k_desc = umma_desc(smem_u32(smem)), v_desc = wide_desc_mn(smem_u32(smem) + C::TILE / 2);
     auto scores = [&](int i) {
@@ -397,9 +478,9 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
       }
       __syncwarp();
     };
-    scores(0);
+    if (warp == 12 && mine) scores(0);
 #pragma unroll 1
-    for (int i = 0; i < mine; i++) {
+    for (int i = 0; i < mine && warp == 12; i++) {
       if (i + 1 < mine) scores(i + 1);
       wait(p_full + (i & 1), (i >> 1) & 1, 7);
       if (i) wait(&u_free, (i - 1) & 1, 8);
@@ -420,61 +501,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
       }
       __syncwarp();
     }
+    __syncthreads_or(0);
   }
-  if (s_abort) {
-    // products still under way land before their memory is used again
-    const long long t0 = clock64();
-    while (clock64() - t0 < (1LL << 22)) {
-    }
-  }
-  bool fine = true;
-#pragma unroll
-  for (int d = 0; d < D / 2; d++) fine = fine && fabsf(out[d]) < INFINITY;
-  __syncwarp();
-  if (__syncthreads_or(working && row < live_rows && !fine) && working) {
-    // ---- one by one: this thread's row and half of the dimensions, over this block's keys ----
-    top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int d = 0; d < D / 2; d++) out[d] = 0.f;
-#pragma unroll 1
-    for (int i = 0; i < mine; i++) {
-      const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS;
-#pragma unroll 1
-      for (int e = 0; e < W_KEYS && key0 + e < keys; e++) {
-        if (!sees(a, b, tr, key0 + e - len)) continue;
-        const uint8_t *const k = kb + (key0 + e) * a.kst[2], *const v = vb + (key0 + e) * a.vst[2];
-        float s = 0.f;
-#pragma unroll 4
-        for (int d = 0; d < a.d; d++) s = fmaf(kv_float(query[d]), cached<CT>(k, ksb + key0 + e, d), s);
-        s *= a.scale * LOG2E;
-        if (!(s <= top)) {  // the maximum moves (or the score is not a number)
-          const float f = s > -INFINITY ? ex2(top - s) : 1.f;
-          sum *= f;
-#pragma unroll
-          for (int d = 0; d < D / 2; d++) out[d] *= f;
-          top = fmaxf(top, s);
-        }
-        const float p = ex2(s - (top == -INFINITY ? 0.f : top));
-        if (part == 0) sum += p;
-#pragma unroll
-        for (int d = 0; d < D / 2; d++) {
-          const int dim = part * (D / 2) + d;
-          if (dim < a.d) out[d] = fmaf(p, cached<CT>(v, vsb + key0 + e, dim), out[d]);
-        }
-      }
-    }
-  }
-  __syncwarp();
-  __syncthreads();  // nobody reads tiles any more
-  float* const so = reinterpret_cast<float*>(smem);
-  if (working) {
-    float* const to = so + row * C::PITCH + part * (D / 2);
-#pragma unroll
-    for (int d = 0; d < D / 2; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(out[d], out[d + 1], out[d + 2], out[d + 3]);
-    s_sum[row][part] = sum;
-    if (part == 0) s_top[row] = top;
-  }
-  __syncwarp();
   if (a.splits > 1)
     asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
   else
@@ -522,6 +550,14 @@ int run_wide(TreeArgs a, cudaStream_t s) {
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), C::SMEM)) return 1;
   int* const error = device_error_word();
   if (!error) return 1;
+  // the shares above come out of what the compiler gave the launch: with fewer registers a warp would wait for more without end
+  static std::atomic<int> launch_regs{0};
+  if (!launch_regs) {
+    cudaFuncAttributes attr;
+    DYN_CUDA(cudaFuncGetAttributes(&attr, kernel));
+    launch_regs = attr.numRegs;
+  }
+  DYN_CHECK(launch_regs * W_THREADS >= W_SOFTMAX * W_MANY + (W_THREADS - W_SOFTMAX) * W_FEW, "tree_attention: built with %d registers a thread", launch_regs.load());
   const int64_t pairs = a.batch * a.kv_heads;
   a.row_blocks = (int)(((int64_t)a.rows * a.group + W_ROWS - 1) / W_ROWS);
   // blocks of a cluster: as many as fit the SMs at once (a block takes an SM), at least two tiles each at full capacity

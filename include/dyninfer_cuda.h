@@ -195,8 +195,8 @@ int dyninfer_cuda_kv_read(void* k_dev, void* v_dev, int type, const int64_t* x_s
  * mask[b, r, j] is not zero (strides: batch, row; a batch stride of 0 shares one mask); mask NULL:
  * where j <= r. Keys from kv_cap on do not exist; a row that sees nothing gets zeros, and so do all
  * rows of an entry whose length is below zero. ctx [batch, rows, heads, d] is dense, of q's type.
- * kv_type F16, BF16, or an 8-bit type with its scales (as kv_write lays them out). d is a multiple
- * of 16 up to 128. */
+ * kv_type F16, BF16, or an 8-bit type with its scales (as kv_write lays them out). scale is above
+ * zero. d is a multiple of 16 up to 128. */
 int dyninfer_cuda_tree_attention(const void* q_dev, int q_type, const int64_t* q_strides, const void* k_cache_dev,
                                  const void* v_cache_dev, int kv_type, const int64_t* cache_strides,
                                  const float* k_scale_dev, const float* v_scale_dev, const int64_t* scale_strides,

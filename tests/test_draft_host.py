@@ -135,7 +135,8 @@ def test_native_tree_attention_refusals(native_lib):
     native_refusal("tree_attention", "head dim 136", *call(d=136))
     native_refusal("tree_attention", "multiple of kv heads", *call(heads=3, kv=2))
     native_refusal("tree_attention", "bad shape", *call(cap=0))
-    native_refusal("tree_attention", "scale is not finite", *call(scale=math.nan))
+    for scale in (math.nan, math.inf, 0.0, -1.0):
+        native_refusal("tree_attention", "scale must be above zero", *call(scale=scale))
     native_refusal("tree_attention", "needs its scales", *call(ks=None))
     native_refusal("tree_attention", "needs its strides", *call(mask=AT))
     native_refusal("tree_attention", "multiples of 16", *call(k=AT + 4))
