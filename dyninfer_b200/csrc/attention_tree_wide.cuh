@@ -2,12 +2,13 @@
 //
 // One block = 128 rows (tokens x query heads of one kv head), the 128 lanes of tensor memory, and a share of the keys in tiles of
 // 64; the blocks of a cluster take the tiles in turn and merge their states through shared memory. Roles:
-//   8 softmax warps   two threads share a row: each has half of a tile's scores and half of the output's dimensions. They turn S
-//                     into P (terms side by side, in place of S) and add the product before, U, to 64 f32 sums.
+//   two streams of four softmax warps, a thread per row: they take a block's tiles in turn, each with a running (maximum, sum, output) of
+//                     its own, so that the latencies and the exponentials of the one run beside the products of the other. A thread turns
+//                     S into P (terms side by side, in place of S) and adds U = P V to its row's f32 sums.
 //   4 filling warps   bring keys and values into shared memory as swizzled 16-bit tiles: 2-byte caches by asynchronous copies
 //                     straight to their places, 8-bit ones by way of a ring of raw tiles, converted on the way.
-//   1 issuing warp    S(i+1) = Q K^T while the softmax warps are at tile i, U(i) = P V while they are at tile i + 1; S has two
-//                     places in tensor memory, Q (up to three terms) lies there as well.
+//   an issuing warp per stream. Q (up to three terms) lies in tensor memory, beside S and U of the streams; an f32 query over a bf16
+//                     cache has three terms of Q and P, whose columns leave room for one stream only.
 // Scores, references, slack, terms and units are those of attention_tree.cuh. Where a result is not finite (weight 0 times
 // an infinity in a key that a row does not see), the block's rows are computed once more one by one, without tensor cores.
 // All waits are bounded; one that runs out leaves a code in the device's error word.
@@ -21,11 +22,7 @@
 namespace dyn {
 namespace tree {
 
-constexpr int W_ROWS = 128, W_KEYS = 64, W_SOFTMAX = 256, W_FILL = 128;
-constexpr int W_THREADS = W_SOFTMAX + W_FILL + 128;  // whole warpgroups, because registers are dealt out per group
-// 512 threads start with 128 registers each; 256 x 168 + 256 x 88 is the same
-constexpr int W_MANY = 168, W_FEW = 88;
-static_assert(W_SOFTMAX * W_MANY + (W_THREADS - W_SOFTMAX) * W_FEW <= W_THREADS * 128, "the groups' shares come out of the launch's registers");
+constexpr int W_ROWS = 128, W_KEYS = 64, W_FILL = 128;
 constexpr int W_BOX = W_KEYS * 128;  // bytes of 64 keys x 64 two-byte dimensions
 
 template <int CT, typename TQ, int D_>
@@ -36,25 +33,30 @@ struct Wide {
   static constexpr int QT = BF ? (QB ? 1 : QF ? 3 : 2) : (QF ? 2 : 1), PT = BF ? (QF ? 3 : 2) : (QB ? 1 : 2);
   static constexpr float SLACK = QF ? 0.f : 8.f;
   static constexpr int PEXP = QF ? 13 : 5;
+  static constexpr int NS = PT == 3 ? 1 : 2;   // streams
+  // whole warpgroups, because registers are dealt out per group: the softmax threads of the streams, fillers, issuing warps
+  static constexpr int SOFTMAX = NS * W_ROWS, THREADS = SOFTMAX + W_FILL + 128;
+  // 512 threads start with 128 registers each, 384 with 168
+  static constexpr int START = NS == 2 ? 128 : 168, MANY = NS == 2 ? 200 : 232, FEW = NS == 2 ? 56 : 136;
+  static_assert(SOFTMAX * MANY + (THREADS - SOFTMAX) * FEW <= THREADS * START, "the groups' shares come out of the launch's registers");
   // tensor memory columns
-  static constexpr int S_COLS = PT == 3 ? 96 : 64, U_COL = 2 * S_COLS, Q_COL = U_COL + D;
-  static_assert(Q_COL + QT * (D / 2) <= 512, "tensor memory has 512 columns");
+  static constexpr int S_COLS = PT == 3 ? 96 : 64, STREAM = S_COLS + D_, Q_COL = NS * STREAM;  // a stream: S, then U
+  static_assert(Q_COL + QT * (D_ / 2) <= 512, "tensor memory has 512 columns");
+  // products' descriptors: kind::f16, f32 accumulator, M = 128, N at bit 17; bf16 operands; B contiguous along N
+  static constexpr uint32_t ID = (1u << 4) | (8u << 24) | (BF ? (1u << 7) | (1u << 10) : 0u);
+  static constexpr uint32_t ID_S = ID | (64u >> 3 << 17), ID_U = ID | ((uint32_t)D_ >> 3 << 17) | (1u << 16);
   // shared memory: tiles (keys, then values), the values' and keys' scales, raw tiles
   static constexpr int TILE = 2 * D * W_KEYS * 2, TILES = WIDE ? 5 : 4;
   static constexpr int RAW = WIDE ? 0 : 2 * D * W_KEYS + 2 * W_KEYS * 4, RAWS = 3;
   static constexpr int PITCH = D + 4;  // floats of a row's final state
   static constexpr int BODY = TILE * TILES + RAW * RAWS;
-  static_assert(W_ROWS * PITCH * 4 <= BODY, "the final states take the tiles' place");
+  static_assert(NS * W_ROWS * PITCH * 4 <= BODY, "the final states take the tiles' place");
   // A block waits for its columns of tensor memory and then for its cluster, so no two blocks of that kind may share an SM: this
   // much shared memory leaves no room for another one of this kernel, nor for one of the other kernels that do both (77 KB and more)
   static constexpr int SMEM = BODY + 1024 > 152 * 1024 ? BODY + 1024 : 152 * 1024;
   static_assert(SMEM + 1024 + 78 * 1024 > 228 * 1024 && SMEM <= 220 * 1024, "see above");
 };
 
-// kind::f16, M = 128, N = n; BF: bf16 operands; mn: B contiguous along N
-__device__ __forceinline__ uint32_t wide_idesc(int n, bool bf, bool mn) {
-  return umma_idesc(n) | (bf ? (1u << 7) | (1u << 10) : 0u) | (mn ? 1u << 16 : 0u);
-}
 // B operand contiguous along N, 128-byte swizzle: a 128-byte row per K element with 64 elements of N; the next 64 a box further
 __device__ __forceinline__ uint64_t wide_desc_mn(uint32_t at) {
   return (uint64_t)((at >> 4) & 0x3fff) | ((uint64_t)(W_BOX >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
@@ -88,18 +90,17 @@ __device__ __forceinline__ float cached(const uint8_t* row, const float* scale, 
 }
 
 template <int CT, typename TQ, int D>
-__global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const __grid_constant__ TreeArgs a, int* error) {
+__global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wide_kernel(const __grid_constant__ TreeArgs a, int* error) {
   using C = Wide<CT, TQ, D>;
   using O = Op<C::BF>;
   extern __shared__ uint8_t wide_shared[];
-  __shared__ uint64_t kv_full[C::TILES], kv_free[C::TILES], s_full[2], p_full[2], u_full, u_free;
+  __shared__ uint64_t kv_full[C::TILES], kv_free[C::TILES], q_full, s_full[C::NS], p_full[C::NS], u_full[C::NS];
   __shared__ uint32_t tmem_base_s;
   __shared__ int s_abort;
   __shared__ __align__(16) float kscale[C::WIDE ? 1 : C::TILES][W_KEYS], vscale[C::WIDE ? 1 : C::TILES][W_KEYS];  // read by fours
-  __shared__ int vexp[C::TILES][4];               // exponents of the tile's largest value scale, of four filling warps
-  __shared__ float s_most[2][2][W_ROWS];          // [parity][half][row]
-  __shared__ __align__(16) float s_sum[W_ROWS][2];  // read by twos
-  __shared__ float s_top[W_ROWS];
+  __shared__ int vexp[C::TILES][4];                           // exponents of the tile's largest value scale, of four filling warps
+  __shared__ float s_mult[W_ROWS];                            // what a row's scores are multiplied with
+  __shared__ __align__(16) float s_state[C::NS][W_ROWS][2];   // (maximum, sum), read by twos
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(wide_shared) + 1023) & ~uintptr_t(1023));
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const int split = (int)blockIdx.x % a.splits;
@@ -107,7 +108,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
   const int64_t b = pair / a.kv_heads;
   const int kvh = (int)(pair - b * a.kv_heads);
   const int row0 = blockIdx.y * W_ROWS, live_rows = min(W_ROWS, a.rows * a.group - row0);
-  const int live_warps = 2 * ((live_rows + 31) / 32);
+  const int live_warps = (live_rows + 31) / 32;  // of a stream
 
   int64_t len = a.lengths[b], keys = 0;
   if (len >= 0) {
@@ -124,11 +125,12 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
   if (tid == 0) {
     s_abort = 0;
     for (int i = 0; i < C::TILES; i++) mbar_init(kv_full + i, W_FILL), mbar_init(kv_free + i, 1);
-    for (int i = 0; i < 2; i++) mbar_init(s_full + i, 1), mbar_init(p_full + i, live_warps);
-    mbar_init(&u_full, 1), mbar_init(&u_free, live_warps);
+    for (int i = 0; i < C::NS; i++) mbar_init(s_full + i, 1), mbar_init(p_full + i, live_warps), mbar_init(u_full + i, 1);
+    mbar_init(&q_full, live_warps);
     mbar_fence_init();
   }
-  if (warp == 12) {
+  constexpr int ISSUING = (C::SOFTMAX + W_FILL) / 32;  // the first issuing warp
+  if (warp == ISSUING) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -140,205 +142,218 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
     if (!mbar_wait_bounded(bar, parity, TG_SPINS, &s_abort) && !s_abort) s_abort = code;
   };
 
-  const int row = (warp & 3) * 32 + lane, part = (warp >> 2) & 1;   // of a softmax thread
-  const bool working = warp < 8 && (warp & 3) * 32 < live_rows;
-  const uint32_t tlane = (uint32_t)((warp & 3) * 32) << 16;
-  const int row_index = row0 + min(row, live_rows - 1), tr = row_index / a.group, gh = row_index - tr * a.group;
-  const TQ* const query = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
   float* const so = reinterpret_cast<float*>(smem);  // the final states, in the tiles' place
-  float mult = 0.f;
-
-  if (working && mine) {
-    // ---- Q into tensor memory: this thread's half of the row ----
-    float mul = 1.f, inv = 1.f;
-    if (!C::BF) {
-      float most = 0.f;
-#pragma unroll 8
-      for (int d = 0; d < D / 2; d++)
-        if (part * (D / 2) + d < a.d) most = fmaxf(most, fabsf(kv_float(query[part * (D / 2) + d])));
-      s_most[0][part][row] = most;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
-      most = fmaxf(most, s_most[0][part ^ 1][row]);
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
-      int ex = (int)((__float_as_uint(most) >> 23) & 0xff);
-      ex = ex < 20 ? 20 : ex > 250 ? 250 : ex;
-      mul = __uint_as_float((uint32_t)(262 - ex) << 23), inv = __uint_as_float((uint32_t)(ex - 8) << 23);
-    }
-    mult = fmaxf(a.scale * LOG2E * inv, 1.2e-38f);  // above zero: -infinity stays itself
-#pragma unroll 1
-    for (int s = 0; s < D / 32; s++) {
-      float x[16];
+  if (warp < C::SOFTMAX / 32) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::MANY));
+    const int stream = warp / 4, row = (warp & 3) * 32 + lane;
+    const bool working = (warp & 3) * 32 < live_rows && mine;
+    const uint32_t tlane = (uint32_t)((warp & 3) * 32) << 16;
+    const int row_index = row0 + min(row, live_rows - 1), tr = row_index / a.group, gh = row_index - tr * a.group;
+    const TQ* const query = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
+    if (working && stream == 0) {
+      // ---- Q into tensor memory ----
+      float x[D];
+      constexpr int N = 16 / sizeof(TQ);
+      // 16 bytes at a time where the rows are aligned (whole pieces are in or out: d is a multiple of 16 dimensions)
+      if (((reinterpret_cast<uintptr_t>(a.q) | (a.qs[0] | a.qs[1] | a.qs[2]) * sizeof(TQ)) & 15) == 0) {
 #pragma unroll
-      for (int e = 0; e < 16; e++) {
-        const int dim = part * (D / 2) + s * 16 + e;
-        x[e] = dim < a.d ? kv_float(query[dim]) * mul : 0.f;
+        for (int d = 0; d < D; d += N) {
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (d < a.d) w = *reinterpret_cast<const uint4*>(query + d);
+          const TQ* const e = reinterpret_cast<const TQ*>(&w);
+#pragma unroll
+          for (int j = 0; j < N; j++) x[d + j] = kv_float(e[j]);
+        }
+      } else {
+#pragma unroll
+        for (int d = 0; d < D; d++) x[d] = d < a.d ? kv_float(query[d]) : 0.f;
       }
+      float mul = 1.f, inv = 1.f;
+      if (!C::BF) {
+        float most = 0.f;
 #pragma unroll
-      for (int n = 0; n < C::QT; n++) {
-        uint32_t f[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) f[e] = O::take(x[2 * e], x[2 * e + 1]);
-        __syncwarp();
-        wide_st8(tmem + tlane + C::Q_COL + n * (D / 2) + part * (D / 4) + s * 8, f);
+        for (int d = 0; d < D; d++) most = fmaxf(most, fabsf(x[d]));
+        int ex = (int)((__float_as_uint(most) >> 23) & 0xff);
+        ex = ex < 20 ? 20 : ex > 250 ? 250 : ex;
+        mul = __uint_as_float((uint32_t)(262 - ex) << 23), inv = __uint_as_float((uint32_t)(ex - 8) << 23);
       }
-    }
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-    tc_fence_before();
-  }
-  __syncthreads();  // Q is complete
-  tc_fence_after();
-
-  if (warp < 8) {
-    // ---- softmax ----
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(W_MANY));
-    float out[D / 2], top = -INFINITY, sum = 0.f;
-    int vex = 30;  // 8-bit: exponent that value scales are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
-#pragma unroll
-    for (int d = 0; d < D / 2; d++) out[d] = 0.f;
-    const uint32_t u_at = tmem + tlane + C::U_COL + (uint32_t)part * (D / 2);
-    auto fold = [&](int i) {  // U of tile i
-      wait(&u_full, i & 1, 3);
+      s_mult[row] = fmaxf(a.scale * LOG2E * inv, 1.2e-38f);  // above zero: -infinity stays itself
       __syncwarp();
-      tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < D / 32; c += 2) {
-        uint32_t u[2][16];
-        tmem_ld16(u_at + 16u * c, u[0]);
-        if (c + 1 < D / 32) tmem_ld16(u_at + 16u * c + 16u, u[1]);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      for (int s = 0; s < D / 16; s++) {
 #pragma unroll
-        for (int e = 0; e < 32 && 16 * c + e < D / 2; e += 2)
-          add2(out[16 * c + e], out[16 * c + e + 1], __uint_as_float(u[e >> 4][e & 15]), __uint_as_float(u[e >> 4][(e & 15) + 1]));
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&u_free);
-    };
-    int buf = 0;
-    unsigned phase = 0;
-#pragma unroll 1
-    for (int i = 0; i < mine && working; i++) {
-      const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS + part * 32;
-      const uint32_t s_at = tmem + tlane + (uint32_t)((i & 1) * C::S_COLS);
-      uint32_t vis = 0xffffffffu;
-      if (key0 + 32 > len) {
-        vis = 0;
-#pragma unroll 1
-        for (int e = 0; e < 32; e++)
-          if (key0 + e < keys && sees(a, b, tr, key0 + e - len)) vis |= 1u << e;
-      }
-      wait(s_full + (i & 1), (i >> 1) & 1, 1);
-      if (!C::WIDE) wait(kv_full + buf, phase, 2);  // for the scales
-      __syncwarp();
-      tc_fence_after();
-      uint32_t raw[2][16];
-      tmem_ld16(s_at + 32u * part, raw[0]);
-      tmem_ld16(s_at + 32u * part + 16u, raw[1]);
-      float grow = 1.f;
-      if (!C::WIDE) {
-        const int ex = max(vexp[buf][2], vexp[buf][3]);
-        if (ex > vex) grow = ex2((float)(vex - ex)), vex = ex;
-      }
-      const float pmul = C::BF ? 1.f : C::WIDE ? (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(254 + C::PEXP - vex) << 23);
-      asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-      float x[32];
+        for (int e = 0; e < 16; e++) x[16 * s + e] *= mul;
 #pragma unroll
-      for (int e = 0; e < 32; e++) x[e] = __uint_as_float(raw[e >> 4][e & 15]);
-      if (!C::WIDE) {
+        for (int n = 0; n < C::QT; n++) {
+          uint32_t f[8];
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 k4 = *reinterpret_cast<const float4*>(&kscale[C::WIDE ? 0 : buf][part * 32 + e]);
-          mul2(x[e], x[e + 1], k4.x, k4.y);
-          mul2(x[e + 2], x[e + 3], k4.z, k4.w);
+          for (int e = 0; e < 8; e++) f[e] = O::take(x[16 * s + 2 * e], x[16 * s + 2 * e + 1]);
+          wide_st8(tmem + tlane + C::Q_COL + n * (D / 2) + s * 8, f);
         }
       }
-      if (vis != 0xffffffffu) {
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full);
+    }
+    // ---- softmax ----
+    float out[D], top = -INFINITY, sum = 0.f, mult = 0.f;
+    int vex = 30;  // 8-bit: exponent that value scales are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
 #pragma unroll
-        for (int e = 0; e < 32; e++)
-          if (!(vis >> e & 1)) x[e] = -INFINITY;
+    for (int d = 0; d < D; d++) out[d] = 0.f;
+    if (working) {
+      wait(&q_full, 0, 9);
+      mult = s_mult[row];
+    }
+    const uint32_t s_at = tmem + tlane + (uint32_t)(stream * C::STREAM), u_at = s_at + C::S_COLS;
+    int buf = stream;
+    unsigned phase = 0, parity = 0;
+#pragma unroll 1
+    for (int i = stream; i < mine && working; i += C::NS) {
+      const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS;
+      uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+      if (key0 + W_KEYS > len) {
+        vis[0] = vis[1] = 0;
+#pragma unroll 1
+        for (int e = 0; e < W_KEYS; e++)
+          if (key0 + e < keys && sees(a, b, tr, key0 + e - len)) {
+            if (e < 32) vis[0] |= 1u << e;
+            else vis[1] |= 1u << (e - 32);
+          }
       }
-      float best = x[0], other = x[1];
+      if (!C::WIDE) wait(kv_full + buf, phase, 2);  // for the scales
+      wait(s_full + stream, parity, 1);
+      __syncwarp();
+      tc_fence_after();
+      float decay = 1.f;
+      if (!C::WIDE) {
+        const int ex = max(vexp[buf][2], vexp[buf][3]);
+        if (ex > vex) decay = ex2((float)(vex - ex)), vex = ex;
+      }
+      const float pmul = C::BF ? 1.f : C::WIDE ? (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(254 + C::PEXP - vex) << 23);
+      // half of a tile's scores, in the row's units; -infinity for keys that are not seen
+      auto half = [&](int h, float (&x)[32]) {
+        uint32_t raw[2][16];
+        tmem_ld16(s_at + 32u * h, raw[0]);
+        tmem_ld16(s_at + 32u * h + 16u, raw[1]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-      for (int e = 2; e < 32; e += 2) best = fmaxf(best, x[e]), other = fmaxf(other, x[e + 1]);
-      best = fmaxf(fmaxf(best, other), -INFINITY) * mult;  // the factor is above zero
-      s_most[i & 1][part][row] = best;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
-      best = fmaxf(best, s_most[i & 1][part ^ 1][row]);
-      float decay = grow;
+        for (int e = 0; e < 32; e++) x[e] = __uint_as_float(raw[e >> 4][e & 15]);
+        if (!C::WIDE) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(&kscale[C::WIDE ? 0 : buf][32 * h + e]);
+            mul2(x[e], x[e + 1], k4.x, k4.y);
+            mul2(x[e + 2], x[e + 3], k4.z, k4.w);
+          }
+        }
+        if (vis[h] != 0xffffffffu) {
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (!(vis[h] >> e & 1)) x[e] = -INFINITY;
+        }
+        __syncwarp();
+      };
+      float best = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float x[32];
+        half(h, x);
+        float m0 = x[0], m1 = x[1];
+#pragma unroll
+        for (int e = 2; e < 32; e += 2) m0 = fmaxf(m0, x[e]), m1 = fmaxf(m1, x[e + 1]);
+        best = fmaxf(best, fmaxf(m0, m1));
+      }
+      best *= mult;  // which is above zero
       if (best > top + C::SLACK || top == -INFINITY) {
         const float f = ex2(top - (best == -INFINITY ? 0.f : best));
         decay *= f, sum *= f, top = best;
       }
-      const bool changed = __any_sync(0xffffffffu, decay != 1.f);
+      if (__any_sync(0xffffffffu, decay != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < D; d += 2) mul2(out[d], out[d + 1], decay, decay);
+      }
       const float base = top == -INFINITY ? 0.f : top;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; c++) {
-        float* const w = x + 16 * c;
+      for (int h = 0; h < 2; h++) {
+        float x[32];
+        half(h, x);
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          fms2(w[e], w[e + 1], mult, base);
-          w[e] = ex2(w[e]), w[e + 1] = ex2(w[e + 1]);
-          add2(s0, s1, w[e], w[e + 1]);
-        }
+        for (int c = 0; c < 2; c++) {
+          float* const w = x + 16 * c;
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          if (C::WIDE) {
-            if (!C::BF) mul2(w[e], w[e + 1], pmul, pmul), mul2(w[e + 2], w[e + 3], pmul, pmul);
-          } else {
-            float4 v4 = *reinterpret_cast<const float4*>(&vscale[C::WIDE ? 0 : buf][part * 32 + 16 * c + e]);
-            mul2(v4.x, v4.y, pmul, pmul);
-            mul2(v4.z, v4.w, pmul, pmul);
-            mul2(w[e], w[e + 1], v4.x, v4.y);
-            mul2(w[e + 2], w[e + 3], v4.z, v4.w);
+          for (int e = 0; e < 16; e += 2) {
+            fms2(w[e], w[e + 1], mult, base);
+            w[e] = ex2(w[e]), w[e + 1] = ex2(w[e + 1]);
+            add2(s0, s1, w[e], w[e + 1]);
           }
-        }
-        if (!C::WIDE && vis != 0xffffffffu) {  // the scale of a key that is not seen may be anything
 #pragma unroll
-          for (int e = 0; e < 16; e++)
-            if (!(vis >> (16 * c + e) & 1)) w[e] = 0.f;
-        }
-        const uint32_t at = s_at + 32u * part + 16u * c;
-        __syncwarp();
+          for (int e = 0; e < 16; e += 4) {
+            if (C::WIDE) {
+              if (!C::BF) mul2(w[e], w[e + 1], pmul, pmul), mul2(w[e + 2], w[e + 3], pmul, pmul);
+            } else {
+              float4 v4 = *reinterpret_cast<const float4*>(&vscale[C::WIDE ? 0 : buf][32 * h + 16 * c + e]);
+              mul2(v4.x, v4.y, pmul, pmul);
+              mul2(v4.z, v4.w, pmul, pmul);
+              mul2(w[e], w[e + 1], v4.x, v4.y);
+              mul2(w[e + 2], w[e + 3], v4.z, v4.w);
+            }
+          }
+          if (!C::WIDE && vis[h] != 0xffffffffu) {  // the scale of a key that is not seen may be anything
 #pragma unroll
-        for (int n = 0; n < C::PT; n++) {
-          uint32_t f[8];
+            for (int e = 0; e < 16; e++)
+              if (!(vis[h] >> (16 * c + e) & 1)) w[e] = 0.f;
+          }
+          __syncwarp();
 #pragma unroll
-          for (int e = 0; e < 8; e++) f[e] = O::take(w[2 * e], w[2 * e + 1]);
-          wide_st8(n < 2 ? at + 8u * n : s_at + 64u + 16u * part + 8u * c, f);
+          for (int n = 0; n < C::PT; n++) {
+            uint32_t f[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e] = O::take(w[2 * e], w[2 * e + 1]);
+            wide_st8(s_at + (n < 2 ? 32u * h + 16u * c + 8u * n : 64u + 16u * h + 8u * c), f);
+          }
         }
       }
       sum += s0 + s1;
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + (i & 1));
-      if (i) fold(i - 1);
-      if (changed) {
+      if (lane == 0) mbar_arrive(p_full + stream);
+      wait(u_full + stream, parity, 3);
+      __syncwarp();
+      tc_fence_after();
 #pragma unroll
-        for (int d = 0; d < D / 2; d += 2) mul2(out[d], out[d + 1], decay, decay);
+      for (int c = 0; c < D / 16; c += 2) {
+        uint32_t u[2][16];
+        tmem_ld16(u_at + 16u * c, u[0]);
+        tmem_ld16(u_at + 16u * c + 16u, u[1]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+          add2(out[16 * c + e], out[16 * c + e + 1], __uint_as_float(u[e >> 4][e & 15]), __uint_as_float(u[e >> 4][(e & 15) + 1]));
       }
-      if (++buf == C::TILES) buf = 0, phase ^= 1u;
+      tc_fence_before();
+      parity ^= 1u;
+      buf += C::NS;
+      if (buf >= C::TILES) buf -= C::TILES, phase ^= 1u;
     }
     bool fine = true;
-    if (working) {
-      if (mine) fold(mine - 1);
-      const float unit = C::BF ? 1.f : C::WIDE ? 1.f / (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(vex - C::PEXP) << 23);
+    const float unit = C::BF ? 1.f : C::WIDE ? 1.f / (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(vex - C::PEXP) << 23);
 #pragma unroll
-      for (int d = 0; d < D / 2; d++) {
-        out[d] *= unit;
-        fine = fine && fabsf(out[d]) < INFINITY;
-      }
-      fine = fine || row >= live_rows;
+    for (int d = 0; d < D; d++) {
+      out[d] *= unit;
+      fine = fine && fabsf(out[d]) < INFINITY;
     }
+    fine = fine || row >= live_rows;
     __syncwarp();
     if (__syncthreads_or(!fine) && working) {
-      // ---- one by one: this thread's row and half of the dimensions, over this block's keys ----
+      // ---- one by one: this thread's row over this stream's keys ----
       top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int d = 0; d < D / 2; d++) out[d] = 0.f;
+      for (int d = 0; d < D; d++) out[d] = 0.f;
 #pragma unroll 1
-      for (int i = 0; i < mine; i++) {
+      for (int i = stream; i < mine; i += C::NS) {
         const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS;
 #pragma unroll 1
         for (int e = 0; e < W_KEYS && key0 + e < keys; e++) {
@@ -352,16 +367,14 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
             const float f = s > -INFINITY ? ex2(top - s) : 1.f;
             sum *= f;
 #pragma unroll
-            for (int d = 0; d < D / 2; d++) out[d] *= f;
+            for (int d = 0; d < D; d++) out[d] *= f;
             top = fmaxf(top, s);
           }
           const float p = ex2(s - (top == -INFINITY ? 0.f : top));
-          if (part == 0) sum += p;
+          sum += p;
 #pragma unroll
-          for (int d = 0; d < D / 2; d++) {
-            const int dim = part * (D / 2) + d;
-            if (dim < a.d) out[d] = fmaf(p, cached<CT>(v, vsb + key0 + e, dim), out[d]);
-          }
+          for (int d = 0; d < D; d++)
+            if (d < a.d) out[d] = fmaf(p, cached<CT>(v, vsb + key0 + e, d), out[d]);
         }
       }
     }
@@ -371,20 +384,19 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
       }
     }
     __syncwarp();
-    // (all tiles have been read: the last U was awaited, and what is read above is the cache itself)
-    if (working) {
-      float* const to = so + row * C::PITCH + part * (D / 2);
+    // (all tiles have been read: the streams' last U were awaited, and what is read above is the cache itself)
+    if ((warp & 3) * 32 < live_rows) {
+      float* const to = so + (stream * W_ROWS + row) * C::PITCH;
 #pragma unroll
-      for (int d = 0; d < D / 2; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(out[d], out[d + 1], out[d + 2], out[d + 3]);
-      s_sum[row][part] = sum;
-      if (part == 0) s_top[row] = top;
+      for (int d = 0; d < D; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(out[d], out[d + 1], out[d + 2], out[d + 3]);
+      s_state[stream][row][0] = top, s_state[stream][row][1] = sum;
     }
     __syncwarp();
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W_FEW));
-  } else if (warp < 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEW));
+  } else if (warp < ISSUING) {
     // ---- filling ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W_FEW));
-    const int ft = tid - W_SOFTMAX, fw = warp - 8;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEW));
+    const int ft = tid - C::SOFTMAX, fw = ft / 32;
     constexpr int PER = C::WIDE ? D / 8 : D / 16;  // 16-byte pieces of a cached row
     constexpr int COPIES = W_KEYS * PER / W_FILL, ROWS = W_FILL / PER;
     // 8-bit: eight lanes have four pieces of two keys, whose places in a tile are in different banks
@@ -455,51 +467,56 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
     __syncthreads_or(0);
   } else {
     // ---- issuing ----
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(W_FEW));
-    const uint32_t id_s = wide_idesc(W_KEYS, C::BF, false), id_u = wide_idesc(D, C::BF, true);
-    const uint64_t k_desc = umma_desc(smem_u32(smem)), v_desc = wide_desc_mn(smem_u32(smem) + C::TILE / 2);
-    auto scores = [&](int i) {
-      const int buf = i % C::TILES;
-      wait(kv_full + buf, (i / C::TILES) & 1, 5);
-      if (i >= 2) wait(&u_full, (i - 2) & 1, 6);  // P of tile i - 2 has been read
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEW));
+    // the reductions only bring what every lane has into uniform registers, where the products' operands come from
+    const int stream = warp - ISSUING, n_tiles = (int)__reduce_max_sync(0xffffffffu, (unsigned)mine);
+    const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem), at = __reduce_max_sync(0xffffffffu, smem_u32(smem));
+    const uint32_t s_col = tm + (uint32_t)(stream * C::STREAM), u_col = s_col + C::S_COLS;
+    const uint64_t k_desc = umma_desc(at), v_desc = wide_desc_mn(at + C::TILE / 2);
+    int buf = stream;
+    unsigned phase = 0, parity = 0;
+    auto scores = [&] {
+      wait(kv_full + buf, phase, 5);
       tc_fence_after();
+      const uint64_t k = k_desc + (uint64_t)(buf * (C::TILE >> 4));
       if (elect_one()) {
-        const uint64_t k = k_desc + (uint64_t)(buf * (C::TILE >> 4));
-        const uint32_t to = tmem + (uint32_t)((i & 1) * C::S_COLS);
-        bool more = false;
 #pragma unroll
         for (int n = C::QT - 1; n >= 0; n--)  // the small terms first
 #pragma unroll
-          for (int s = 0; s < D / 16; s++) {
-            umma_f16_ts(to, tmem + C::Q_COL + n * (D / 2) + 8u * s, k + (uint64_t)((s >> 2) * (W_BOX >> 4) + 2 * (s & 3)), id_s, more ? 1u : 0u);
-            more = true;
-          }
-        umma_commit(s_full + (i & 1));
+          for (int s = 0; s < D / 16; s++)
+            umma_f16_ts(s_col, tm + C::Q_COL + n * (D / 2) + 8u * s, k + (uint64_t)((s >> 2) * (W_BOX >> 4) + 2 * (s & 3)), C::ID_S,
+                        n == C::QT - 1 && s == 0 ? 0u : 1u);
+        umma_commit(s_full + stream);
       }
       __syncwarp();
     };
-    if (warp == 12 && mine) scores(0);
+    if (stream < C::NS && stream < n_tiles) {
+      wait(&q_full, 0, 6);
+      scores();
 #pragma unroll 1
-    for (int i = 0; i < mine && warp == 12; i++) {
-      if (i + 1 < mine) scores(i + 1);
-      wait(p_full + (i & 1), (i >> 1) & 1, 7);
-      if (i) wait(&u_free, (i - 1) & 1, 8);
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t v = v_desc + (uint64_t)(i % C::TILES * (C::TILE >> 4));
-        const uint32_t p = tmem + (uint32_t)((i & 1) * C::S_COLS);
-        bool more = false;
+      for (int i = stream; i < n_tiles; i += C::NS) {
+        wait(p_full + stream, parity, 7);  // (the U before has been read as well)
+        tc_fence_after();
+        const uint64_t v = v_desc + (uint64_t)(buf * (C::TILE >> 4));
+        if (elect_one()) {
 #pragma unroll
-        for (int n = C::PT - 1; n >= 0; n--)
+          for (int n = C::PT - 1; n >= 0; n--)
 #pragma unroll
-          for (int s = 0; s < W_KEYS / 16; s++) {
-            umma_f16_ts(tmem + C::U_COL, n < 2 ? p + 16u * s + 8u * n : p + 64u + 8u * s, v + (uint64_t)(s * (2048 >> 4)), id_u, more ? 1u : 0u);
-            more = true;
-          }
-        umma_commit(&u_full);
-        umma_commit(kv_free + i % C::TILES);
+            for (int s = 0; s < W_KEYS / 16; s++)
+              umma_f16_ts(u_col, s_col + (n < 2 ? 16u * s + 8u * n : 64u + 8u * s), v + (uint64_t)(s * (2048 >> 4)), C::ID_U,
+                          n == C::PT - 1 && s == 0 ? 0u : 1u);
+          umma_commit(u_full + stream);
+          umma_commit(kv_free + buf);
+        }
+        __syncwarp();
+        buf += C::NS;
+        if (buf >= C::TILES) buf -= C::TILES, phase ^= 1u;
+        if (i + C::NS < n_tiles) {
+          wait(u_full + stream, parity, 8);  // P has been read
+          scores();
+        }
+        parity ^= 1u;
       }
-      __syncwarp();
     }
     __syncthreads_or(0);
   }
@@ -507,25 +524,26 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
     asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");
   else
     __syncthreads();
-  const uint32_t so_at = smem_u32(so), top_at = smem_u32(s_top), sum_at = smem_u32(&s_sum[0][0]);
-  for (int i = split * W_THREADS + tid; i < live_rows * (D / 4); i += a.splits * W_THREADS) {
+  const uint32_t so_at = smem_u32(so), state_at = smem_u32(&s_state[0][0][0]);
+  for (int i = split * C::THREADS + tid; i < live_rows * (D / 4); i += a.splits * C::THREADS) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
     float m = -INFINITY, l = 0.f, o[4] = {};
     for (int p = 0; p < a.splits; p++) {
-      uint32_t at_m, at_l, at_o;
-      float pm, l0, l1, x[4];
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_m) : "r"(top_at + (uint32_t)r * 4), "r"(p));
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_l) : "r"(sum_at + (uint32_t)r * 8), "r"(p));
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_o) : "r"(so_at + (uint32_t)(r * C::PITCH + c) * 4), "r"(p));
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(pm) : "r"(at_m) : "memory");
-      asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(l0), "=f"(l1) : "r"(at_l) : "memory");
-      asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(at_o) : "memory");
-      const float next = fmaxf(m, pm), base = next == -INFINITY ? 0.f : next;
-      const float fa = ex2(m - base), fb = ex2(pm - base);
-      l = l * fa + (l0 + l1) * fb;
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[e] = o[e] * fa + x[e] * fb;
-      m = next;
+      for (int st = 0; st < C::NS; st++) {
+        uint32_t at_m, at_o;
+        float pm, pl, x[4];
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_m) : "r"(state_at + (uint32_t)(st * W_ROWS + r) * 8), "r"(p));
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at_o) : "r"(so_at + (uint32_t)((st * W_ROWS + r) * C::PITCH + c) * 4), "r"(p));
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(pm), "=f"(pl) : "r"(at_m) : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(at_o) : "memory");
+        const float next = fmaxf(m, pm), base = next == -INFINITY ? 0.f : next;
+        const float fa = ex2(m - base), fb = ex2(pm - base);
+        l = l * fa + pl * fb;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = o[e] * fa + x[e] * fb;
+        m = next;
+      }
     }
     const int t2 = (row0 + r) / a.group, g2 = row0 + r - t2 * a.group;
     TQ* to = static_cast<TQ*>(a.out) + ((b * a.rows + t2) * a.heads + (int64_t)kvh * a.group + g2) * a.d + c;
@@ -539,7 +557,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) tree_attention_wide_kernel(const
   if (a.splits > 1)
     asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");  // others read this block's states
   tc_fence_after();
-  if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  if (warp == ISSUING) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   if (tid == 0 && s_abort) report_wait_expired(error, DEV_ERR_GEMM_PIPE);
 }
 
@@ -557,7 +575,7 @@ int run_wide(TreeArgs a, cudaStream_t s) {
     DYN_CUDA(cudaFuncGetAttributes(&attr, kernel));
     launch_regs = attr.numRegs;
   }
-  DYN_CHECK(launch_regs * W_THREADS >= W_SOFTMAX * W_MANY + (W_THREADS - W_SOFTMAX) * W_FEW, "tree_attention: built with %d registers a thread", launch_regs.load());
+  DYN_CHECK(launch_regs >= C::START, "tree_attention: built with %d registers a thread", launch_regs.load());
   const int64_t pairs = a.batch * a.kv_heads;
   a.row_blocks = (int)(((int64_t)a.rows * a.group + W_ROWS - 1) / W_ROWS);
   // blocks of a cluster: as many as fit the SMs at once (a block takes an SM), at least two tiles each at full capacity
@@ -566,7 +584,7 @@ int run_wide(TreeArgs a, cudaStream_t s) {
   a.splits = splits;
   DYN_CHECK(pairs * splits <= 0x7fffffff && a.row_blocks <= 65535, "tree_attention: too many sequences or rows for one call");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(pairs * splits), (unsigned)a.row_blocks), cfg.blockDim = dim3(W_THREADS);
+  cfg.gridDim = dim3((unsigned)(pairs * splits), (unsigned)a.row_blocks), cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM, cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
