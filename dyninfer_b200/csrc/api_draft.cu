@@ -36,7 +36,7 @@ int kv_rows(const char* what, const void* k, const void* v, int type, const int6
             bool write, void* stream) {
   DYN_CHECK(plain_type(type), "%s: type %d unsupported (f32, f16 or bf16)", what, type);
   DYN_CHECK(kv_type == DYNINFER_KV_Q8 || kv_type == DYNINFER_KV_E4M3, "%s: cache type %d is not an 8-bit one", what, kv_type);
-  DYN_CHECK(sane(batch) && sane(rows) && heads > 0 && heads <= 65536 && cap > 0 && sane(cap) && batch * rows <= (1ll << 40), "%s: bad shape", what);
+  DYN_CHECK(sane(batch) && sane(rows) && heads > 0 && heads <= 65536 && cap > 0 && sane(cap) && rows * heads <= (1ll << 30), "%s: bad shape", what);
   DYN_CHECK(d > 0 && d % 16 == 0 && d <= 256, "%s: head dim %lld unsupported (a multiple of 16 up to 256)", what, (long long)d);
   if (batch == 0 || rows == 0) return 0;
   DYN_CHECK(k && v && k_cache && v_cache && k_scale && v_scale && starts && x_strides && cache_strides && scale_strides,

@@ -9,15 +9,18 @@
 // A row whose top is below 2^-100 becomes zeros with scale 0 (1 / top would leave f32's range). A row with an infinity or NaN
 // gets a NaN scale over zero codes: it reads back as NaN, and no product ever meets a code that is not finite.
 //
-// Memory bounds both directions. A thread holds eight entries of a key row and of the value row beside it, a row's threads
-// (d / 8 rounded up to a power of two) share its maximum by shuffles, and everything is touched once.
+// Memory bounds both directions. A thread holds eight entries of a key row and of the value row beside it, of two such pairs; a
+// row's threads (d / 8 rounded up to a power of two) share its maximum by shuffles, and everything is touched once. What is read is asked for
+// before anything is computed.
+#include <algorithm>
+
 #include "kv_codes.cuh"
 
 namespace dyn {
 
 namespace {
 
-constexpr int KV_THREADS = 256;
+constexpr int KV_THREADS = 128;
 
 struct KvRowArgs {
   const void* x[2];       // write: keys, values [batch][row][head][d]; unused when reading
@@ -29,7 +32,7 @@ struct KvRowArgs {
   int64_t ss[2][2];       // floats between slots, heads
   const int64_t* starts;  // [batch]
   const int64_t* counts;  // [batch] or NULL
-  int64_t rows, cap, total;  // total = batch * rows * heads
+  int64_t batch, rows, cap;
   int heads, units;          // units of eight entries per row
 };
 
@@ -48,44 +51,52 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
   }
 }
 
-// Where row `index` (batch entry, row, head; the head runs fastest) stands; false: nothing to do for it.
-__device__ __forceinline__ bool locate(const KvRowArgs& a, int64_t index, int64_t* batch, int64_t* row, int* head, int64_t* at) {
-  if (index >= a.total) return false;
-  const int64_t per = a.rows * a.heads;
-  *batch = index / per;
-  const int64_t rest = index - *batch * per;
-  *row = rest / a.heads, *head = (int)(rest - *row * a.heads);
+// Whether a row of a batch entry has a place in the cache.
+__device__ __forceinline__ bool in_cache(const KvRowArgs& a, int64_t batch, int row, int64_t start) {
   // a start far outside must not wrap around into the cache
-  const int64_t start = a.starts[*batch];
-  *at = start + *row;
-  return start > -a.cap - a.rows && start < a.cap && *at >= 0 && *at < a.cap && (!a.counts || *row < a.counts[*batch]);
+  return start > -a.cap - a.rows && start < a.cap && start + row >= 0 && start + row < a.cap && (!a.counts || row < a.counts[batch]);
 }
+
+constexpr int KV_PAIRS = 1;  // (row, head) pairs of a thread
 
 template <typename T, bool E4M3, bool WIDE, int P>
 __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const __grid_constant__ KvRowArgs a) {
   const int lane = threadIdx.x & (P - 1);
-  const int64_t index = (int64_t)blockIdx.x * (KV_THREADS / P) + threadIdx.x / P;
-  int64_t batch = 0, row = 0, at = 0;
-  int head = 0;
-  const bool live = locate(a, index, &batch, &row, &head, &at), mine = live && lane < a.units;
-  float v[2][8] = {};
+  const unsigned pairs = (unsigned)(a.rows * a.heads), first = blockIdx.x * (KV_THREADS / P * KV_PAIRS) + threadIdx.x / P;
+  for (int64_t batch = blockIdx.y; batch < a.batch; batch += gridDim.y) {
+    const int64_t start = a.starts[batch];
+    float v[KV_PAIRS][2][8] = {};
+    int row[KV_PAIRS], head[KV_PAIRS];
+    bool mine[KV_PAIRS];
 #pragma unroll
-  for (int w = 0; w < 2; w++)
-    if (mine)
-      load8<T, WIDE>(static_cast<const T*>(a.x[w]) + batch * a.xs[w][0] + row * a.xs[w][1] + head * a.xs[w][2] + lane * 8, v[w]);
+    for (int i = 0; i < KV_PAIRS; i++) {
+      const unsigned at = first + i * (KV_THREADS / P);
+      row[i] = (int)(at / (unsigned)a.heads), head[i] = (int)(at - (unsigned)row[i] * (unsigned)a.heads);
+      mine[i] = at < pairs && lane < a.units;
 #pragma unroll
-  for (int w = 0; w < 2; w++) {
-    uint32_t top = 0;  // magnitudes compare as integers; infinities and NaN come out on top
+      for (int w = 0; w < 2; w++)
+        if (mine[i])
+          load8<T, WIDE>(static_cast<const T*>(a.x[w]) + batch * a.xs[w][0] + row[i] * a.xs[w][1] + head[i] * a.xs[w][2] + lane * 8, v[i][w]);
+    }
 #pragma unroll
-    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[w][i]) & 0x7fffffffu);
+    for (int i = 0; i < KV_PAIRS; i++) {
+      mine[i] = mine[i] && in_cache(a, batch, row[i], start);
 #pragma unroll
-    for (int o = P / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float scale, inv;
-    kv_scale<E4M3>(top, &scale, &inv);
-    if (mine) {
-      *reinterpret_cast<uint2*>(a.codes[w] + batch * a.cs[w][0] + head * a.cs[w][1] + at * a.cs[w][2] + lane * 8) =
-          kv_encode8<E4M3>(v[w], inv);
-      if (lane == 0) a.scales[w][batch * a.ss[w][0] + head * a.ss[w][1] + at] = scale;
+      for (int w = 0; w < 2; w++) {
+        uint32_t top = 0;  // magnitudes compare as integers; infinities and NaN come out on top
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[i][w][e]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = P / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        float scale, inv;
+        kv_scale<E4M3>(top, &scale, &inv);
+        if (mine[i]) {
+          const int64_t at = start + row[i];
+          *reinterpret_cast<uint2*>(a.codes[w] + batch * a.cs[w][0] + head[i] * a.cs[w][1] + at * a.cs[w][2] + lane * 8) =
+              kv_encode8<E4M3>(v[i][w], inv);
+          if (lane == 0) a.scales[w][batch * a.ss[w][0] + head[i] * a.ss[w][1] + at] = scale;
+        }
+      }
     }
   }
 }
@@ -93,46 +104,59 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const __grid_const
 template <typename T, bool E4M3, bool WIDE, int P>
 __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_constant__ KvRowArgs a) {
   const int lane = threadIdx.x & (P - 1);
-  const int64_t index = (int64_t)blockIdx.x * (KV_THREADS / P) + threadIdx.x / P;
-  int64_t batch = 0, row = 0, at = 0;
-  int head = 0;
-  const bool live = locate(a, index, &batch, &row, &head, &at);
-  if (index >= a.total || lane >= a.units) return;
-  uint2 raw[2] = {};
-  float scale[2] = {};
+  const unsigned pairs = (unsigned)(a.rows * a.heads), first = blockIdx.x * (KV_THREADS / P * KV_PAIRS) + threadIdx.x / P;
+  if (lane >= a.units) return;
+  for (int64_t batch = blockIdx.y; batch < a.batch; batch += gridDim.y) {
+    const int64_t start = a.starts[batch];
+    uint2 raw[KV_PAIRS][2] = {};
+    float scale[KV_PAIRS][2] = {};
+    int row[KV_PAIRS], head[KV_PAIRS];
+    bool live[KV_PAIRS];
 #pragma unroll
-  for (int w = 0; w < 2; w++)
-    if (live) {
-      raw[w] = *reinterpret_cast<const uint2*>(a.codes[w] + batch * a.cs[w][0] + head * a.cs[w][1] + at * a.cs[w][2] + lane * 8);
-      scale[w] = a.scales[w][batch * a.ss[w][0] + head * a.ss[w][1] + at];
+    for (int i = 0; i < KV_PAIRS; i++) {
+      const unsigned at = first + i * (KV_THREADS / P);
+      row[i] = (int)(at / (unsigned)a.heads), head[i] = (int)(at - (unsigned)row[i] * (unsigned)a.heads);
+      live[i] = at < pairs && in_cache(a, batch, row[i], start);
+#pragma unroll
+      for (int w = 0; w < 2; w++)
+        if (live[i]) {
+          const int64_t where = start + row[i];
+          raw[i][w] = *reinterpret_cast<const uint2*>(a.codes[w] + batch * a.cs[w][0] + head[i] * a.cs[w][1] + where * a.cs[w][2] + lane * 8);
+          scale[i][w] = a.scales[w][batch * a.ss[w][0] + head[i] * a.ss[w][1] + where];
+        }
     }
 #pragma unroll
-  for (int w = 0; w < 2; w++) {
-    float v[8];
-    kv_decode8<E4M3>(raw[w], scale[w], v);
-    T* to = static_cast<T*>(a.y[w]) + batch * a.xs[w][0] + row * a.xs[w][1] + head * a.xs[w][2] + lane * 8;
-    uint4 packed[sizeof(T) / 2];
-    T* e = reinterpret_cast<T*>(packed);
+    for (int i = 0; i < KV_PAIRS; i++) {
+      if (first + i * (KV_THREADS / P) >= pairs) continue;
 #pragma unroll
-    for (int i = 0; i < 8; i++) kv_store(live ? v[i] : 0.f, e + i);
-    if (WIDE) {
+      for (int w = 0; w < 2; w++) {
+        float v[8];
+        kv_decode8<E4M3>(raw[i][w], scale[i][w], v);
+        T* to = static_cast<T*>(a.y[w]) + batch * a.xs[w][0] + row[i] * a.xs[w][1] + head[i] * a.xs[w][2] + lane * 8;
+        uint4 packed[sizeof(T) / 2];
+        T* e = reinterpret_cast<T*>(packed);
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; i++) reinterpret_cast<uint4*>(to)[i] = packed[i];
-    } else {
+        for (int j = 0; j < 8; j++) kv_store(live[i] ? v[j] : 0.f, e + j);
+        if (WIDE) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) to[i] = e[i];
+          for (int j = 0; j < (int)sizeof(T) / 2; j++) reinterpret_cast<uint4*>(to)[j] = packed[j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; j++) to[j] = e[j];
+        }
+      }
     }
   }
 }
 
 template <typename T, bool E4M3, bool WIDE, int P>
 int kv_run(const KvRowArgs& a, bool write, cudaStream_t s) {
-  const int64_t blocks = (a.total + KV_THREADS / P - 1) / (KV_THREADS / P);
-  DYN_CHECK(blocks <= 0x7fffffff, "8-bit cache: %lld rows are too many for one call", (long long)a.total);
+  const int64_t blocks = (a.rows * a.heads + KV_THREADS / P * KV_PAIRS - 1) / (KV_THREADS / P * KV_PAIRS);
+  const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(a.batch, 65535));
   if (write)
-    kv_write_kernel<T, E4M3, WIDE, P><<<(unsigned)blocks, KV_THREADS, 0, s>>>(a);
+    kv_write_kernel<T, E4M3, WIDE, P><<<grid, KV_THREADS, 0, s>>>(a);
   else
-    kv_read_kernel<T, E4M3, WIDE, P><<<(unsigned)blocks, KV_THREADS, 0, s>>>(a);
+    kv_read_kernel<T, E4M3, WIDE, P><<<grid, KV_THREADS, 0, s>>>(a);
   count_launch();
   DYN_CUDA(cudaGetLastError());
   return 0;
@@ -162,9 +186,9 @@ int kv_type(const KvRowArgs& a, bool e4m3, bool write, cudaStream_t s) {
 
 int launch_kv_rows(const KvRows& r, bool write, cudaStream_t s) {
   KvRowArgs a{};
-  a.rows = r.rows, a.cap = r.cap, a.total = r.batch * r.rows * r.heads, a.heads = (int)r.heads, a.units = (int)(r.d / 8);
+  a.batch = r.batch, a.rows = r.rows, a.cap = r.cap, a.heads = (int)r.heads, a.units = (int)(r.d / 8);
   a.starts = r.starts, a.counts = r.counts;
-  if (a.total == 0) return 0;
+  if (a.batch * a.rows * a.heads == 0) return 0;
   for (int w = 0; w < 2; w++) {
     a.x[w] = r.x[w], a.y[w] = r.x[w];
     a.codes[w] = static_cast<uint8_t*>(r.codes[w]), a.scales[w] = r.scales[w];

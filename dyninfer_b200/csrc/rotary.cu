@@ -47,7 +47,7 @@ __device__ __forceinline__ void from_f(float x, float* y) { *y = x; }
 __device__ __forceinline__ void from_f(float x, __half* y) { *y = __float2half_rn(x); }
 __device__ __forceinline__ void from_f(float x, __nv_bfloat16* y) { *y = __float2bfloat16_rn(x); }
 
-constexpr int ROTARY_THREADS = 256;
+constexpr int ROTARY_THREADS = 128;
 
 // Spelled out, so that every form of the kernel rounds alike.
 __device__ __forceinline__ float2 turn(float a, float b, float2 cs) {

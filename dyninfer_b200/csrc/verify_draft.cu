@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_draft_kernel(const __gri
   int* path = parent + a.nodes;
   __shared__ double own[2][VD_WARPS], all[16 * VD_WARPS], part[VD_WARPS];
   __shared__ long long s_found, s_last;
-  __shared__ int s_node, s_m, s_i, s_count, s_owner;  // where the walk stands; whose run holds the drawn token
-  __shared__ double s_total, s_z, s_before;
+  __shared__ int s_node, s_m, s_i, s_count;  // where the walk stands
+  __shared__ double s_z;
 
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, n = a.nodes;
   const int rank = (int)blockIdx.x % a.blocks;
@@ -105,8 +105,11 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_draft_kernel(const __gri
 
   const int64_t lo = min(a.vocab, ((int64_t)rank * VD_WARPS + warp) * a.run), hi = min(a.vocab, lo + a.run);
   const int runs = a.blocks * VD_WARPS;
+  const int per_lane = (runs + 31) / 32, from_run = min(runs, lane * per_lane), to_run = min(runs, from_run + per_lane);
+  auto place = [&](int i) { return i % per_lane * 32 + i / per_lane; };  // in all[]: a lane's neighbours beside it
   int round = 0;
-  constexpr int N = 16 / sizeof(T), LOADS = 16 / N;
+  double mine = 0., upto = 0., total = 0.;  // of this lane's runs, of those up to them, of all
+  constexpr int N = 16 / sizeof(T), LOADS = DRAFT ? 16 / N : 4;
   struct alignas(16) Piece {
     T v[N];
   };
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_draft_kernel(const __gri
       }
     }
   };
-  // all[] = every warp's sum of what is left at `node` after m refusals, s_total = their sum: the same in all blocks
+  // all[] = every warp's sum of what is left at `node` after m refusals, total = their sum: the same in all warps of all blocks
   auto sum_up = [&](int node, int m) {
     const T* p = target + (int64_t)node * a.ts[1];
     const T* q = DRAFT ? draft + (int64_t)node * a.ds[1] : nullptr;
@@ -177,19 +180,20 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_draft_kernel(const __gri
     // buffers alternate: one is written again behind a barrier that all its readers have passed
     if (lane == 0) own[round & 1][warp] = sum;
     cluster_sync();
-    if (tid < runs) all[tid] = peer_f64(&own[round & 1][tid % VD_WARPS], tid / VD_WARPS);
+    if (tid < runs) all[place(tid)] = peer_f64(&own[round & 1][tid % VD_WARPS], tid / VD_WARPS);
     round++;
     __syncthreads();
-    if (warp == 0) {
-      double t = 0.;
-      for (int i = lane; i < runs; i += 32) t += all[i];
+    // every warp adds them up for itself, a lane consecutive ones
+    mine = 0.;
+    for (int i = from_run; i < to_run; i++) mine += all[place(i)];
+    upto = mine;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-      if (lane == 0) {
-        s_total = t;
-        if (m) inv[m] = t > 0. ? 1. / t : 0., s_z = t;
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const double below = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += below;
     }
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    if (m && tid == 0) inv[m] = total > 0. ? 1. / total : 0., s_z = total;
     __syncthreads();
   };
   for (int have_node = -1, have_m = -1;;) {
@@ -229,48 +233,38 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_draft_kernel(const __gri
   }
   const int node = s_node;
   int m = s_m;
-  if (m && s_total == 0.) {
-    __syncthreads();
-    sum_up(node, m = 0);
-  }
-  const double border = (double)uniform[0] * s_total;
-  if (warp == 0) {
-    // the first run that reaches beyond the border, else the last one with anything in it
-    const int per = (runs + 31) / 32, from = min(runs, lane * per), to = min(runs, from + per);
-    double sum = 0.;
-    for (int i = from; i < to; i++) sum += all[i];
-    double upto = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double below = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += below;
-    }
-    double before = upto - sum, before_last = 0., before_found = 0.;
+  if (m && total == 0.) sum_up(node, m = 0);
+  const double border = (double)uniform[0] * total;
+  // the first run that reaches beyond the border, else the last one with anything in it
+  int owner;
+  double before_owner;
+  {
+    double before = upto - mine, before_last = 0., before_found = 0.;
     int last = -1, found = runs;
-    for (int i = from; i < to; i++) {
-      if (all[i] > 0.) {
+    for (int i = from_run; i < to_run; i++) {
+      const double r = all[place(i)];
+      if (r > 0.) {
         last = i, before_last = before;
-        if (found == runs && before + all[i] > border) found = i, before_found = before;
+        if (found == runs && before + r > border) found = i, before_found = before;
       }
-      before += all[i];
+      before += r;
     }
     const int first = __reduce_min_sync(0xffffffffu, found), final = __reduce_max_sync(0xffffffffu, last);
-    if (lane == 0) s_owner = first < runs ? first : final;
-    if (first < runs ? found == first : final >= 0 && last == final) s_before = first < runs ? before_found : before_last;
+    owner = first < runs ? first : final;
+    before_owner = __shfl_sync(0xffffffffu, first < runs ? before_found : before_last, max(0, owner) / per_lane);
   }
-  __syncthreads();
   if (rank == 0) {
     for (int i = tid; i < n; i += VD_THREADS) a.path[b * n + i] = i <= s_count ? path[i] : -1;
     if (tid == 0) a.accepted[b] = s_count;
   }
-  const bool fine = s_total > 0. && s_total < __longlong_as_double(0x7ff0000000000000ll);
-  if (!fine || s_owner < 0) {
+  const bool fine = total > 0. && total < __longlong_as_double(0x7ff0000000000000ll);
+  if (!fine || owner < 0) {
     if (rank == 0 && tid == 0) a.next[b] = -1;
-  } else if (s_owner / VD_WARPS == rank) {
+  } else if (owner / VD_WARPS == rank) {
     // the run's entries once more, over all warps of its block; a lane takes consecutive ones
     const T* p = target + (int64_t)node * a.ts[1];
     const T* q = DRAFT ? draft + (int64_t)node * a.ds[1] : nullptr;
-    const int64_t begin = min(a.vocab, (int64_t)s_owner * a.run), end = min(a.vocab, begin + a.run);
+    const int64_t begin = min(a.vocab, (int64_t)owner * a.run), end = min(a.vocab, begin + a.run);
     const int64_t per = (end - begin + VD_THREADS - 1) / VD_THREADS, from = min(end, begin + tid * per), to = min(end, from + per);
     auto entries = [&](int64_t v, double* r) {  // of v .. v + N - 1, zero from `to` on
       T pv[N] = {}, qv[N] = {};
@@ -287,28 +281,26 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_draft_kernel(const __gri
       }
       all_left(pv, qv, DRAFT ? m : 0, r);
     };
-    double sum = 0.;
+    double sum = 0., r[N];
     for (int64_t v = from; v < to; v += N) {
-      double r[N];
       entries(v, r);
 #pragma unroll
       for (int e = 0; e < N; e++) sum += r[e];
     }
-    double upto = sum;
+    double below_me = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const double below = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += below;
+      const double below = __shfl_up_sync(0xffffffffu, below_me, o);
+      if (lane >= o) below_me += below;
     }
-    if (lane == 31) part[warp] = upto;
+    if (lane == 31) part[warp] = below_me;
     if (tid == 0) s_found = a.vocab, s_last = -1;
     __syncthreads();
-    double run = s_before + (upto - sum);
+    double run = before_owner + (below_me - sum);
     for (int w = 0; w < warp; w++) run += part[w];
     long long found = a.vocab, last = -1;
     for (int64_t v = from; v < to; v += N) {
-      double r[N];
-      entries(v, r);
+      if (per > N) entries(v, r);  // else they are at hand
 #pragma unroll
       for (int e = 0; e < N; e++) {
         run += r[e];
