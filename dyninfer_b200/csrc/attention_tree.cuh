@@ -866,10 +866,10 @@ int run(TreeArgs a, cudaStream_t s) {
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), C::SMEM)) return 1;
   const int64_t pairs = a.batch * a.kv_heads;
   a.row_blocks = (int)(((int64_t)a.rows * a.group + C::RB - 1) / C::RB);
-  // blocks of a cluster: as many as there is room for at once, at least two tiles for each key group at full capacity
+  // blocks of a cluster: as many as there is room for at once, at least a tile for each key group at full capacity
   const int64_t room = (int64_t)std::max(1, sm_count()) * std::max(1, std::min(std::max(2, C::BLOCKS), (227 << 10) / (C::SMEM + 1024)));
   int splits = 16;
-  while (splits > 1 && (pairs * a.row_blocks * splits > room || a.cap < (int64_t)splits * WK * C::KT * 2)) splits--;
+  while (splits > 1 && (pairs * a.row_blocks * splits > room || a.cap < (int64_t)splits * WK * C::KT)) splits--;
   if (splits > 8) DYN_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   a.splits = splits;
   DYN_CHECK(pairs * splits <= 0x7fffffff && a.row_blocks <= 65535, "tree_attention: too many sequences or rows for one call");

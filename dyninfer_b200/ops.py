@@ -220,12 +220,11 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     `magnitude`; the other dimensions are copied. `layout` is "half" (pairs i, i + r/2) or "interleaved" (2i, 2i + 1).
     `frequencies` is a float64 tensor in host memory (`rotary_frequencies` makes one); angles are exact modulo a turn at any
     position. `out` may be x itself: a view of the leading heads of fused [q | k | v] rows turns q and k where they lie."""
-    kind = _WT.get(x.dtype)
+    kind, shape, sx = _WT.get(x.dtype), x.shape, x.stride()
     if kind is None:
         raise TypeError(f"x must be float32, float16 or bfloat16, not {x.dtype}")
     if layout != "half" and layout != "interleaved":
         raise ValueError(f"layout {layout!r} is neither 'half' nor 'interleaved'")
-    shape = x.shape
     if len(shape) == 3:
         (rows, heads, d), batch = shape, 1
     elif len(shape) == 4:
@@ -234,22 +233,26 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
         raise ValueError(f"x must be [rows, heads, d] or [batch, rows, heads, d], not {tuple(shape)}")
     if frequencies.is_cuda or frequencies.dtype is not torch.float64 or frequencies.dim() != 1:
         raise ValueError("frequencies must be a one-dimensional float64 tensor in host memory")
-    _dense_last("x", x)
-    _shape("positions", positions, shape[:-2])
+    if sx[-1] != 1:
+        _dense_last("x", x)
+    if positions.shape != shape[:-2]:
+        _shape("positions", positions, shape[:-2])
     positions = _index("positions", positions)
     if not frequencies.is_contiguous():
         frequencies = frequencies.contiguous()
     if out is None:
-        out = x.new_empty(shape)
-    elif out.dtype != x.dtype or out.shape != shape:
-        raise ValueError("out must have x's type and shape")
-    _dense_last("out", out)
-    sx, so = x.stride(), out.stride()
-    if batch == 1:      # a dimension of one entry is not stepped along, whatever its stride says
-        sx, so = (0, *sx[-3:]), (0, *so[-3:])
-    _run(_devices(x, positions, out), lib().dyninfer_cuda_rotary, x.data_ptr(), kind, _pack3(sx[0], sx[1], sx[2]),
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        so = out.stride()
+    else:
+        so = out.stride()
+        if out.dtype != x.dtype or out.shape != shape:
+            raise ValueError("out must have x's type and shape")
+        if so[-1] != 1:
+            _dense_last("out", out)
+    # (with one batch entry its stride is never used, whatever it says)
+    _run(_devices(x, positions, out), lib().dyninfer_cuda_rotary, x.data_ptr(), kind, _pack3(sx[-4] if batch > 1 else 0, sx[-3], sx[-2]),
          positions.data_ptr(), frequencies.data_ptr(), 2 * frequencies.numel(), layout == "interleaved", magnitude, batch, rows,
-         heads, d, out.data_ptr(), _pack3(so[0], so[1], so[2]))
+         heads, d, out.data_ptr(), _pack3(so[-4] if batch > 1 else 0, so[-3], so[-2]))
     return out
 
 
@@ -294,24 +297,28 @@ def rotary_frequencies(rotary_dim: int, theta: float = 1e6, scaling: str = "none
 
 
 def _cache(k_cache, v_cache):
-    if k_cache.dim() != 4:
-        raise ValueError(f"a cache is [slots, kv_heads, capacity, d], not {tuple(k_cache.shape)}")
-    _shape("v_cache", v_cache, k_cache.shape)
-    _dense_last("k_cache", k_cache)
-    _dense_last("v_cache", v_cache)
-    k, v = k_cache.stride(), v_cache.stride()
-    return _pack6(k[0], k[1], k[2], v[0], v[1], v[2])
+    """(shape, packed strides) of a cache."""
+    shape, k, v = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if len(shape) != 4:
+        raise ValueError(f"a cache is [slots, kv_heads, capacity, d], not {tuple(shape)}")
+    if v_cache.shape != shape:
+        _shape("v_cache", v_cache, shape)
+    if k[3] != 1 or v[3] != 1:
+        _dense_last("k_cache", k_cache)
+        _dense_last("v_cache", v_cache)
+    return shape, _pack6(k[0], k[1], k[2], v[0], v[1], v[2])
 
 
-def _scales(k_cache, k_scale, v_scale):
-    """Scales [slots, kv_heads, capacity] of an 8-bit cache's rows."""
-    shape = k_cache.shape[:3]
-    for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if scale is None or scale.dtype is not torch.float32:
-            raise TypeError(f"{name} must be float32")
-        _shape(name, scale, shape)
-        _dense_last(name, scale)
-    k, v = k_scale.stride(), v_scale.stride()
+def _scales(shape, k_scale, v_scale):
+    """Packed strides of the scales [slots, kv_heads, capacity] of an 8-bit cache's rows."""
+    if k_scale is None or v_scale is None or k_scale.dtype is not torch.float32 or v_scale.dtype is not torch.float32:
+        bad = "k_scale" if k_scale is None or k_scale.dtype is not torch.float32 else "v_scale"
+        raise TypeError(f"{bad} must be float32")
+    k, v, shape = k_scale.stride(), v_scale.stride(), shape[:3]
+    if k_scale.shape != shape or v_scale.shape != shape or k[2] != 1 or v[2] != 1:
+        for name, scale in (("k_scale", k_scale), ("v_scale", v_scale)):
+            _shape(name, scale, shape)
+            _dense_last(name, scale)
     return _pack4(k[0], k[1], v[0], v[1])
 
 
@@ -331,21 +338,24 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, k_cache: to
     if kind is None or v.dtype != k.dtype:
         raise TypeError(f"k and v must both be float32, float16 or bfloat16, not {k.dtype} and {v.dtype}")
     cache = _scaled_kind(k_cache, v_cache)
-    steps, scale_steps = _cache(k_cache, v_cache), _scales(k_cache, k_scale, v_scale)
-    slots, heads, cap, d = k_cache.shape
-    if k.dim() != 4:
-        raise ValueError(f"k must be [slots, rows, kv_heads, d], not {tuple(k.shape)}")
-    rows = k.shape[1]
-    _shape("k", k, (slots, rows, heads, d))
-    _shape("v", v, k.shape)
-    _dense_last("k", k)
-    _dense_last("v", v)
-    _shape("starts", starts, (slots,))
+    whole, steps = _cache(k_cache, v_cache)
+    scale_steps = _scales(whole, k_scale, v_scale)
+    slots, heads, cap, d = whole
+    shape, sk, sv = k.shape, k.stride(), v.stride()
+    if len(shape) != 4:
+        raise ValueError(f"k must be [slots, rows, kv_heads, d], not {tuple(shape)}")
+    rows = shape[1]
+    if shape != (slots, rows, heads, d) or v.shape != shape or sk[3] != 1 or sv[3] != 1:
+        _shape("k", k, (slots, rows, heads, d))
+        _shape("v", v, shape)
+        _dense_last("k", k)
+        _dense_last("v", v)
+    if starts.shape != whole[:1]:
+        _shape("starts", starts, (slots,))
     starts = _index("starts", starts)
     if counts is not None:
         _shape("counts", counts, (slots,))
         counts = _index("counts", counts)
-    sk, sv = k.stride(), v.stride()
     _run(_devices(k, v, starts, counts, k_cache, v_cache, k_scale, v_scale), lib().dyninfer_cuda_kv_write, k.data_ptr(), v.data_ptr(),
          kind, _pack6(sk[0], sk[1], sk[2], sv[0], sv[1], sv[2]), k_cache.data_ptr(), v_cache.data_ptr(), cache, steps,
          k_scale.data_ptr(), v_scale.data_ptr(), scale_steps, starts.data_ptr(), _p(counts), slots, rows, heads, d, cap)
@@ -361,15 +371,18 @@ def kv_read(starts: torch.Tensor, rows: int, k_cache: torch.Tensor, v_cache: tor
     if rows < 0:
         raise ValueError(f"rows must be at least zero, not {rows}")
     cache = _scaled_kind(k_cache, v_cache)
-    steps, scale_steps = _cache(k_cache, v_cache), _scales(k_cache, k_scale, v_scale)
-    slots, heads, cap, d = k_cache.shape
-    _shape("starts", starts, (slots,))
+    whole, steps = _cache(k_cache, v_cache)
+    scale_steps = _scales(whole, k_scale, v_scale)
+    slots, heads, cap, d = whole
+    if starts.shape != whole[:1]:
+        _shape("starts", starts, (slots,))
     starts = _index("starts", starts)
-    k, v = k_cache.new_empty((2, slots, rows, heads, d), dtype=dtype).unbind(0)
-    sk = rows * heads * d, heads * d, d
-    _run(_devices(k, starts, k_cache, v_cache, k_scale, v_scale), lib().dyninfer_cuda_kv_read, k.data_ptr(), v.data_ptr(), kind,
-         _pack6(*sk, *sk), k_cache.data_ptr(), v_cache.data_ptr(), cache, steps, k_scale.data_ptr(), v_scale.data_ptr(), scale_steps,
-         starts.data_ptr(), slots, rows, heads, d, cap)
+    k = k_scale.new_empty((slots, rows, heads, d), dtype=dtype)
+    v = torch.empty_like(k)
+    row, head = heads * d, d
+    _run(_devices(starts, k_cache, v_cache, k_scale, v_scale), lib().dyninfer_cuda_kv_read, k.data_ptr(), v.data_ptr(), kind,
+         _pack6(rows * row, row, head, rows * row, row, head), k_cache.data_ptr(), v_cache.data_ptr(), cache, steps,
+         k_scale.data_ptr(), v_scale.data_ptr(), scale_steps, starts.data_ptr(), slots, rows, heads, d, cap)
     return k, v
 
 
@@ -386,31 +399,35 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise TypeError(f"q must be float32, float16 or bfloat16, not {q.dtype}")
     if cache is None or v_cache.dtype != k_cache.dtype:
         raise TypeError(f"caches must both be float16, bfloat16, int8 or float8_e4m3fn, not {k_cache.dtype} and {v_cache.dtype}")
-    steps, scale_steps = _cache(k_cache, v_cache), None
+    (whole, steps), scale_steps = _cache(k_cache, v_cache), None
     if cache >= _lib.KV["q8"]:
-        scale_steps = _scales(k_cache, k_scale, v_scale)
+        scale_steps = _scales(whole, k_scale, v_scale)
     elif k_scale is not None or v_scale is not None:
         raise ValueError(f"a cache of {k_cache.dtype} has no scales")
-    slots, kv_heads, cap, d = k_cache.shape
-    if q.dim() != 4:
-        raise ValueError(f"q must be [slots, rows, heads, d], not {tuple(q.shape)}")
-    shape = q.shape
+    slots, kv_heads, cap, d = whole
+    shape, sq = q.shape, q.stride()
+    if len(shape) != 4:
+        raise ValueError(f"q must be [slots, rows, heads, d], not {tuple(shape)}")
     _, rows, heads, _ = shape
-    _shape("q", q, (slots, rows, heads, d))
-    _dense_last("q", q)
-    _shape("lengths", lengths, (slots,))
+    if shape[0] != slots or shape[3] != d or sq[3] != 1:
+        _shape("q", q, (slots, rows, heads, d))
+        _dense_last("q", q)
+    if lengths.shape != whole[:1]:
+        _shape("lengths", lengths, (slots,))
     lengths = _index("lengths", lengths)
     masked = None
     if mask is not None:
         if mask.dtype is not torch.bool:
             raise TypeError(f"mask must be bool, not {mask.dtype}")
         shared = mask.dim() == 2
-        _shape("mask", mask, (rows, rows) if shared else (slots, rows, rows))
-        if mask.stride(-1) != 1 and rows > 1:
+        if mask.shape != ((rows, rows) if shared else (slots, rows, rows)):
+            _shape("mask", mask, (rows, rows) if shared else (slots, rows, rows))
+        sm = mask.stride()
+        if sm[-1] != 1 and rows > 1:
             mask = mask.contiguous()
-        masked = _pack2(0 if shared else mask.stride(0), mask.stride(-2))
-    out = q.new_empty(shape)
-    sq = q.stride()
+            sm = mask.stride()
+        masked = _pack2(0 if shared else sm[0], sm[-2])
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     _run(_devices(q, k_cache, v_cache, lengths, mask, k_scale, v_scale), lib().dyninfer_cuda_tree_attention, q.data_ptr(), kind,
          _pack3(sq[0], sq[1], sq[2]), k_cache.data_ptr(), v_cache.data_ptr(), cache, steps, _p(k_scale), _p(v_scale), scale_steps,
          lengths.data_ptr(), _p(mask), masked, slots, rows, heads, kv_heads, d, cap, d ** -0.5 if scale is None else scale,
@@ -434,15 +451,17 @@ def verify_draft(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tens
     kind = _WT.get(target.dtype)
     if kind is None:
         raise TypeError(f"target must be float32, float16 or bfloat16, not {target.dtype}")
-    slots, nodes, vocab = target.shape
-    each = (slots, nodes)
-    _shape("tokens", tokens, each)
+    shape, st = target.shape, target.stride()
+    slots, nodes, vocab = shape
+    each = shape[:2]
     shared = parents.dim() == 1
-    _shape("parents", parents, (nodes,) if shared else each)
-    _shape("uniforms", uniforms, each)
+    if tokens.shape != each or parents.shape != (each[1:] if shared else each) or uniforms.shape != each or st[2] != 1:
+        _shape("tokens", tokens, each)
+        _shape("parents", parents, each[1:] if shared else each)
+        _shape("uniforms", uniforms, each)
+        _dense_last("target", target)
     if uniforms.dtype is not torch.float32:
         raise TypeError(f"uniforms must be float32, not {uniforms.dtype}")
-    _dense_last("target", target)
     tokens, parents = _index("tokens", tokens), _index("parents", parents)
     if not uniforms.is_contiguous():
         uniforms = uniforms.contiguous()
@@ -450,13 +469,15 @@ def verify_draft(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tens
     if draft is not None:
         if draft.dtype != target.dtype:
             raise TypeError(f"draft must have the target's type {target.dtype}, not {draft.dtype}")
-        _shape("draft", draft, (slots, nodes, vocab))
-        _dense_last("draft", draft)
-        drafted = _pack2(draft.stride(0), draft.stride(1))
-    path = tokens.new_empty(each)
-    accepted, following = tokens.new_empty(slots), tokens.new_empty(slots)
+        sd = draft.stride()
+        if draft.shape != shape or sd[2] != 1:
+            _shape("draft", draft, shape)
+            _dense_last("draft", draft)
+        drafted = _pack2(sd[0], sd[1])
+    path, accepted = torch.empty_like(tokens), tokens.new_empty(slots)
+    following = torch.empty_like(accepted)
     _run(_devices(target, tokens, parents, uniforms, draft), lib().dyninfer_cuda_verify_draft, tokens.data_ptr(), parents.data_ptr(),
-         0 if shared else nodes, target.data_ptr(), _pack2(target.stride(0), target.stride(1)), _p(draft), drafted, kind,
+         0 if shared else nodes, target.data_ptr(), _pack2(st[0], st[1]), _p(draft), drafted, kind,
          uniforms.data_ptr(), slots, nodes, vocab, accepted.data_ptr(), path.data_ptr(), following.data_ptr())
     return accepted, path, following
 
