@@ -39,8 +39,13 @@ struct Wide {
   // 512 threads start with 128 registers each, 384 with 168
   static constexpr int START = NS == 2 ? 128 : 168, MANY = NS == 2 ? 200 : 232, FEW = NS == 2 ? 56 : 136;
   static_assert(SOFTMAX * MANY + (THREADS - SOFTMAX) * FEW <= THREADS * START, "the groups' shares come out of the launch's registers");
+  // bf16 results leave the output in tensor memory, where the products add it up: an accumulation is off by 2^-24 of the sum, toward zero,
+  // which 2^-9 does not see before some ten thousand tiles; rows whose reference moves are rescaled there. With f16 operands (one
+  // term of P) there is room for P beside S, and the next tile's S is made under the present one's exponentials.
+  static constexpr bool STAYS = QB, BESIDE = STAYS && PT == 1;
   // tensor memory columns
-  static constexpr int S_COLS = PT == 3 ? 96 : 64, STREAM = S_COLS + D_, Q_COL = NS * STREAM;  // a stream: S, then U
+  static constexpr int S_COLS = PT == 3 ? 96 : 64, P_COL = BESIDE ? 64 : 0, U_AT = BESIDE ? 96 : S_COLS;  // a stream: S, P, U
+  static constexpr int STREAM = U_AT + D_, Q_COL = NS * STREAM;
   static_assert(Q_COL + QT * (D_ / 2) <= 512, "tensor memory has 512 columns");
   // products' descriptors: kind::f16, f32 accumulator, M = 128, N at bit 17; bf16 operands; B contiguous along N
   static constexpr uint32_t ID = (1u << 4) | (8u << 24) | (BF ? (1u << 7) | (1u << 10) : 0u);
@@ -94,7 +99,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
   using C = Wide<CT, TQ, D>;
   using O = Op<C::BF>;
   extern __shared__ uint8_t wide_shared[];
-  __shared__ uint64_t kv_full[C::TILES], kv_free[C::TILES], q_full, s_full[C::NS], p_full[C::NS], u_full[C::NS];
+  __shared__ uint64_t kv_full[C::TILES], kv_free[C::TILES], q_full, s_full[C::NS], s_free[C::NS], p_full[C::NS], u_full[C::NS];
   __shared__ uint32_t tmem_base_s;
   __shared__ int s_abort;
   __shared__ __align__(16) float kscale[C::WIDE ? 1 : C::TILES][W_KEYS], vscale[C::WIDE ? 1 : C::TILES][W_KEYS];  // read by fours
@@ -125,8 +130,8 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
   if (tid == 0) {
     s_abort = 0;
     for (int i = 0; i < C::TILES; i++) mbar_init(kv_full + i, W_FILL), mbar_init(kv_free + i, 1);
-    for (int i = 0; i < C::NS; i++) mbar_init(s_full + i, 1), mbar_init(p_full + i, live_warps), mbar_init(u_full + i, 1);
-    mbar_init(&q_full, live_warps);
+    for (int i = 0; i < C::NS; i++) mbar_init(s_full + i, 1), mbar_init(s_free + i, live_warps), mbar_init(p_full + i, live_warps), mbar_init(u_full + i, 1);
+    mbar_init(&q_full, C::NS == 2 && live_rows <= 64 ? 2 * live_warps : live_warps);
     mbar_fence_init();
   }
   constexpr int ISSUING = (C::SOFTMAX + W_FILL) / 32;  // the first issuing warp
@@ -145,12 +150,14 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
   float* const so = reinterpret_cast<float*>(smem);  // the final states, in the tiles' place
   if (warp < C::SOFTMAX / 32) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::MANY));
-    const int stream = warp / 4, row = (warp & 3) * 32 + lane;
-    const bool working = (warp & 3) * 32 < live_rows && mine;
+    // up to 64 rows stand in the lanes a second time, for the second stream, so that its warps are on the other half of the SM
+    const bool twice = C::NS == 2 && live_rows <= 64;
+    const int stream = warp / 4, row = ((warp & 3) * 32 + lane) - (twice ? 64 * stream : 0);
+    const bool holds = (row & ~31) >= 0 && (row & ~31) < live_rows, working = holds && mine;
     const uint32_t tlane = (uint32_t)((warp & 3) * 32) << 16;
-    const int row_index = row0 + min(row, live_rows - 1), tr = row_index / a.group, gh = row_index - tr * a.group;
+    const int row_index = row0 + max(0, min(row, live_rows - 1)), tr = row_index / a.group, gh = row_index - tr * a.group;
     const TQ* const query = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
-    if (working && stream == 0) {
+    if (working && (stream == 0 || twice)) {
       // ---- Q into tensor memory ----
       float x[D];
       constexpr int N = 16 / sizeof(TQ);
@@ -205,7 +212,19 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
       wait(&q_full, 0, 9);
       mult = s_mult[row];
     }
-    const uint32_t s_at = tmem + tlane + (uint32_t)(stream * C::STREAM), u_at = s_at + C::S_COLS;
+    const uint32_t s_at = tmem + tlane + (uint32_t)(stream * C::STREAM), p_at = s_at + C::P_COL, u_at = s_at + C::U_AT;
+    auto add_up = [&] {  // U
+#pragma unroll
+      for (int c = 0; c < D / 16; c += 2) {
+        uint32_t u[2][16];
+        tmem_ld16(u_at + 16u * c, u[0]);
+        tmem_ld16(u_at + 16u * c + 16u, u[1]);
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
+          add2(out[16 * c + e], out[16 * c + e + 1], __uint_as_float(u[e >> 4][e & 15]), __uint_as_float(u[e >> 4][(e & 15) + 1]));
+      }
+    };
     int buf = stream;
     unsigned phase = 0, parity = 0;
 #pragma unroll 1
@@ -254,31 +273,9 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
         }
         __syncwarp();
       };
-      float best = -INFINITY;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        float x[32];
-        half(h, x);
-        float m0 = x[0], m1 = x[1];
-#pragma unroll
-        for (int e = 2; e < 32; e += 2) m0 = fmaxf(m0, x[e]), m1 = fmaxf(m1, x[e + 1]);
-        best = fmaxf(best, fmaxf(m0, m1));
-      }
-      best *= mult;  // which is above zero
-      if (best > top + C::SLACK || top == -INFINITY) {
-        const float f = ex2(top - (best == -INFINITY ? 0.f : best));
-        decay *= f, sum *= f, top = best;
-      }
-      if (__any_sync(0xffffffffu, decay != 1.f)) {
-#pragma unroll
-        for (int d = 0; d < D; d += 2) mul2(out[d], out[d + 1], decay, decay);
-      }
-      const float base = top == -INFINITY ? 0.f : top;
       float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        float x[32];
-        half(h, x);
+      // half of a tile's weights into their place as operands
+      auto weights = [&](int h, float* x, float base) {
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           float* const w = x + 16 * c;
@@ -311,32 +308,98 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
             uint32_t f[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) f[e] = O::take(w[2 * e], w[2 * e + 1]);
-            wide_st8(s_at + (n < 2 ? 32u * h + 16u * c + 8u * n : 64u + 16u * h + 8u * c), f);
+            wide_st8(C::BESIDE ? p_at + 16u * h + 8u * c : s_at + (n < 2 ? 32u * h + 16u * c + 8u * n : 64u + 16u * h + 8u * c), f);
           }
         }
-      }
-      sum += s0 + s1;
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + stream);
-      wait(u_full + stream, parity, 3);
-      __syncwarp();
-      tc_fence_after();
+      };
+      float best = -INFINITY;
+      auto reference = [&] {  // what the row's scores are taken relative to
+        best *= mult;         // which is above zero
+        if (best > top + C::SLACK || top == -INFINITY) {
+          const float f = ex2(top - (best == -INFINITY ? 0.f : best));
+          decay *= f, sum *= f, top = best;
+        }
+        return top == -INFINITY ? 0.f : top;
+      };
+      if constexpr (C::STAYS) {
+        float x[64];
+        half(0, reinterpret_cast<float(&)[32]>(x[0]));
+        half(1, reinterpret_cast<float(&)[32]>(x[32]));
+        if (C::BESIDE) {  // S may be overwritten
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free + stream);
+        }
+        float m[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-      for (int c = 0; c < D / 16; c += 2) {
-        uint32_t u[2][16];
-        tmem_ld16(u_at + 16u * c, u[0]);
-        tmem_ld16(u_at + 16u * c + 16u, u[1]);
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        for (int e = 4; e < 64; e++) m[e & 3] = fmaxf(m[e & 3], x[e]);
+        best = fmaxf(best, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+        const float base = reference();
+        const bool moved = __any_sync(0xffffffffu, decay != 1.f);
+        if (i > stream && (C::BESIDE || moved)) {  // the products before are done with P and U
+          wait(u_full + stream, parity ^ 1u, 3);
+          __syncwarp();
+          tc_fence_after();
+          if (moved) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t u[16];
+              tmem_ld16(u_at + c, u);
+              asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int e = 0; e < 32; e += 2)
-          add2(out[16 * c + e], out[16 * c + e + 1], __uint_as_float(u[e >> 4][e & 15]), __uint_as_float(u[e >> 4][(e & 15) + 1]));
+              for (int e = 0; e < 16; e++) u[e] = __float_as_uint(__uint_as_float(u[e]) * decay);
+              tmem_st16(u_at + c, u);
+            }
+          }
+        }
+        weights(0, x, base);
+        weights(1, x + 32, base);
+        sum += s0 + s1;
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + stream);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          float x[32];
+          half(h, x);
+          float m0 = x[0], m1 = x[1];
+#pragma unroll
+          for (int e = 2; e < 32; e += 2) m0 = fmaxf(m0, x[e]), m1 = fmaxf(m1, x[e + 1]);
+          best = fmaxf(best, fmaxf(m0, m1));
+        }
+        const float base = reference();
+        if (__any_sync(0xffffffffu, decay != 1.f)) {
+#pragma unroll
+          for (int d = 0; d < D; d += 2) mul2(out[d], out[d + 1], decay, decay);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          float x[32];
+          half(h, x);
+          weights(h, x, base);
+        }
+        sum += s0 + s1;
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + stream);
+        wait(u_full + stream, parity, 3);
+        __syncwarp();
+        tc_fence_after();
+        add_up();
+        tc_fence_before();
       }
-      tc_fence_before();
       parity ^= 1u;
       buf += C::NS;
       if (buf >= C::TILES) buf -= C::TILES, phase ^= 1u;
+    }
+    if (C::STAYS && working && stream < mine) {
+      wait(u_full + stream, parity ^ 1u, 3);
+      __syncwarp();
+      tc_fence_after();
+      add_up();
     }
     bool fine = true;
     const float unit = C::BF ? 1.f : C::WIDE ? 1.f / (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(vex - C::PEXP) << 23);
@@ -345,7 +408,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
       out[d] *= unit;
       fine = fine && fabsf(out[d]) < INFINITY;
     }
-    fine = fine || row >= live_rows;
+    fine = fine || row < 0 || row >= live_rows;
     __syncwarp();
     if (__syncthreads_or(!fine) && working) {
       // ---- one by one: this thread's row over this stream's keys ----
@@ -385,7 +448,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
     }
     __syncwarp();
     // (all tiles have been read: the streams' last U were awaited, and what is read above is the cache itself)
-    if ((warp & 3) * 32 < live_rows) {
+    if (holds) {
       float* const to = so + (stream * W_ROWS + row) * C::PITCH;
 #pragma unroll
       for (int d = 0; d < D; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(out[d], out[d + 1], out[d + 2], out[d + 3]);
@@ -431,9 +494,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
 #pragma unroll 1
     for (int i = 0; i < mine; i++) {
       if (C::WIDE) {
-        free_place(i + AHEAD);
-        copy(i + AHEAD);
-        cp_wait<AHEAD>();
+        cp_wait<AHEAD - 1>();
       } else {
         cp_wait<AHEAD - 1>();
         asm volatile("bar.sync 5, %0;" ::"n"(W_FILL) : "memory");  // everybody's copies are there, and the oldest raw tile is done with
@@ -462,6 +523,11 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
       }
       fence_async_smem();
       mbar_arrive(kv_full + i % C::TILES);
+      if (C::WIDE) {
+        // behind the arrival: the products of the tile that is waited for may come after this one's scores
+        free_place(i + AHEAD);
+        copy(i + AHEAD);
+      }
     }
     cp_wait<0>();
     __syncthreads_or(0);
@@ -471,14 +537,14 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
     // the reductions only bring what every lane has into uniform registers, where the products' operands come from
     const int stream = warp - ISSUING, n_tiles = (int)__reduce_max_sync(0xffffffffu, (unsigned)mine);
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem), at = __reduce_max_sync(0xffffffffu, smem_u32(smem));
-    const uint32_t s_col = tm + (uint32_t)(stream * C::STREAM), u_col = s_col + C::S_COLS;
+    const uint32_t s_col = tm + (uint32_t)(stream * C::STREAM), p_col = s_col + C::P_COL, u_col = s_col + C::U_AT;
     const uint64_t k_desc = umma_desc(at), v_desc = wide_desc_mn(at + C::TILE / 2);
-    int buf = stream;
-    unsigned phase = 0, parity = 0;
+    int buf = stream, k_buf = stream;  // of the values and of the keys that come next
+    unsigned k_phase = 0, parity = 0;
     auto scores = [&] {
-      wait(kv_full + buf, phase, 5);
+      wait(kv_full + k_buf, k_phase, 5);
       tc_fence_after();
-      const uint64_t k = k_desc + (uint64_t)(buf * (C::TILE >> 4));
+      const uint64_t k = k_desc + (uint64_t)(k_buf * (C::TILE >> 4));
       if (elect_one()) {
 #pragma unroll
         for (int n = C::QT - 1; n >= 0; n--)  // the small terms first
@@ -489,12 +555,18 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
         umma_commit(s_full + stream);
       }
       __syncwarp();
+      k_buf += C::NS;
+      if (k_buf >= C::TILES) k_buf -= C::TILES, k_phase ^= 1u;
     };
     if (stream < C::NS && stream < n_tiles) {
       wait(&q_full, 0, 6);
       scores();
 #pragma unroll 1
       for (int i = stream; i < n_tiles; i += C::NS) {
+        if (C::BESIDE && i + C::NS < n_tiles) {
+          wait(s_free + stream, parity, 8);
+          scores();
+        }
         wait(p_full + stream, parity, 7);  // (the U before has been read as well)
         tc_fence_after();
         const uint64_t v = v_desc + (uint64_t)(buf * (C::TILE >> 4));
@@ -503,15 +575,15 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
           for (int n = C::PT - 1; n >= 0; n--)
 #pragma unroll
             for (int s = 0; s < W_KEYS / 16; s++)
-              umma_f16_ts(u_col, s_col + (n < 2 ? 16u * s + 8u * n : 64u + 8u * s), v + (uint64_t)(s * (2048 >> 4)), C::ID_U,
-                          n == C::PT - 1 && s == 0 ? 0u : 1u);
+              umma_f16_ts(u_col, C::BESIDE ? p_col + 8u * s : s_col + (n < 2 ? 16u * s + 8u * n : 64u + 8u * s), v + (uint64_t)(s * (2048 >> 4)), C::ID_U,
+                          n == C::PT - 1 && s == 0 ? (C::STAYS && i > stream ? 1u : 0u) : 1u);
           umma_commit(u_full + stream);
           umma_commit(kv_free + buf);
         }
         __syncwarp();
         buf += C::NS;
-        if (buf >= C::TILES) buf -= C::TILES, phase ^= 1u;
-        if (i + C::NS < n_tiles) {
+        if (buf >= C::TILES) buf -= C::TILES;
+        if (!C::BESIDE && i + C::NS < n_tiles) {
           wait(u_full + stream, parity, 8);  // P has been read
           scores();
         }

@@ -167,8 +167,9 @@ int launch_rotary(const void* x, int type, int64_t batch, int64_t rows, int64_t 
   if (batch * rows * heads == 0) return 0;
   RotaryTable table{};
   for (int64_t i = 0; i < rot / 2; i++) {
-    long double turns = (long double)frequencies[i] / 6.283185307179586476925286766559L;
-    turns -= floorl(turns);
+    long double turns = (long double)frequencies[i] * 0.15915494309189533576888376337251436L;  // one over 2 pi
+    turns -= fabsl(turns) < 4e18L ? (long double)(int64_t)turns : floorl(turns);
+    if (turns < 0) turns += 1;
     table.turn[i] = turns < 1.0L ? (uint64_t)(turns * 18446744073709551616.0L) : 0;
   }
   RotaryArgs a{};
