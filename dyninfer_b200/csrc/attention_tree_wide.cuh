@@ -37,7 +37,7 @@ struct Wide {
   // whole warpgroups, because registers are dealt out per group: the softmax threads of the streams, fillers, issuing warps
   static constexpr int SOFTMAX = NS * W_ROWS, THREADS = SOFTMAX + W_FILL + 128;
   // 512 threads start with 128 registers each, 384 with 168
-  static constexpr int START = NS == 2 ? 128 : 168, MANY = NS == 2 ? 200 : 232, FEW = NS == 2 ? 56 : 136;
+  static constexpr int START = NS == 2 ? 128 : 168, MANY = NS == 2 ? (QB ? 168 : 200) : 232, FEW = NS == 2 ? (QB ? 88 : 56) : 136;
   static_assert(SOFTMAX * MANY + (THREADS - SOFTMAX) * FEW <= THREADS * START, "the groups' shares come out of the launch's registers");
   // bf16 results leave the output in tensor memory, where the products add it up: an accumulation is off by 2^-24 of the sum, toward zero,
   // which 2^-9 does not see before some ten thousand tiles; rows whose reference moves are rescaled there. With f16 operands (one
@@ -465,23 +465,40 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
     // 8-bit: eight lanes have four pieces of two keys, whose places in a tile are in different banks
     const int key_l = C::WIDE || D == 64 ? ft / PER : ft / 16 * 2 + (ft >> 2 & 1), piece = C::WIDE || D == 64 ? ft % PER : (ft & 3) + (ft >> 1 & 4);
     const bool my_dims = piece * 16 < a.d * (C::WIDE ? 2 : 1);
-    auto copy = [&](int i) {  // tile i of this block's: into its place, or into the raw ring
+    // this thread's pieces of a tile lie ROWS keys apart, in the cache and in shared memory
+    const uint32_t to0 = C::WIDE ? box_chunk(key_l, piece) : (uint32_t)(key_l * D + (D == 128 ? piece ^ (key_l & 1) << 2 : piece) * 16);
+    constexpr uint32_t TO_STEP = C::WIDE ? ROWS * 128 : ROWS * D, TO_VALUES = C::WIDE ? C::TILE / 2 : D * W_KEYS;
+    const uint32_t tiles_at = smem_u32(smem), raw_at = tiles_at + (uint32_t)(C::TILES * C::TILE);
+    const uint8_t *k_from = kb + ((int64_t)split * W_KEYS + key_l) * a.kst[2] + piece * 16, *v_from = vb + ((int64_t)split * W_KEYS + key_l) * a.vst[2] + piece * 16;
+    const int64_t k_tile = (int64_t)a.splits * W_KEYS * a.kst[2], v_tile = (int64_t)a.splits * W_KEYS * a.vst[2];
+    const int64_t k_step = ROWS * a.kst[2], v_step = ROWS * a.vst[2];
+    uint32_t copy_at = C::WIDE ? tiles_at : raw_at;  // of the next tile that is asked for
+    int copy_place = 0;
+    auto copy = [&](int i) {  // tile i of this block's, in order: into its place, or into the raw ring
       if (i < mine) {
         const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS;
-        const uint32_t at = smem_u32(smem) + (uint32_t)(C::WIDE ? i % C::TILES * C::TILE : C::TILES * C::TILE + i % C::RAWS * C::RAW);
+        if (key0 + W_KEYS <= keys) {
 #pragma unroll
-        for (int j = 0; j < COPIES; j++) {
-          const int key = key_l + j * ROWS;
-          const bool live = my_dims && key0 + key < keys;
-          const uint32_t to = C::WIDE ? box_chunk(key, piece) : (uint32_t)(key * D + (D == 128 ? piece ^ (key & 1) << 2 : piece) * 16);
-          cp16(at + to, live ? kb + (key0 + key) * a.kst[2] + piece * 16 : kb, live);
-          cp16(at + (C::WIDE ? C::TILE / 2 : D * W_KEYS) + to, live ? vb + (key0 + key) * a.vst[2] + piece * 16 : vb, live);
+          for (int j = 0; j < COPIES; j++) {
+            cp16(copy_at + to0 + j * TO_STEP, my_dims ? k_from + j * k_step : kb, my_dims);
+            cp16(copy_at + TO_VALUES + to0 + j * TO_STEP, my_dims ? v_from + j * v_step : vb, my_dims);
+          }
+        } else {
+#pragma unroll 1
+          for (int j = 0; j < COPIES; j++) {
+            const bool live = my_dims && key0 + key_l + j * ROWS < keys;
+            cp16(copy_at + to0 + j * TO_STEP, live ? k_from + j * k_step : kb, live);
+            cp16(copy_at + TO_VALUES + to0 + j * TO_STEP, live ? v_from + j * v_step : vb, live);
+          }
         }
         if (!C::WIDE) {
           const int64_t kk = key0 + (ft & (W_KEYS - 1));
           const float* const of = ft < W_KEYS ? ksb : vsb;
-          cp4(at + 2 * D * W_KEYS + ft * 4, kk < keys ? of + kk : of, kk < keys);
+          cp4(copy_at + 2 * D * W_KEYS + ft * 4, kk < keys ? of + kk : of, kk < keys);
         }
+        k_from += k_tile, v_from += v_tile;
+        copy_at += C::WIDE ? C::TILE : C::RAW;
+        if (++copy_place == (C::WIDE ? C::TILES : C::RAWS)) copy_place = 0, copy_at = C::WIDE ? tiles_at : raw_at;
       }
       cp_commit();
     };
@@ -501,18 +518,23 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
         copy(i + AHEAD);
         free_place(i);
         const int to = i % C::TILES;
+        const uint32_t raw = raw_at + (uint32_t)(i % C::RAWS * C::RAW);
+        // dimensions 16 piece .. of this thread's keys: two pieces of eight, the same places in every eighth row
         uint8_t* const tile = smem + to * C::TILE;
-        const uint32_t raw = smem_u32(smem) + (uint32_t)(C::TILES * C::TILE + i % C::RAWS * C::RAW);
+        const uint32_t at0 = box_chunk(key_l, 2 * piece), at1 = box_chunk(key_l, 2 * piece + 1);
 #pragma unroll
-        for (int j = 0; j < 2 * COPIES; j++) {
-          const int key = key_l + j % COPIES * ROWS, at = j / COPIES * D * W_KEYS + key * D + (D == 128 ? piece ^ (key & 1) << 2 : piece) * 16;
-          const uint4 w = lds16(raw + at);
-          uint4 f[2];
-          widen<C::E4M3>(w.x, &f[0].x, &f[0].y), widen<C::E4M3>(w.y, &f[0].z, &f[0].w);
-          widen<C::E4M3>(w.z, &f[1].x, &f[1].y), widen<C::E4M3>(w.w, &f[1].z, &f[1].w);
-          uint8_t* const half = tile + j / COPIES * (C::TILE / 2);
-          *reinterpret_cast<uint4*>(half + box_chunk(key, 2 * piece)) = f[0];
-          *reinterpret_cast<uint4*>(half + box_chunk(key, 2 * piece + 1)) = f[1];
+        for (int kv = 0; kv < 2; kv++) {
+          uint4 w[COPIES];
+#pragma unroll
+          for (int j = 0; j < COPIES; j++) w[j] = lds16(raw + kv * TO_VALUES + to0 + j * TO_STEP);
+#pragma unroll
+          for (int j = 0; j < COPIES; j++) {
+            uint4 f[2];
+            widen<C::E4M3>(w[j].x, &f[0].x, &f[0].y), widen<C::E4M3>(w[j].y, &f[0].z, &f[0].w);
+            widen<C::E4M3>(w[j].z, &f[1].x, &f[1].y), widen<C::E4M3>(w[j].w, &f[1].z, &f[1].w);
+            *reinterpret_cast<uint4*>(tile + kv * (C::TILE / 2) + at0 + j * ROWS * 128) = f[0];
+            *reinterpret_cast<uint4*>(tile + kv * (C::TILE / 2) + at1 + j * ROWS * 128) = f[1];
+          }
         }
         const float scale = lds4(raw + 2 * D * W_KEYS + ft * 4);
         if (ft < W_KEYS) kscale[C::WIDE ? 0 : to][ft] = scale;
