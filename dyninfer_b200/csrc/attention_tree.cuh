@@ -237,6 +237,34 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int64_t b, int row, int6
   return a.mask ? a.mask[b * a.ms[0] + row * a.ms[1] + j] != 0 : j <= row;
 }
 
+// Bit e: whether a row sees key key0 + e, of N <= 32. Sixteen bytes of the mask are asked for at once.
+template <int N>
+__device__ __forceinline__ uint32_t seen_of(const TreeArgs& a, int64_t b, int row, int64_t key0, int64_t keys, int64_t len) {
+  const int64_t j0 = key0 - len;
+  uint32_t bits = 0;
+  if (!a.mask) {
+#pragma unroll
+    for (int e = 0; e < N; e++)
+      if (key0 + e < keys && j0 + e <= row) bits |= 1u << e;
+    return bits;
+  }
+  const uint8_t* const of = a.mask + b * a.ms[0] + row * a.ms[1];
+#pragma unroll
+  for (int e0 = 0; e0 < N; e0 += 16) {
+    uint8_t m[16];
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      const int64_t j = j0 + e0 + e;
+      m[e] = j < 0 ? 1 : 0;
+      if (e0 + e < N && j >= 0 && j < a.rows) m[e] = of[j];
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+      if (e0 + e < N && key0 + e0 + e < keys && m[e]) bits |= 1u << (e0 + e);
+  }
+  return bits;
+}
+
 template <int CT, typename TQ, int D, int MT_, int WR, int WK>
 __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLOCKS) tree_attention_kernel(const __grid_constant__ TreeArgs a) {
   using C = Cfg<CT, TQ, D, MT_, WR, WK>;
@@ -547,7 +575,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
             const int r = row0 + (wr * MT + m) * 16 + g + 8 * h;
             const int tr = r < total_rows ? r / a.group : 0;
             uint32_t bits = 0;
-#pragma unroll 1
+#pragma unroll
             for (int i = 0; i < 2 * NK; i++) {
               const int64_t key = key0 + (i >> 1) * 8 + 2 * t + (i & 1);
               if (key < keys && sees(a, b, tr, key - len)) bits |= 1u << i;

@@ -230,15 +230,11 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
 #pragma unroll 1
     for (int i = stream; i < mine && working; i += C::NS) {
       const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS;
+      const bool tail = key0 + W_KEYS > len;  // a tile with keys that not every row sees
       uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
-      if (key0 + W_KEYS > len) {
-        vis[0] = vis[1] = 0;
-#pragma unroll 1
-        for (int e = 0; e < W_KEYS; e++)
-          if (key0 + e < keys && sees(a, b, tr, key0 + e - len)) {
-            if (e < 32) vis[0] |= 1u << e;
-            else vis[1] |= 1u << (e - 32);
-          }
+      if (tail) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) vis[h] = seen_of<32>(a, b, tr, key0 + 32 * h, keys, len);
       }
       if (!C::WIDE) wait(kv_full + buf, phase, 2);  // for the scales
       wait(s_full + stream, parity, 1);
@@ -266,14 +262,13 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
             mul2(x[e + 2], x[e + 3], k4.z, k4.w);
           }
         }
-        if (vis[h] != 0xffffffffu) {
+        if (tail) {
 #pragma unroll
           for (int e = 0; e < 32; e++)
             if (!(vis[h] >> e & 1)) x[e] = -INFINITY;
         }
-        __syncwarp();
       };
-      float s0 = 0.f, s1 = 0.f;
+      float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
       // half of a tile's weights into their place as operands
       auto weights = [&](int h, float* x, float base) {
 #pragma unroll
@@ -283,7 +278,8 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
           for (int e = 0; e < 16; e += 2) {
             fms2(w[e], w[e + 1], mult, base);
             w[e] = ex2(w[e]), w[e + 1] = ex2(w[e + 1]);
-            add2(s0, s1, w[e], w[e + 1]);
+            if (e & 2) add2(s2, s3, w[e], w[e + 1]);
+            else add2(s0, s1, w[e], w[e + 1]);
           }
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
@@ -297,12 +293,11 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
               mul2(w[e + 2], w[e + 3], v4.z, v4.w);
             }
           }
-          if (!C::WIDE && vis[h] != 0xffffffffu) {  // the scale of a key that is not seen may be anything
+          if (!C::WIDE && tail) {  // the scale of a key that is not seen may be anything
 #pragma unroll
             for (int e = 0; e < 16; e++)
               if (!(vis[h] >> (16 * c + e) & 1)) w[e] = 0.f;
           }
-          __syncwarp();
 #pragma unroll
           for (int n = 0; n < C::PT; n++) {
             uint32_t f[8];
@@ -354,7 +349,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
         }
         weights(0, x, base);
         weights(1, x + 32, base);
-        sum += s0 + s1;
+        sum += (s0 + s1) + (s2 + s3);
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         __syncwarp();
@@ -380,7 +375,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
           half(h, x);
           weights(h, x, base);
         }
-        sum += s0 + s1;
+        sum += (s0 + s1) + (s2 + s3);
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc_fence_before();
         __syncwarp();
