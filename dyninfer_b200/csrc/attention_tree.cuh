@@ -201,9 +201,9 @@ struct Cfg {
   static constexpr int NQ = HALF ? (QT + 1) / 2 : QT, NP = HALF ? (PT + 1) / 2 : PT;   // operands of Q and P
   static constexpr int RB = 8 * H * MT * WR;                             // rows of a block
   static constexpr int THREADS = 32 * WR * WK;
-  static constexpr int KT = (WIDE || HALF ? 16 : 32) * (WR >= 2 ? 2 : 1); // keys of a tile
-  static constexpr int STAGES = HALF && !WIDE ? 4 : 3;
-  static constexpr int BLOCKS = HALF ? (WIDE ? 2 : 3) : 1;               // of an SM, as far as registers go
+  static constexpr int KT = (WIDE ? 16 : 32) * (WR >= 2 ? 2 : 1); // keys of a tile
+  static constexpr int STAGES = 3;
+  static constexpr int BLOCKS = HALF ? 2 : 1;                            // of an SM, as far as registers go
   static constexpr int TILE = KT * D * ES;
   static constexpr int STAGE = 2 * TILE + (WIDE ? 0 : 2 * KT * 4);
   static constexpr int RING = STAGE * STAGES * WK;
@@ -895,7 +895,7 @@ int run(TreeArgs a, cudaStream_t s) {
   const int64_t pairs = a.batch * a.kv_heads;
   a.row_blocks = (int)(((int64_t)a.rows * a.group + C::RB - 1) / C::RB);
   // blocks of a cluster: as many as there is room for at once, at least a tile for each key group at full capacity
-  const int64_t room = (int64_t)std::max(1, sm_count()) * std::max(1, std::min(std::max(2, C::BLOCKS), (227 << 10) / (C::SMEM + 1024)));
+  const int64_t room = (int64_t)std::max(1, sm_count()) * std::max(1, std::min(2, (227 << 10) / (C::SMEM + 1024)));
   int splits = 16;
   while (splits > 1 && (pairs * a.row_blocks * splits > room || a.cap < (int64_t)splits * WK * C::KT)) splits--;
   if (splits > 8) DYN_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));

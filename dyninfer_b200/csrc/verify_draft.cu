@@ -24,7 +24,7 @@ namespace dyn {
 
 namespace {
 
-constexpr int VD_THREADS = 512, VD_WARPS = VD_THREADS / 32;
+constexpr int VD_THREADS = 256, VD_WARPS = VD_THREADS / 32;
 
 struct VdArgs {
   const int64_t *tokens, *parents;  // [batch][nodes]
@@ -71,7 +71,7 @@ __device__ __forceinline__ double left_of(double p, double q, int64_t v, int m, 
 }
 
 template <typename T, bool DRAFT>
-__global__ void __launch_bounds__(VD_THREADS, 2) verify_draft_kernel(const __grid_constant__ VdArgs a) {
+__global__ void __launch_bounds__(VD_THREADS, 4) verify_draft_kernel(const __grid_constant__ VdArgs a) {
   extern __shared__ double vd_shared[];
   double* p_of = vd_shared;                 // [nodes] target's entry of the node's token in its parent's row
   double* q_of = p_of + a.nodes;            // [nodes] the draft's
@@ -327,9 +327,9 @@ int vd_run(VdArgs a, int64_t batch, cudaStream_t s) {
   auto kernel = verify_draft_kernel<T, DRAFT>;
   const int smem = a.nodes * (5 * 8 + 3 * 4);
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return 1;
-  // blocks per sequence: up to two per SM, no run of fewer than 128 entries
+  // blocks per sequence: up to four per SM, no run of fewer than 128 entries
   int blocks = 16;
-  while (blocks > 1 && (batch * blocks > 2 * std::max(1, sm_count()) || a.vocab < (int64_t)blocks * VD_WARPS * 128)) blocks /= 2;
+  while (blocks > 1 && (batch * blocks > 4 * std::max(1, sm_count()) || a.vocab < (int64_t)blocks * VD_WARPS * 128)) blocks /= 2;
   if (blocks > 8) DYN_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   a.blocks = blocks;
   a.run = ((a.vocab + blocks * VD_WARPS - 1) / (blocks * VD_WARPS) + 31) / 32 * 32;
