@@ -5,7 +5,7 @@
 // f32 scale per (head, position).
 //
 // The T * G rows that share a kv head (G query heads) are one block of rows, so that a key or value is fetched once for all of
-// them. Work on a (sequence, kv head) is split over the keys: over the key groups of a block and over the blocks of a cluster,
+// them. Work on a (sequence, kv head) is split over the keys: over the warps of a block and over the blocks of a cluster,
 // each with a running (maximum, sum, output) of its own; the states meet in a fixed order, in shared memory.
 //   S = Q K^T  mma.sync. The order of the head's dimensions inside the product is free, so 8-bit keys are read 16 bytes per lane
 //              as they lie; the key's scale multiplies the score. q8 keys enter whole-number products (m16n8k32) unconverted,
@@ -41,7 +41,7 @@ struct TreeArgs {
   int64_t kss[2], vss[2];   // floats between batch entries, heads
   int64_t ms[2];            // bytes between batch entries, rows
   int64_t batch, cap;
-  int rows, heads, kv_heads, group, d, splits, row_blocks;
+  int rows, heads, kv_heads, group, d, splits;
   float scale;
 };
 
@@ -77,14 +77,6 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
 // Operand type of the products: f16, or bf16 for bf16 caches.
 template <bool BF>
 struct Op {
-  __device__ static __forceinline__ uint32_t pack(float x, float y) {
-    if (BF) {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-      return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
   // x and y keep what the packed pair left of them
   __device__ static __forceinline__ uint32_t take(float& x, float& y) {
     if (BF) {
@@ -184,24 +176,24 @@ __device__ __forceinline__ void add2(float& x, float& y, float u, float v) {
       : "f"(u), "f"(v));
 }
 
-// CT: cache; TQ: type of q and out; D: head dimensions, d filled up with zeros; MT: 16-row tiles per warp; WR: warps along the
-// rows; WK: key groups. MT = 0: up to eight rows, an operand's leading terms in rows 0 .. 7 of a tile and its second ones in rows
-// 8 .. 15, so that one mma takes both and a thread has scores and outputs of one row instead of two.
-template <int CT, typename TQ, int D_, int MT_, int WR_, int WK_>
+// CT: cache; TQ: type of q and out; D: head dimensions, d filled up with zeros. HALF: up to eight rows, an operand's leading terms in
+// rows 0 .. 7 of a 16-row tile and its second ones in rows 8 .. 15, so that one mma takes both and a thread has scores and outputs
+// of one row instead of two; else sixteen rows. Every warp of a block takes tiles of keys of its own.
+template <int CT, typename TQ, int D_, bool HALF_>
 struct Cfg {
-  static constexpr bool HALF = MT_ == 0;
-  static constexpr int D = D_, MT = HALF ? 1 : MT_, WR = WR_, WK = WK_, H = HALF ? 1 : 2;   // H: rows of a thread in a tile
+  static constexpr bool HALF = HALF_;
+  static constexpr int D = D_, WK = 4, H = HALF ? 1 : 2;                 // warps of a block; rows of a thread
   static constexpr bool BF = CT == TREE_BF16, WIDE = CT == TREE_BF16 || CT == TREE_F16, E4M3 = CT == TREE_E4M3;
   static constexpr int ES = WIDE ? 2 : 1;
   static constexpr bool QF = std::is_same<TQ, float>::value, QB = std::is_same<TQ, __nv_bfloat16>::value;
-  // q8 keys of few rows are operands as they are, of whole-number products; Q is three signed bytes of its row's largest element
-  static constexpr bool I8 = CT == TREE_Q8 && MT_ <= 1;
+  // q8 keys are operands as they are, of whole-number products; Q is three signed bytes of its row's largest element
+  static constexpr bool I8 = CT == TREE_Q8;
   static constexpr int QT = I8 ? 3 : BF ? (QB ? 1 : QF ? 3 : 2) : (QF ? 2 : 1);   // terms of Q
   static constexpr int PT = BF ? (QF ? 3 : 2) : (QB ? 1 : 2);            // terms of P
   static constexpr int NQ = HALF ? (QT + 1) / 2 : QT, NP = HALF ? (PT + 1) / 2 : PT;   // operands of Q and P
-  static constexpr int RB = 8 * H * MT * WR;                             // rows of a block
-  static constexpr int THREADS = 32 * WR * WK;
-  static constexpr int KT = (WIDE ? 16 : 32) * (WR >= 2 ? 2 : 1); // keys of a tile
+  static constexpr int RB = 8 * H;                                       // rows of a block
+  static constexpr int THREADS = 32 * WK;
+  static constexpr int KT = WIDE ? 16 : 32;                              // keys of a tile
   static constexpr int STAGES = 3;
   static constexpr int BLOCKS = HALF ? 2 : 1;                            // of an SM, as far as registers go
   static constexpr int TILE = KT * D * ES;
@@ -212,11 +204,8 @@ struct Cfg {
   // keep the weights' bits instead
   static constexpr float SLACK = QF ? 0.f : 8.f;
   static constexpr int PEXP = QF ? 13 : 5;                               // f16 weights enter times 2^PEXP
-  static constexpr bool QREG = MT == 1;                                  // Q stays in registers, else in shared memory
-  static constexpr int QSM = QREG ? 0 : RB * D * 2 * QT;
-  static constexpr int STATE = WK * RB * (D + 2) * 4;                    // (output, maximum, sum) of every key group
-  static constexpr int BODY = RING > STATE ? RING : STATE;
-  static constexpr int SMEM = BODY + QSM;
+  static constexpr int STATE = WK * RB * (D + 2) * 4;                    // (output, maximum, sum) of every warp
+  static constexpr int SMEM = RING > STATE ? RING : STATE;
 };
 
 template <typename C>
@@ -265,19 +254,18 @@ __device__ __forceinline__ uint32_t seen_of(const TreeArgs& a, int64_t b, int ro
   return bits;
 }
 
-template <int CT, typename TQ, int D, int MT_, int WR, int WK>
-__global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLOCKS) tree_attention_kernel(const __grid_constant__ TreeArgs a) {
-  using C = Cfg<CT, TQ, D, MT_, WR, WK>;
+template <int CT, typename TQ, int D, bool HALF>
+__global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, HALF>::BLOCKS) tree_attention_kernel(const __grid_constant__ TreeArgs a) {
+  using C = Cfg<CT, TQ, D, HALF>;
   using O = Op<C::BF>;
-  constexpr int KT = C::KT, NT = D / 8, KS = D / 16, NK = KT / 8, MT = C::MT, H = C::H, NE = 2 * H;  // NE: a thread's entries of an n8 tile
+  constexpr int KT = C::KT, NT = D / 8, KS = D / 16, NK = KT / 8, WK = C::WK, H = C::H, NE = 2 * H;  // NE: a thread's entries of an n8 tile
   extern __shared__ __align__(128) uint8_t tree_shared[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-  const int wr = warp % WR, wk = warp / WR;
   const int split = (int)blockIdx.x % a.splits;
   const int64_t pair = blockIdx.x / a.splits;
   const int64_t b = pair / a.kv_heads;
   const int kvh = (int)(pair - b * a.kv_heads);
-  const int total_rows = a.rows * a.group, row0 = blockIdx.y * C::RB;
+  const int total_rows = a.rows * a.group;  // at most C::RB
 
   int64_t len = a.lengths[b];
   int64_t keys = 0;
@@ -290,13 +278,12 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
   const float* ksb = C::WIDE ? nullptr : a.ks + b * a.kss[0] + kvh * a.kss[1];
   const float* vsb = C::WIDE ? nullptr : a.vs + b * a.vss[0] + kvh * a.vss[1];
 
-  // ---- tiles: the group takes every (splits * WK)-th one ----
+  // ---- tiles: a warp takes every (splits * WK)-th one ----
   const int tiles = (int)((keys + KT - 1) / KT);
-  const int first = split * WK + wk, step = a.splits * WK;
-  const uint32_t ring = smem_u32(tree_shared) + (uint32_t)(wk * C::STAGES * C::STAGE);
-  const int gtid = wr * 32 + lane;
-  constexpr int PER = D * C::ES / 16, ROWS = 32 * WR / PER, COPIES = KT / ROWS;  // a thread's copies lie ROWS keys apart
-  const int my_key = gtid / PER, my_chunk = gtid % PER;
+  const int first = split * WK + warp, step = a.splits * WK;
+  const uint32_t ring = smem_u32(tree_shared) + (uint32_t)(warp * C::STAGES * C::STAGE);
+  constexpr int PER = D * C::ES / 16, ROWS = 32 / PER, COPIES = KT / ROWS;  // a thread's copies lie ROWS keys apart
+  const int my_key = lane / PER, my_chunk = lane % PER;
   const bool my_dims = my_chunk < a.d * C::ES / 16;
   const uint8_t* const kp = kb + my_key * a.kst[2] + my_chunk * 16;
   const uint8_t* const vp = vb + my_key * a.vst[2] + my_chunk * 16;
@@ -322,7 +309,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
       }
       if (!C::WIDE) {
 #pragma unroll
-        for (int u = gtid; u < 2 * KT; u += 32 * WR) {  // the keys' scales, then the values'
+        for (int u = lane; u < 2 * KT; u += 32) {  // the keys' scales, then the values'
           const int64_t kk = key0 + (u & (KT - 1));
           const float* const of = u < KT ? ksb : vsb;
           cp4(at + 2 * C::TILE + u * 4, kk < keys ? of + kk : of, kk < keys);
@@ -339,15 +326,13 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
 
   // ---- Q: this warp's rows, in the order in which keys' dimensions come out ----
   // element e (0 .. 3) of k16 step s at lane quarter t: 2-byte keys 16 s + 2 t + {0, 1, 8, 9}; 8-bit keys lie 16 bytes per lane
-  uint32_t qf[C::QREG ? C::NQ : 1][C::QREG ? C::QS : 1][4];
-  uint8_t* qs = tree_shared + C::BODY;
-  float mult[MT][H];  // what a row's scores are multiplied with: log2(e) * scale / the row's factor
-#pragma unroll
-  for (int m = 0; m < MT; m++) {
+  uint32_t qf[C::NQ][C::QS][4];
+  float mult[H];  // what a row's scores are multiplied with: log2(e) * scale / the row's factor
+  {
     float x[H][KS][4];
 #pragma unroll
     for (int h = 0; h < H; h++) {
-      const int r = row0 + (wr * MT + m) * 16 + g + 8 * h;
+      const int r = g + 8 * h;
       const bool live = r < total_rows;
       const int tr = live ? r / a.group : 0, gh = live ? r - tr * a.group : 0;
       const TQ* src = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
@@ -382,15 +367,11 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
 #pragma unroll
           for (int e = 0; e < 4; e++) x[h][s][e] *= mul;
       }
-      mult[m][h] = a.scale * LOG2E * inv;
+      mult[h] = a.scale * LOG2E * inv;
     }
     auto keep = [&](int n, int s, const uint32_t (&f)[4]) {
-      if (C::QREG) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) qf[C::QREG ? n : 0][C::QREG ? s : 0][i] = f[i];
-      } else if (wk == 0) {
-        *reinterpret_cast<uint4*>(qs + ((((wr * MT + m) * C::NQ + n) * C::QS + s) * 32 + lane) * 16) = make_uint4(f[0], f[1], f[2], f[3]);
-      }
+      for (int i = 0; i < 4; i++) qf[n][s][i] = f[i];
     };
     if (C::I8) {
 #pragma unroll
@@ -427,42 +408,25 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
         }
     }
   }
-  if (!C::QREG) __syncthreads();
-  const uint32_t qaddr = smem_u32(qs) + (uint32_t)(wr * MT * C::NQ * C::QS * 512 + lane * 16);
-  auto query = [&](int m, int n, int s, uint32_t (&f)[4]) {
-    if (C::QREG) {
-#pragma unroll
-      for (int i = 0; i < 4; i++) f[i] = qf[C::QREG ? n : 0][C::QREG ? s : 0][i];
-    } else {
-      const uint4 w = lds16(qaddr + (uint32_t)(((m * C::NQ + n) * C::QS + s) * 512));
-      f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w;
-    }
-  };
 
   // ---- the running state ----
-  float out[MT][NT][NE], top[MT][H], sum[MT][H];
+  float out[NT][NE], top[H], sum[H];
   int vex = 30;  // 8-bit: exponent that the values' scales are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
   // Values that are not finite: weight 0, or a weight's zero second term, times one is not a number. Where a result is not finite
   // the keys are gone through once more, with such entries left out of the products and added one by one. (Codes of q8 are finite.)
   constexpr bool ODD = CT != TREE_Q8;
   for (bool careful = false;; careful = true) {
 #pragma unroll
-    for (int m = 0; m < MT; m++) {
+    for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int n = 0; n < NT; n++)
+      for (int e = 0; e < NE; e++) out[n][e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < NE; e++) out[m][n][e] = 0.f;
-#pragma unroll
-      for (int h = 0; h < H; h++) top[m][h] = -INFINITY, sum[m][h] = 0.f;
-    }
+    for (int h = 0; h < H; h++) top[h] = -INFINITY, sum[h] = 0.f;
     vex = 30;
     int stage = 0;
     for (int tile = first; tile < tiles; tile += step) {
       cp_wait<C::STAGES - 2>();
-      if (WR > 1)
-        asm volatile("bar.sync %0, %1;" ::"r"(wk + 1), "n"(32 * WR) : "memory");
-      else
-        __syncwarp();
+      __syncwarp();
       {
         int ahead = stage + C::STAGES - 1;
         if (ahead >= C::STAGES) ahead -= C::STAGES;
@@ -472,7 +436,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
       if (++stage == C::STAGES) stage = 0;
 
       // S
-      float sc[MT][NK][NE];
+      float sc[NK][NE];
       if constexpr (C::I8) {
         int acc[3][NK][4] = {};  // leading, second (not HALF: HALF has both in one), last terms
         uint4 raw[NK][D / 64];
@@ -484,12 +448,10 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
         for (int s = 0; s < C::QS; s++)
 #pragma unroll
           for (int n = 0; n < C::NQ; n++) {
-            uint32_t f[4];
-            query(0, n, s, f);
 #pragma unroll
             for (int j = 0; j < NK; j++) {
               const uint4 w = raw[j][s / 2];
-              mma_s8(acc[n][j], f, s & 1 ? w.z : w.x, s & 1 ? w.w : w.y);
+              mma_s8(acc[n][j], qf[n][s], s & 1 ? w.z : w.x, s & 1 ? w.w : w.y);
             }
           }
 #pragma unroll
@@ -497,10 +459,10 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
 #pragma unroll
           for (int e = 0; e < NE; e++) {
             const int lead = acc[0][j][e], mid = C::HALF ? acc[0][j][(e + 2) & 3] : acc[1][j][e], low = acc[C::NQ - 1][j][e];
-            sc[0][j][e] = fmaf((float)lead, 65536.f, (float)(mid * 256 + low));
+            sc[j][e] = fmaf((float)lead, 65536.f, (float)(mid * 256 + low));
           }
       } else {
-        float acc[MT][NK][4] = {};
+        float acc[NK][4] = {};
 #pragma unroll
         for (int s = 0; s < KS; s++) {
           uint32_t kf[NK][2];
@@ -521,21 +483,15 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
             }
           }
 #pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
             for (int n = C::NQ - 1; n >= 0; n--) {
-              uint32_t f[4];
-              query(m, n, s % C::QS, f);
 #pragma unroll
-              for (int j = 0; j < NK; j++) O::mma(acc[m][j], f, kf[j][0], kf[j][1]);
+              for (int j = 0; j < NK; j++) O::mma(acc[j], qf[n][s % C::QS], kf[j][0], kf[j][1]);
             }
         }
 #pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
           for (int j = 0; j < NK; j++)
 #pragma unroll
-            for (int e = 0; e < NE; e++) sc[m][j][e] = C::HALF ? acc[m][j][e] + acc[m][j][e + 4 - NE] : acc[m][j][e];
+            for (int e = 0; e < NE; e++) sc[j][e] = C::HALF ? acc[j][e] + acc[j][e + 4 - NE] : acc[j][e];
       }
 
       // scores in powers of two, masked
@@ -552,9 +508,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
             most = fmaxf(most, vscale[C::WIDE ? 0 : j][e]);
             const float kscale = lds4(st + (uint32_t)(j * 8 + 2 * t + e) * 4);
 #pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
-              for (int h = 0; h < H; h++) sc[m][j][2 * h + e] *= kscale;
+              for (int h = 0; h < H; h++) sc[j][2 * h + e] *= kscale;
           }
         int ex = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23);
         ex = ex < 30 ? 30 : ex > 240 ? 240 : ex;
@@ -562,17 +516,13 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
       }
       const float pmul = C::BF ? 1.f : C::WIDE ? (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(254 + C::PEXP - vex) << 23);
       const bool tail = key0 + KT > len;
-      uint32_t vis[MT][H];
+      uint32_t vis[H];
 #pragma unroll
-      for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int h = 0; h < H; h++) vis[m][h] = 0xffffffffu;
+        for (int h = 0; h < H; h++) vis[h] = 0xffffffffu;
       if (tail) {
 #pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
           for (int h = 0; h < H; h++) {
-            const int r = row0 + (wr * MT + m) * 16 + g + 8 * h;
+            const int r = g + 8 * h;
             const int tr = r < total_rows ? r / a.group : 0;
             uint32_t bits = 0;
 #pragma unroll
@@ -580,13 +530,11 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
               const int64_t key = key0 + (i >> 1) * 8 + 2 * t + (i & 1);
               if (key < keys && sees(a, b, tr, key - len)) bits |= 1u << i;
             }
-            vis[m][h] = bits;
+            vis[h] = bits;
           }
       }
-      float decay[MT][H];
+      float decay[H];
       bool change = grow != 1.f;
-#pragma unroll
-      for (int m = 0; m < MT; m++)
 #pragma unroll
         for (int h = 0; h < H; h++) {
           // the maximum in powers of two; a score and its reference go through one fma, so that the score is not rounded before
@@ -596,57 +544,53 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
           for (int j = 0; j < NK; j++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              const float s = sc[m][j][2 * h + e] * mult[m][h];
-              best = fmaxf(best, !tail || vis[m][h] >> (2 * j + e) & 1 ? s : -INFINITY);
+              const float s = sc[j][2 * h + e] * mult[h];
+              best = fmaxf(best, !tail || vis[h] >> (2 * j + e) & 1 ? s : -INFINITY);
             }
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-          decay[m][h] = grow;
-          if (best > top[m][h] + C::SLACK || top[m][h] == -INFINITY) {
-            if (best > -INFINITY) decay[m][h] *= ex2(top[m][h] - best), change = true;
-            sum[m][h] *= ex2(top[m][h] - (best == -INFINITY ? 0.f : best));
-            top[m][h] = best;
+          decay[h] = grow;
+          if (best > top[h] + C::SLACK || top[h] == -INFINITY) {
+            if (best > -INFINITY) decay[h] *= ex2(top[h] - best), change = true;
+            sum[h] *= ex2(top[h] - (best == -INFINITY ? 0.f : best));
+            top[h] = best;
           }
-          const float base = top[m][h] == -INFINITY ? 0.f : top[m][h];
+          const float base = top[h] == -INFINITY ? 0.f : top[h];
           float part = 0.f;
 #pragma unroll
           for (int j = 0; j < NK; j++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              float p = ex2(fmaf(sc[m][j][2 * h + e], mult[m][h], -base));
-              if (tail && !(vis[m][h] >> (2 * j + e) & 1)) p = 0.f;
-              sc[m][j][2 * h + e] = p;
+              float p = ex2(fmaf(sc[j][2 * h + e], mult[h], -base));
+              if (tail && !(vis[h] >> (2 * j + e) & 1)) p = 0.f;
+              sc[j][2 * h + e] = p;
               part += p;
             }
-          sum[m][h] += part;
+          sum[h] += part;
         }
       if (__any_sync(0xffffffffu, change)) {
 #pragma unroll
-        for (int m = 0; m < MT; m++)
-#pragma unroll
           for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < NE; e++) out[m][n][e] *= decay[m][e >> 1];
+            for (int e = 0; e < NE; e++) out[n][e] *= decay[e >> 1];
       }
       // weights as operands
-      uint32_t pf[MT][C::NP][NK / 2][4];
-#pragma unroll
-      for (int m = 0; m < MT; m++)
+      uint32_t pf[C::NP][NK / 2][4];
 #pragma unroll
         for (int j = 0; j < NK; j++) {
           float w[NE];
 #pragma unroll
           for (int e = 0; e < NE; e++) {
-            w[e] = sc[m][j][e] * pmul;
+            w[e] = sc[j][e] * pmul;
             if (!C::WIDE) {
               w[e] *= vscale[C::WIDE ? 0 : j][e & 1];
-              if (tail && !(vis[m][e >> 1] >> (2 * j + (e & 1)) & 1)) w[e] = 0.f;  // the scale of a key that is not seen
+              if (tail && !(vis[e >> 1] >> (2 * j + (e & 1)) & 1)) w[e] = 0.f;  // the scale of a key that is not seen
             }
           }
 #pragma unroll
           for (int n = 0; n < C::NP; n++) {
-            pf[m][n][j / 2][(j & 1) * 2] = O::take(w[0], w[1]);
-            pf[m][n][j / 2][(j & 1) * 2 + 1] = !C::HALF || 2 * n + 1 < C::PT ? O::take(w[NE - 2], w[NE - 1]) : 0u;
+            pf[n][j / 2][(j & 1) * 2] = O::take(w[0], w[1]);
+            pf[n][j / 2][(j & 1) * 2 + 1] = !C::HALF || 2 * n + 1 < C::PT ? O::take(w[NE - 2], w[NE - 1]) : 0u;
           }
         }
       bool odd = false;
@@ -660,14 +604,14 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
         odd = __any_sync(0xffffffffu, odd);
       }
       // O += P V: products of the tile start from zero
-      auto fold = [&](int m, int n, const float (&u)[4]) {
+      auto fold = [&](int n, const float (&u)[4]) {
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) add2(out[m][n][e % NE], out[m][n][e % NE + 1], u[e], u[e + 1]);
+        for (int e = 0; e < 4; e += 2) add2(out[n][e % NE], out[n][e % NE + 1], u[e], u[e + 1]);
       };
       if (C::WIDE) {
 #pragma unroll
         for (int nb = 0; nb < NT / 2; nb++) {
-          float u[MT][2][4] = {};
+          float u[2][4] = {};
 #pragma unroll
           for (int kk = 0; kk < NK / 2; kk++) {
             uint32_t r[4];
@@ -678,17 +622,13 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
               for (int i = 0; i < 4; i++) without_odd<C::BF>(r[i]);
             }
 #pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
               for (int n = C::NP - 1; n >= 0; n--) {
-                O::mma(u[m][0], pf[m][n][kk], r[0], r[1]);
-                O::mma(u[m][1], pf[m][n][kk], r[2], r[3]);
+                O::mma(u[0], pf[n][kk], r[0], r[1]);
+                O::mma(u[1], pf[n][kk], r[2], r[3]);
               }
           }
 #pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) fold(m, 2 * nb + i, u[m][i]);
+            for (int i = 0; i < 2; i++) fold(2 * nb + i, u[i]);
         }
       } else {
         // lane g has D / 8 consecutive dimensions of a key: n8 tile i is dimension g * D / 8 + i
@@ -713,23 +653,19 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
           }
 #pragma unroll
         for (int w = 0; w < WORDS; w++) {
-          float u[MT][4][4] = {};
+          float u[4][4] = {};
 #pragma unroll
           for (int kk = 0; kk < NK / 2; kk++) {
             uint32_t r0[4], r1[4];
             widen_pairs<C::E4M3>(x[kk][0][w], x[kk][1][w], r0);
             widen_pairs<C::E4M3>(x[kk][2][w], x[kk][3][w], r1);
 #pragma unroll
-            for (int m = 0; m < MT; m++)
-#pragma unroll
               for (int n = C::NP - 1; n >= 0; n--)
 #pragma unroll
-                for (int i = 0; i < 4; i++) O::mma(u[m][i], pf[m][n][kk], r0[i], r1[i]);
+                for (int i = 0; i < 4; i++) O::mma(u[i], pf[n][kk], r0[i], r1[i]);
           }
 #pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) fold(m, w * 4 + i, u[m][i]);
+            for (int i = 0; i < 4; i++) fold(w * 4 + i, u[i]);
         }
       }
       if (ODD && odd) {
@@ -738,15 +674,13 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
         for (int key = 0; key < KT; key++) {
           const int j = key / 8, from = (lane & ~3) + (key & 7) / 2;
 #pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
             for (int h = 0; h < H; h++) {
               // which of the two columns is a matter of the key: picked without indexing registers
               float p = 0.f;
               uint32_t seen = 0;
 #pragma unroll
               for (int jj = 0; jj < NK; jj++)
-                if (jj == j) p = key & 1 ? sc[m][jj][2 * h + 1] : sc[m][jj][2 * h], seen = vis[m][h] >> (2 * jj + (key & 1)) & 1;
+                if (jj == j) p = key & 1 ? sc[jj][2 * h + 1] : sc[jj][2 * h], seen = vis[h] >> (2 * jj + (key & 1)) & 1;
               p = __shfl_sync(0xffffffffu, p, from), seen = __shfl_sync(0xffffffffu, seen, from);
 #pragma unroll
               for (int n = 0; n < NT; n++)
@@ -765,7 +699,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
                     asm volatile("ld.shared.u8 %0, [%1];" : "=r"(bits) : "r"(at));
                     if ((bits & 0x7fu) == 0x7fu) val = __uint_as_float(0x7fc00000u);
                   }
-                  if (seen && val != 0.f) out[m][n][2 * h + e] += p * val;
+                  if (seen && val != 0.f) out[n][2 * h + e] += p * val;
                 }
             }
         }
@@ -775,59 +709,50 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
     if (!ODD || careful) break;
     bool finite = true;
 #pragma unroll
-    for (int m = 0; m < MT; m++)
-#pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
-        for (int e = 0; e < NE; e++) finite = finite && fabsf(out[m][n][e]) < INFINITY;
+        for (int e = 0; e < NE; e++) finite = finite && fabsf(out[n][e]) < INFINITY;
     if (!__syncthreads_or(!finite)) break;
     begin();
   }
   // out in its own units again
   const float unit = C::BF ? 1.f : C::WIDE ? 1.f / (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(vex - C::PEXP) << 23);
 #pragma unroll
-  for (int m = 0; m < MT; m++)
-#pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int e = 0; e < NE; e++) out[m][n][e] *= unit;
-#pragma unroll
-  for (int m = 0; m < MT; m++)
+      for (int e = 0; e < NE; e++) out[n][e] *= unit;
 #pragma unroll
     for (int h = 0; h < H; h++) {
-      sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 1);
-      sum[m][h] += __shfl_xor_sync(0xffffffffu, sum[m][h], 2);
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+      sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
     }
   __syncthreads();  // the ring becomes the states' place
 
-  // ---- states of the key groups, then of the cluster's blocks ----
+  // ---- states of the warps, then of the cluster's blocks ----
   float* so = reinterpret_cast<float*>(tree_shared);          // [WK][RB][D]
   float* sm = so + WK * C::RB * D;                             // [WK][RB] (maximum, sum)
 #pragma unroll
-  for (int m = 0; m < MT; m++)
-#pragma unroll
     for (int h = 0; h < H; h++) {
-      const int r = (wr * MT + m) * 16 + g + 8 * h;
-      float* to = so + (wk * C::RB + r) * D;
+      const int r = g + 8 * h;
+      float* to = so + (warp * C::RB + r) * D;
       if (C::WIDE) {
 #pragma unroll
-        for (int n = 0; n < NT; n++) *reinterpret_cast<float2*>(to + n * 8 + 2 * t) = make_float2(out[m][n][2 * h], out[m][n][2 * h + 1]);
+        for (int n = 0; n < NT; n++) *reinterpret_cast<float2*>(to + n * 8 + 2 * t) = make_float2(out[n][2 * h], out[n][2 * h + 1]);
       } else {
 #pragma unroll
         for (int e = 0; e < 2; e++)
 #pragma unroll
           for (int n = 0; n < NT; n += 4)
             *reinterpret_cast<float4*>(to + (2 * t + e) * (D / 8) + n) =
-                make_float4(out[m][n][2 * h + e], out[m][n + 1][2 * h + e], out[m][n + 2][2 * h + e], out[m][n + 3][2 * h + e]);
+                make_float4(out[n][2 * h + e], out[n + 1][2 * h + e], out[n + 2][2 * h + e], out[n + 3][2 * h + e]);
       }
-      if (t == 0) sm[(wk * C::RB + r) * 2] = top[m][h], sm[(wk * C::RB + r) * 2 + 1] = sum[m][h];
+      if (t == 0) sm[(warp * C::RB + r) * 2] = top[h], sm[(warp * C::RB + r) * 2 + 1] = sum[h];
     }
   __syncthreads();
   // group states into the first one: a thread takes four dimensions of a row
-  const int live_rows = min(C::RB, total_rows - row0);
   if (WK > 1) {
     float best[1];
-    for (int i = threadIdx.x; i < live_rows * (D / 4); i += C::THREADS) {
+    for (int i = threadIdx.x; i < total_rows * (D / 4); i += C::THREADS) {
       const int r = i / (D / 4), c = i % (D / 4) * 4;
       best[0] = -INFINITY;
 #pragma unroll
@@ -843,7 +768,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
       *reinterpret_cast<float4*>(so + r * D + c) = o;
     }
     __syncthreads();
-    for (int r = threadIdx.x; r < live_rows; r += C::THREADS) {
+    for (int r = threadIdx.x; r < total_rows; r += C::THREADS) {
       float m = -INFINITY, l = 0.f;
 #pragma unroll
       for (int w = 0; w < WK; w++) m = fmaxf(m, sm[(w * C::RB + r) * 2]);
@@ -858,7 +783,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
     __syncthreads();
   // a block of the cluster takes every splits-th piece of four dimensions
   const uint32_t so_at = smem_u32(so), sm_at = smem_u32(sm);
-  for (int i = split * C::THREADS + threadIdx.x; i < live_rows * (D / 4); i += a.splits * C::THREADS) {
+  for (int i = split * C::THREADS + threadIdx.x; i < total_rows * (D / 4); i += a.splits * C::THREADS) {
     const int r = i / (D / 4), c = i % (D / 4) * 4;
     float m = -INFINITY, l = 0.f;
     float o[4] = {};
@@ -876,7 +801,7 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
       for (int e = 0; e < 4; e++) o[e] = o[e] * fa + x[e] * fb;
       m = next;
     }
-    const int tr = (row0 + r) / a.group, gh = row0 + r - tr * a.group;
+    const int tr = r / a.group, gh = r - tr * a.group;
     TQ* to = static_cast<TQ*>(a.out) + ((b * a.rows + tr) * a.heads + (int64_t)kvh * a.group + gh) * a.d + c;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (c < a.d) {
@@ -887,22 +812,21 @@ __global__ void __launch_bounds__(32 * WR * WK, Cfg<CT, TQ, D, MT_, WR, WK>::BLO
   if (a.splits > 1) asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");  // others read this block's states
 }
 
-template <int CT, typename TQ, int D, int MT, int WR, int WK>
+template <int CT, typename TQ, int D, bool HALF>
 int run(TreeArgs a, cudaStream_t s) {
-  using C = Cfg<CT, TQ, D, MT, WR, WK>;
-  auto kernel = tree_attention_kernel<CT, TQ, D, MT, WR, WK>;
+  using C = Cfg<CT, TQ, D, HALF>;
+  auto kernel = tree_attention_kernel<CT, TQ, D, HALF>;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), C::SMEM)) return 1;
   const int64_t pairs = a.batch * a.kv_heads;
-  a.row_blocks = (int)(((int64_t)a.rows * a.group + C::RB - 1) / C::RB);
-  // blocks of a cluster: as many as there is room for at once, at least a tile for each key group at full capacity
+  // blocks of a cluster: as many as there is room for at once, at least a tile for each warp at full capacity
   const int64_t room = (int64_t)std::max(1, sm_count()) * std::max(1, std::min(2, (227 << 10) / (C::SMEM + 1024)));
   int splits = 16;
-  while (splits > 1 && (pairs * a.row_blocks * splits > room || a.cap < (int64_t)splits * WK * C::KT)) splits--;
+  while (splits > 1 && (pairs * splits > room || a.cap < (int64_t)splits * C::WK * C::KT)) splits--;
   if (splits > 8) DYN_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   a.splits = splits;
-  DYN_CHECK(pairs * splits <= 0x7fffffff && a.row_blocks <= 65535, "tree_attention: too many sequences or rows for one call");
+  DYN_CHECK(pairs * splits <= 0x7fffffff, "tree_attention: too many sequences for one call");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(pairs * splits), (unsigned)a.row_blocks), cfg.blockDim = dim3(C::THREADS);
+  cfg.gridDim = dim3((unsigned)(pairs * splits)), cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM, cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -666,14 +666,14 @@ int run_wide(TreeArgs a, cudaStream_t s) {
   }
   DYN_CHECK(launch_regs >= C::START, "tree_attention: built with %d registers a thread", launch_regs.load());
   const int64_t pairs = a.batch * a.kv_heads;
-  a.row_blocks = (int)(((int64_t)a.rows * a.group + W_ROWS - 1) / W_ROWS);
+  const int64_t row_blocks = ((int64_t)a.rows * a.group + W_ROWS - 1) / W_ROWS;
   // blocks of a cluster: as many as fit the SMs at once (a block takes an SM), at least two tiles each at full capacity
   int splits = 8;
-  while (splits > 1 && (pairs * a.row_blocks * splits > std::max(1, sm_count()) || a.cap < (int64_t)splits * W_KEYS * 2)) splits--;
+  while (splits > 1 && (pairs * row_blocks * splits > std::max(1, sm_count()) || a.cap < (int64_t)splits * W_KEYS * 2)) splits--;
   a.splits = splits;
-  DYN_CHECK(pairs * splits <= 0x7fffffff && a.row_blocks <= 65535, "tree_attention: too many sequences or rows for one call");
+  DYN_CHECK(pairs * splits <= 0x7fffffff && row_blocks <= 65535, "tree_attention: too many sequences or rows for one call");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(pairs * splits), (unsigned)a.row_blocks), cfg.blockDim = dim3(C::THREADS);
+  cfg.gridDim = dim3((unsigned)(pairs * splits), (unsigned)row_blocks), cfg.blockDim = dim3(C::THREADS);
   cfg.dynamicSmemBytes = C::SMEM, cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -686,10 +686,12 @@ int run_wide(TreeArgs a, cudaStream_t s) {
 
 template <int CT, typename TQ, int D>
 int by_rows(const TreeArgs& a, cudaStream_t s) {
+  // us with 8 kv heads of 128, 4 query heads each; 16 rows here / there: q8 keys with f32 queries, 1 sequence of 500 14.3 / 17.9, of 4000
+  // 18.0 / 25.4, 8 of 500 19.5 / 19.4, 8 of 4000 35.4 / 57.3; bf16 for both 12.7 / 11.9, 16.2 / 17.6, 14.3 / 12.7, 33.6 / 35.4. 20 rows in
+  // two tiles of sixteen per warp / there: 20.6 / 18.5, 40.0 / 25.8, 22.3 / 19.7, 63.8 / 57.2, and 18.9 / 12.0, 23.5 / 17.5, 21.3 / 12.6, 50.7 / 35.4
   const int64_t rows = (int64_t)a.rows * a.group;
-  if (rows <= 8) return run<CT, TQ, D, 0, 1, 4>(a, s);
-  if (rows <= 16) return run<CT, TQ, D, 1, 1, 4>(a, s);
-  if (rows <= 32) return run<CT, TQ, D, 2, 1, 4>(a, s);
+  if (rows <= 8) return run<CT, TQ, D, true>(a, s);
+  if (rows <= 16) return run<CT, TQ, D, false>(a, s);
   return run_wide<CT, TQ, D>(a, s);
 }
 
