@@ -25,8 +25,12 @@ bool sane(int64_t n) { return n >= 0 && n <= (1ll << 31) - 1; }
 template <int N>
 struct Steps {
   int64_t v[N];
+  bool repeats = false;  // a dimension of several entries without a step: what is written there would meet
   Steps(const int64_t* of, const int64_t* extents, int dims) {
-    for (int i = 0; i < N; i++) v[i] = of && extents[i % dims] > 1 ? of[i] : 0;
+    for (int i = 0; i < N; i++) {
+      v[i] = of && extents[i % dims] > 1 ? of[i] : 0;
+      repeats = repeats || (extents[i % dims] > 1 && v[i] == 0);
+    }
   }
 };
 
@@ -50,6 +54,8 @@ int kv_rows(const char* what, const void* k, const void* v, int type, const int6
   bool even = aligned(k_cache, 16) && aligned(v_cache, 16);
   for (int64_t step : cache_steps.v) even = even && step % 16 == 0;
   DYN_CHECK(even, "%s: caches and their strides must be multiples of 16 bytes", what);
+  DYN_CHECK(!write || !(cache_steps.repeats || scale_steps.repeats), "%s: a cache dimension has stride 0, rows would be written over one another", what);
+  DYN_CHECK(write || !x_steps.repeats, "%s: an output dimension has stride 0", what);
   if (have_device()) return 1;
   KvRows r{};
   // read-only when writing; the struct serves both directions
@@ -82,9 +88,10 @@ int dyninfer_cuda_rotary(const void* x_dev, int type, const int64_t* x_strides, 
   DYN_CHECK(aligned(x_dev, type_bytes(type)) && aligned(y_dev, type_bytes(type)) && aligned(positions_dev, 8),
             "rotary: a pointer is not aligned to its type");
   for (int64_t i = 0; i < rotary_dim / 2; i++) DYN_CHECK(isfinite(frequencies[i]), "rotary: frequency %lld is not finite", (long long)i);
-  if (have_device()) return 1;
   const int64_t extents[3] = {batch, rows, heads};
   const Steps<3> x_steps(x_strides, extents, 3), y_steps(y_strides, extents, 3);
+  DYN_CHECK(!y_steps.repeats, "rotary: an output dimension has stride 0");
+  if (have_device()) return 1;
   return launch_rotary(x_dev, type, batch, rows, heads, d, x_steps.v, positions_dev, frequencies, rotary_dim, interleaved != 0,
                        magnitude, y_dev, y_steps.v, (cudaStream_t)stream);
 }

@@ -159,6 +159,10 @@ def argmax(v: torch.Tensor) -> int:
 
 
 # ---- speculative decoding: a tree of drafted tokens over a cache -----------------------------------------------------
+# A step: `rotary` turns the drafted rows to their depths, `kv_write` puts their keys and values behind the cache's rows,
+# `tree_attention` attends under the tree's mask, `verify_draft` says which tokens stand; the rows that do are written once more in
+# their order (`kv_write` of the path's rows with counts). All are asynchronous on torch's current stream and may be captured; the
+# first call of each on a device does set-up work.
 
 _SCALED = {torch.int8: _lib.KV["q8"], torch.float8_e4m3fn: _lib.KV["e4m3"]}
 _KV = {**_SCALED, torch.float16: ENC["plain.f16"], torch.bfloat16: ENC["plain.bf16"]}

@@ -150,8 +150,11 @@ int dyninfer_cuda_argmax_static(const float* v_dev, int64_t n, int64_t* out_inde
  * A step over a tree of drafted tokens: its rows are rotated to their depths, written behind the
  * cache's rows, attended to under the tree's mask, and verified against the target. Strides are
  * host arrays that count elements (not bytes); the last dimension is always dense. `type` is
- * DYNINFER_ENC_F32, _F16 or _BF16. Work is asynchronous on `stream`, nothing is allocated, and
- * nothing is kept between calls, so all five may be captured into graphs. */
+ * DYNINFER_ENC_F32, _F16 or _BF16. Work is asynchronous on `stream`, takes no scratch and keeps nothing
+ * between calls, so all five may be captured into graphs (the first call of each on a device does
+ * set-up work: make it before the capture). tree_attention of more than 16 rows x query heads per kv
+ * head waits inside its kernel, with limits: dyninfer_cuda_check_device_error says if one ran out.
+ * Outputs may not repeat memory (stride 0) nor overlap inputs, but for rotary in place. */
 
 /* cache types besides DYNINFER_ENC_F16 / _BF16: one byte per element and one f32 scale per row */
 enum {

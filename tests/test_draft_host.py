@@ -104,6 +104,8 @@ def test_native_rotary_refusals(native_lib):
     native_refusal("rotary", "magnitude", AT, 0, S3, AT, at, 8, 0, math.inf, 1, 1, 1, 8, AT, S3, None)
     native_refusal("rotary", "NULL", None, 0, S3, AT, at, 8, 0, 1.0, 1, 1, 1, 8, AT, S3, None)
     native_refusal("rotary", "aligned", AT + 2, 0, S3, AT, at, 8, 0, 1.0, 1, 1, 1, 8, AT, S3, None)
+    flat = (C.c_int64 * 3)(16, 0, 16)
+    native_refusal("rotary", "stride 0", AT, 0, flat, AT, at, 8, 0, 1.0, 1, 2, 2, 8, AT, flat, None)
     f[2] = math.nan
     native_refusal("rotary", "frequency 2", AT, 0, S3, AT, at, 8, 0, 1.0, 1, 1, 1, 8, AT, S3, None)
     assert native_lib.dyninfer_cuda_rotary(None, 0, None, None, at, 8, 0, 1.0, 0, 1, 1, 8, None, None, None) == 0   # nothing to do
@@ -121,6 +123,7 @@ def test_native_cache_refusals(native_lib):
     native_refusal("kv_write", "aligned", *write(x=AT + 2))
     native_refusal("kv_write", "multiples of 16", *write(codes=AT + 8))
     native_refusal("kv_write", "multiples of 16", *write(strides=(C.c_int64 * 6)(16, 16, 16, 16, 16, 24), cap=2))
+    native_refusal("kv_write", "stride 0", *write(strides=(C.c_int64 * 6)(0, 16, 16, 0, 16, 16), batch=2))
     assert native_lib.dyninfer_cuda_kv_write(*write(x=None, rows=0)) == 0
     read = (AT, AT, 0, S6, AT, AT, 32, S6, AT, AT, S4, AT, 1, 1, 1, 24, 1, None)
     native_refusal("kv_read", "kv_read: head dim 24", *read)
