@@ -9,9 +9,9 @@
 // A row whose top is below 2^-100 becomes zeros with scale 0 (1 / top would leave f32's range). A row with an infinity or NaN
 // gets a NaN scale over zero codes: it reads back as NaN, and no product ever meets a code that is not finite.
 //
-// Memory bounds both directions. A thread holds eight entries of a key row and of the value row beside it, of two such pairs; a
-// row's threads (d / 8 rounded up to a power of two) share its maximum by shuffles, and everything is touched once. What is read is asked for
-// before anything is computed.
+// Memory bounds both directions. A thread holds sixteen entries of a key row and of the value row beside it; a row's threads
+// (d / 16 rounded up to a power of two) share its maximum by shuffles, and everything is touched once, 16 bytes at a time. What is
+// read is asked for before anything is computed.
 #include <algorithm>
 
 #include "kv_codes.cuh"
@@ -33,21 +33,21 @@ struct KvRowArgs {
   const int64_t* starts;  // [batch]
   const int64_t* counts;  // [batch] or NULL
   int64_t batch, rows, cap;
-  int heads, units;          // units of eight entries per row
+  int heads, units;          // units of sixteen entries per row
 };
 
 template <typename T, bool WIDE>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+__device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
   if (WIDE) {
-    uint4 raw[sizeof(T) / 2];
+    uint4 raw[sizeof(T)];
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; i++) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < (int)sizeof(T); i++) raw[i] = reinterpret_cast<const uint4*>(p)[i];
     const T* e = reinterpret_cast<const T*>(raw);
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = kv_float(e[i]);
+    for (int i = 0; i < 16; i++) v[i] = kv_float(e[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = kv_float(p[i]);
+    for (int i = 0; i < 16; i++) v[i] = kv_float(p[i]);
   }
 }
 
@@ -57,45 +57,35 @@ __device__ __forceinline__ bool in_cache(const KvRowArgs& a, int64_t batch, int 
   return start > -a.cap - a.rows && start < a.cap && start + row >= 0 && start + row < a.cap && (!a.counts || row < a.counts[batch]);
 }
 
-constexpr int KV_PAIRS = 1;  // (row, head) pairs of a thread
-
 template <typename T, bool E4M3, bool WIDE, int P>
 __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const __grid_constant__ KvRowArgs a) {
   const int lane = threadIdx.x & (P - 1);
-  const unsigned pairs = (unsigned)(a.rows * a.heads), first = blockIdx.x * (KV_THREADS / P * KV_PAIRS) + threadIdx.x / P;
+  const unsigned pair = blockIdx.x * (KV_THREADS / P) + threadIdx.x / P;  // row and head; the head runs fastest
+  const int row = (int)(pair / (unsigned)a.heads), head = (int)(pair - (unsigned)row * (unsigned)a.heads);
+  const bool here = pair < (unsigned)(a.rows * a.heads) && lane < a.units;
   for (int64_t batch = blockIdx.y; batch < a.batch; batch += gridDim.y) {
-    const int64_t start = a.starts[batch];
-    float v[KV_PAIRS][2][8] = {};
-    int row[KV_PAIRS], head[KV_PAIRS];
-    bool mine[KV_PAIRS];
+    const int64_t start = a.starts[batch], at = start + row;
+    float v[2][16] = {};
 #pragma unroll
-    for (int i = 0; i < KV_PAIRS; i++) {
-      const unsigned at = first + i * (KV_THREADS / P);
-      row[i] = (int)(at / (unsigned)a.heads), head[i] = (int)(at - (unsigned)row[i] * (unsigned)a.heads);
-      mine[i] = at < pairs && lane < a.units;
+    for (int w = 0; w < 2; w++)
+      if (here)
+        load16<T, WIDE>(static_cast<const T*>(a.x[w]) + batch * a.xs[w][0] + row * a.xs[w][1] + head * a.xs[w][2] + lane * 16, v[w]);
+    const bool mine = here && in_cache(a, batch, row, start);
 #pragma unroll
-      for (int w = 0; w < 2; w++)
-        if (mine[i])
-          load8<T, WIDE>(static_cast<const T*>(a.x[w]) + batch * a.xs[w][0] + row[i] * a.xs[w][1] + head[i] * a.xs[w][2] + lane * 8, v[i][w]);
-    }
+    for (int w = 0; w < 2; w++) {
+      uint32_t top = 0;  // magnitudes compare as integers; infinities and NaN come out on top
 #pragma unroll
-    for (int i = 0; i < KV_PAIRS; i++) {
-      mine[i] = mine[i] && in_cache(a, batch, row[i], start);
+      for (int e = 0; e < 16; e++) top = max(top, __float_as_uint(v[w][e]) & 0x7fffffffu);
 #pragma unroll
-      for (int w = 0; w < 2; w++) {
-        uint32_t top = 0;  // magnitudes compare as integers; infinities and NaN come out on top
-#pragma unroll
-        for (int e = 0; e < 8; e++) top = max(top, __float_as_uint(v[i][w][e]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = P / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        float scale, inv;
-        kv_scale<E4M3>(top, &scale, &inv);
-        if (mine[i]) {
-          const int64_t at = start + row[i];
-          *reinterpret_cast<uint2*>(a.codes[w] + batch * a.cs[w][0] + head[i] * a.cs[w][1] + at * a.cs[w][2] + lane * 8) =
-              kv_encode8<E4M3>(v[i][w], inv);
-          if (lane == 0) a.scales[w][batch * a.ss[w][0] + head[i] * a.ss[w][1] + at] = scale;
-        }
+      for (int o = P / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      float scale, inv;
+      kv_scale<E4M3>(top, &scale, &inv);
+      if (mine) {
+        const uint2 lo = kv_encode8<E4M3>(reinterpret_cast<float(&)[8]>(v[w][0]), inv);
+        const uint2 hi = kv_encode8<E4M3>(reinterpret_cast<float(&)[8]>(v[w][8]), inv);
+        *reinterpret_cast<uint4*>(a.codes[w] + batch * a.cs[w][0] + head * a.cs[w][1] + at * a.cs[w][2] + lane * 16) =
+            make_uint4(lo.x, lo.y, hi.x, hi.y);
+        if (lane == 0) a.scales[w][batch * a.ss[w][0] + head * a.ss[w][1] + at] = scale;
       }
     }
   }
@@ -104,46 +94,36 @@ __global__ void __launch_bounds__(KV_THREADS) kv_write_kernel(const __grid_const
 template <typename T, bool E4M3, bool WIDE, int P>
 __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_constant__ KvRowArgs a) {
   const int lane = threadIdx.x & (P - 1);
-  const unsigned pairs = (unsigned)(a.rows * a.heads), first = blockIdx.x * (KV_THREADS / P * KV_PAIRS) + threadIdx.x / P;
-  if (lane >= a.units) return;
+  const unsigned pair = blockIdx.x * (KV_THREADS / P) + threadIdx.x / P;
+  const int row = (int)(pair / (unsigned)a.heads), head = (int)(pair - (unsigned)row * (unsigned)a.heads);
+  if (lane >= a.units || pair >= (unsigned)(a.rows * a.heads)) return;
   for (int64_t batch = blockIdx.y; batch < a.batch; batch += gridDim.y) {
-    const int64_t start = a.starts[batch];
-    uint2 raw[KV_PAIRS][2] = {};
-    float scale[KV_PAIRS][2] = {};
-    int row[KV_PAIRS], head[KV_PAIRS];
-    bool live[KV_PAIRS];
+    const int64_t start = a.starts[batch], at = start + row;
+    const bool live = in_cache(a, batch, row, start);
+    uint4 raw[2] = {};
+    float scale[2] = {};
 #pragma unroll
-    for (int i = 0; i < KV_PAIRS; i++) {
-      const unsigned at = first + i * (KV_THREADS / P);
-      row[i] = (int)(at / (unsigned)a.heads), head[i] = (int)(at - (unsigned)row[i] * (unsigned)a.heads);
-      live[i] = at < pairs && in_cache(a, batch, row[i], start);
+    for (int w = 0; w < 2; w++)
+      if (live) {
+        raw[w] = *reinterpret_cast<const uint4*>(a.codes[w] + batch * a.cs[w][0] + head * a.cs[w][1] + at * a.cs[w][2] + lane * 16);
+        scale[w] = a.scales[w][batch * a.ss[w][0] + head * a.ss[w][1] + at];
+      }
 #pragma unroll
-      for (int w = 0; w < 2; w++)
-        if (live[i]) {
-          const int64_t where = start + row[i];
-          raw[i][w] = *reinterpret_cast<const uint2*>(a.codes[w] + batch * a.cs[w][0] + head[i] * a.cs[w][1] + where * a.cs[w][2] + lane * 8);
-          scale[i][w] = a.scales[w][batch * a.ss[w][0] + head[i] * a.ss[w][1] + where];
-        }
-    }
+    for (int w = 0; w < 2; w++) {
+      float v[16];
+      kv_decode8<E4M3>(make_uint2(raw[w].x, raw[w].y), scale[w], reinterpret_cast<float(&)[8]>(v[0]));
+      kv_decode8<E4M3>(make_uint2(raw[w].z, raw[w].w), scale[w], reinterpret_cast<float(&)[8]>(v[8]));
+      T* to = static_cast<T*>(a.y[w]) + batch * a.xs[w][0] + row * a.xs[w][1] + head * a.xs[w][2] + lane * 16;
+      uint4 packed[sizeof(T)];
+      T* e = reinterpret_cast<T*>(packed);
 #pragma unroll
-    for (int i = 0; i < KV_PAIRS; i++) {
-      if (first + i * (KV_THREADS / P) >= pairs) continue;
+      for (int j = 0; j < 16; j++) kv_store(live ? v[j] : 0.f, e + j);
+      if (WIDE) {
 #pragma unroll
-      for (int w = 0; w < 2; w++) {
-        float v[8];
-        kv_decode8<E4M3>(raw[i][w], scale[i][w], v);
-        T* to = static_cast<T*>(a.y[w]) + batch * a.xs[w][0] + row[i] * a.xs[w][1] + head[i] * a.xs[w][2] + lane * 8;
-        uint4 packed[sizeof(T) / 2];
-        T* e = reinterpret_cast<T*>(packed);
+        for (int j = 0; j < (int)sizeof(T); j++) reinterpret_cast<uint4*>(to)[j] = packed[j];
+      } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) kv_store(live[i] ? v[j] : 0.f, e + j);
-        if (WIDE) {
-#pragma unroll
-          for (int j = 0; j < (int)sizeof(T) / 2; j++) reinterpret_cast<uint4*>(to)[j] = packed[j];
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; j++) to[j] = e[j];
-        }
+        for (int j = 0; j < 16; j++) to[j] = e[j];
       }
     }
   }
@@ -151,7 +131,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_read_kernel(const __grid_consta
 
 template <typename T, bool E4M3, bool WIDE, int P>
 int kv_run(const KvRowArgs& a, bool write, cudaStream_t s) {
-  const int64_t blocks = (a.rows * a.heads + KV_THREADS / P * KV_PAIRS - 1) / (KV_THREADS / P * KV_PAIRS);
+  const int64_t blocks = (a.rows * a.heads + KV_THREADS / P - 1) / (KV_THREADS / P);
   const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(a.batch, 65535));
   if (write)
     kv_write_kernel<T, E4M3, WIDE, P><<<grid, KV_THREADS, 0, s>>>(a);
@@ -164,10 +144,10 @@ int kv_run(const KvRowArgs& a, bool write, cudaStream_t s) {
 
 template <typename T, bool E4M3, bool WIDE>
 int kv_lanes(const KvRowArgs& a, bool write, cudaStream_t s) {
+  if (a.units <= 2) return kv_run<T, E4M3, WIDE, 2>(a, write, s);
   if (a.units <= 4) return kv_run<T, E4M3, WIDE, 4>(a, write, s);
   if (a.units <= 8) return kv_run<T, E4M3, WIDE, 8>(a, write, s);
-  if (a.units <= 16) return kv_run<T, E4M3, WIDE, 16>(a, write, s);
-  return kv_run<T, E4M3, WIDE, 32>(a, write, s);
+  return kv_run<T, E4M3, WIDE, 16>(a, write, s);
 }
 
 template <typename T>
@@ -186,7 +166,7 @@ int kv_type(const KvRowArgs& a, bool e4m3, bool write, cudaStream_t s) {
 
 int launch_kv_rows(const KvRows& r, bool write, cudaStream_t s) {
   KvRowArgs a{};
-  a.batch = r.batch, a.rows = r.rows, a.cap = r.cap, a.heads = (int)r.heads, a.units = (int)(r.d / 8);
+  a.batch = r.batch, a.rows = r.rows, a.cap = r.cap, a.heads = (int)r.heads, a.units = (int)(r.d / 16);
   a.starts = r.starts, a.counts = r.counts;
   if (a.batch * a.rows * a.heads == 0) return 0;
   for (int w = 0; w < 2; w++) {
