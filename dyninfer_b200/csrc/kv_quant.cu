@@ -11,7 +11,8 @@
 //
 // Memory bounds both directions. A thread holds sixteen entries of a key row and of the value row beside it; a row's threads
 // (d / 16 rounded up to a power of two) share its maximum by shuffles, and everything is touched once, 16 bytes at a time. What is
-// read is asked for before anything is computed.
+// read is asked for before anything is computed. 8 x 2048 x 8 rows of 128 bf16 entries: written 17.4 us (e4m3) and 18.9 (q8), 88 and 81 % of
+// the copy bandwidth, read 21 (73 %); with eight entries per thread 25, 28 and 24.
 #include <algorithm>
 
 #include "kv_codes.cuh"
