@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
           odd += __shfl_xor_sync(0xffffffffu, odd, 1);
           odd += __shfl_xor_sync(0xffffffffu, odd, 2);
           most = fminf(fmaxf(most, 1e-31f), 3e38f);
-          mul = odd == 0.f ? 8323072.f / most : 0.f, inv = odd == 0.f ? most / 8323072.f : __uint_as_float(0x7fc00000u);
+          mul = odd == 0.f ? 127.f * 65536.f / most : 0.f, inv = odd == 0.f ? most / (127.f * 65536.f) : __uint_as_float(0x7fc00000u);
         } else {
           // the row's largest element to 2^8 .. 2^9; zeros, infinities and extremes of f32 keep a bounded factor
           int ex = (int)((__float_as_uint(most) >> 23) & 0xff);

@@ -10,7 +10,7 @@
 //   an issuing warp per stream. Q (up to three terms) lies in tensor memory, beside S and U of the streams; an f32 query over a bf16
 //                     cache has three terms of Q and P, whose columns leave room for one stream only.
 // Scores, references, slack, terms and units are those of attention_tree.cuh. Where a result is not finite (weight 0 times
-// an infinity in a key that a row does not see), the block's rows are computed once more one by one, without tensor cores.
+// an infinity in a key that a row does not see), such rows are computed once more one by one, without tensor cores.
 // All waits are bounded; one that runs out leaves a code in the device's error word.
 // 4 x 64 rows of 32 heads at 8192 over e4m3, bf16: 70 us, 26 % of the measured bf16 rate; 8 x 13 at 2048 over q8, f32 (two terms of Q and P): 39.5.
 // A stream's tile takes 3800 (bf16) to 5000 cycles (f32): maximum 750, weights 1500, the wait for U 700 to 1000 and its fold 330 with
@@ -408,7 +408,8 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
     }
     fine = fine || row < 0 || row >= live_rows;
     __syncwarp();
-    if (__syncthreads_or(!fine) && working) {
+    __syncthreads();  // all tiles have been read
+    if (working && !fine) {
       // ---- one by one: this thread's row over this stream's keys ----
       top = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -445,7 +446,6 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
       }
     }
     __syncwarp();
-    // (all tiles have been read: the streams' last U were awaited, and what is read above is the cache itself)
     if (holds) {
       float* const to = so + (stream * W_ROWS + row) * C::PITCH;
 #pragma unroll
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
       }
     }
     cp_wait<0>();
-    __syncthreads_or(0);
+    __syncthreads();
   } else {
     // ---- issuing ----
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::FEW));
@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
         parity ^= 1u;
       }
     }
-    __syncthreads_or(0);
+    __syncthreads();
   }
   if (a.splits > 1)
     asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");

@@ -15,6 +15,8 @@
 // bandwidth; 2048 of 40 bf16 heads 10.4 us (62 %), where blocks starting and ending count.
 #include <math.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace dyn {
@@ -59,7 +61,7 @@ __device__ __forceinline__ float2 turn(float a, float b, float2 cs) {
 // threadIdx: x = unit inside the head (rotated units first, then copied ones), y = head, z = row of the block.
 // A rotated unit is N elements of either half, or N interleaved elements (N = 1: one pair of single elements).
 template <typename T, int N, bool INTER>
-__global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const __grid_constant__ RotaryArgs a,
+__global__ void __launch_bounds__(ROTARY_MAX_DIM) rotary_kernel(const __grid_constant__ RotaryArgs a,
                                                                 const __grid_constant__ RotaryTable table) {
   constexpr bool SPLIT = !INTER || N == 1;  // the pair's elements come by two accesses
   constexpr int PAIRS = SPLIT ? N : N / 2;
@@ -133,10 +135,9 @@ template <typename T, int N, bool INTER>
 int rotary_run(const RotaryArgs& a, const RotaryTable& table, cudaStream_t s) {
   const int per = INTER && N > 1 ? N / 2 : N;
   const int ux = a.pairs / per + (a.copy ? (a.d - a.rot) / N : 0);
-  int hy = ROTARY_THREADS / ux;
-  if (hy > a.heads) hy = a.heads;
-  int rz = ROTARY_THREADS / (ux * hy);
-  if (rz > 64) rz = 64;
+  // (single elements of a large head may be more units than that: never more than the head has dimensions)
+  const int hy = std::max(1, std::min(ROTARY_THREADS / ux, a.heads));
+  const int rz = std::max(1, std::min(ROTARY_THREADS / (ux * hy), 64));
   const int64_t blocks = (a.total + rz - 1) / rz;
   DYN_CHECK(blocks <= 0x7fffffff, "rotary: %lld rows are too many for one call", (long long)a.total);
   rotary_kernel<T, N, INTER><<<(unsigned)blocks, dim3(ux, hy, rz), (size_t)rz * a.pairs * sizeof(float2), s>>>(a, table);

@@ -48,7 +48,8 @@ def rotated(x, angle, rot, layout, magnitude):
 @pytest.mark.parametrize("layout", ["half", "interleaved"])
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("rows,heads,d,rot", [(1, 1, 2, 2), (5, 24, 128, 128), (7, 3, 80, 34), (33, 5, 256, 256), (300, 40, 128, 64),
-                                              (2, 1, 96, 96), (65, 2, 64, 6), (1, 700, 16, 8)])
+                                              (2, 1, 96, 96), (65, 2, 64, 6), (1, 700, 16, 8), (3, 2, 256, 34), (5, 3, 256, 2),
+                                              (2, 3, 255, 254)])
 def test_rotary(native_lib, layout, kind, rows, heads, d, rot):
     x = normal(rows + d, rows, heads, d).to(TYPES[kind])
     positions = torch.randint(0, 300000, (rows,), generator=gen(3), device="cuda")
@@ -390,6 +391,23 @@ def test_codes_that_are_not_numbers_reach_those_that_see_them(native_lib):
         nan = torch.zeros_like(want, dtype=torch.bool)
         nan[0, 1, :, 77] = True
         assert torch.equal(got.isnan(), nan) and bool(((got.double() - want).abs() <= bound)[~nan].all())
+
+
+@pytest.mark.parametrize("cache", ["bf16", "q8"])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [3, 12, 40])
+def test_queries_that_are_not_finite_spoil_their_own_rows_only(native_lib, cache, kind, rows):
+    """As a padded batch may hold them."""
+    args, k, v = make_cache(cache, 39, 2, 1, 500, 64)
+    q, mask = normal(4, 2, rows, 2, 64).to(TYPES[kind]), tree_mask(3, 2, rows)
+    clean = q.clone()
+    q[0, rows - 1], q[1, 1, 0, 5], q[1, 2, 1, 9] = math.nan, math.inf, -math.inf
+    spoilt = ~q.isfinite().all(-1)
+    n = torch.tensor([400, 333], device="cuda")
+    got = ops.tree_attention(q, args[0], args[1], n, mask, args[2], args[3])
+    want, bound = attended(torch.where(spoilt[..., None], 0.0, q.float()).to(q.dtype), k, v, [400, 333], mask, 0.125)
+    assert bool(((got.double() - want).abs() <= bound)[~spoilt].all()) and bool(got[spoilt].isnan().all())
+    assert torch.equal(got[~spoilt], ops.tree_attention(clean, args[0], args[1], n, mask, args[2], args[3])[~spoilt])
 
 
 @pytest.mark.parametrize("cache", ["q8", "e4m3"])
