@@ -2,6 +2,8 @@
 // their verification. Arguments are checked here, on the host, before any launch.
 #include <math.h>
 
+#include <atomic>
+
 #include "attention_tree.cuh"
 #include "common.cuh"
 
@@ -9,10 +11,13 @@ namespace dyn {
 namespace {
 
 int have_device() {
+  static std::atomic<bool> seen{false};  // a device that was there stays
+  if (seen.load(std::memory_order_relaxed)) return 0;
   int n = 0;
   const cudaError_t e = cudaGetDeviceCount(&n);
   DYN_CHECK(e == cudaSuccess && n > 0, "no usable CUDA device (%s); this target has no CPU fallback",
             e == cudaSuccess ? "device count is 0" : cudaGetErrorString(e));
+  seen.store(true, std::memory_order_relaxed);
   return 0;
 }
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }

@@ -184,14 +184,10 @@ def _devices(*tensors):
     return at
 
 
-def _here():
-    return _raw_device() if _raw_device is not None else torch.cuda.current_device()
-
-
 def _run(device, call, *args):
     """call(*args, stream) on a device, which may be another than the current one."""
-    if device == _here():
-        if call(*args, _stream()):
+    if _raw_device is not None and _raw_stream is not None and device == _raw_device():
+        if call(*args, _raw_stream(device)):
             check(1)
     else:
         with torch.cuda.device(device):
