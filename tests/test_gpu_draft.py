@@ -228,6 +228,18 @@ def test_cache_rows_outside_and_counts(native_lib):
     assert ops.kv_read(starts, 0, *whole)[0].shape == (6, 0, 2, 16)
 
 
+def test_cache_of_very_many_slots(native_lib):
+    slots = 70000
+    k = normal(3, slots, 1, 1, 16)
+    whole = empty_cache("q8", slots, 1, 2, 16)
+    starts = torch.arange(slots, device="cuda") % 2
+    ops.kv_write(k, -k, starts, *whole)
+    got = ops.kv_read(starts, 1, *whole)
+    step = k.abs().amax(-1, keepdim=True) / 127
+    # half a step, and the roundings of scale, factor and product: 127 (2 + 1) 2^-24 steps
+    assert bool(((got[0] - k).abs() <= 0.50003 * step).all()) and torch.equal(got[1], -got[0])
+
+
 def test_cache_views(native_lib):
     """Part of a larger cache, heads and rows in another order, entries that are not 16-byte aligned: the same bytes."""
     x = normal(4, 2 * 6 * 3 * 32 + 1)[1:].view(2, 3, 6, 32).transpose(1, 2)
@@ -299,6 +311,7 @@ ATTEND = [  # slots, rows, heads, kv heads, d, lengths, capacity
     (3, 3, 6, 2, 64, [0, 31, 32], 64), (2, 16, 4, 4, 128, [15, 16], 64), (2, 13, 32, 8, 128, [1000, 77], 1200),
     (1, 33, 5, 5, 80, [255], 300), (1, 33, 4, 2, 96, [1], 34), (2, 64, 8, 2, 128, [513, 2], 600), (1, 70, 6, 1, 48, [129], 200),
     (1, 129, 2, 1, 128, [65], 194), (5, 2, 4, 1, 112, [-1, 3, 0, -5, 40], 50), (1, 1, 40, 1, 128, [5000], 5001),
+    (1, 1, 8, 1, 128, [20000], 20001), (1, 4, 4, 1, 64, [9000], 9004), (40, 1, 16, 16, 64, list(range(0, 400, 10)), 420),
 ]
 
 
