@@ -21,6 +21,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -814,17 +815,42 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
   if (a.splits > 1) asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");  // others read this block's states
 }
 
+// Clusters of `size` blocks that the current device runs at once: a cluster stays within a part of the device whose SMs the size
+// rarely divides (a block per SM: 74 clusters of 2, 22 of 6, 15 of 7 to 9, 11 of 10, 7 of 11 to 16).
+template <auto KERNEL, int THREADS, int SMEM>
+int clusters_at_once(int size) {
+  static std::atomic<int> kept[16][17];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  std::atomic<int>* const slot = dev < 16 ? &kept[dev][size] : nullptr;
+  int n = slot ? slot->load(std::memory_order_relaxed) : 0;
+  if (n) return n;
+  const void* const kernel = reinterpret_cast<const void*>(KERNEL);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(size * 64)), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = SMEM;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)size, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    if (size > 8) return 0;  // sizes up to eight can be launched everywhere
+    n = std::max(1, sm_count() / size);
+  }
+  if (slot) slot->store(n, std::memory_order_relaxed);
+  return n;
+}
+
 template <int CT, typename TQ, int D, bool HALF>
 int run(TreeArgs a, cudaStream_t s) {
   using C = Cfg<CT, TQ, D, HALF>;
   auto kernel = tree_attention_kernel<CT, TQ, D, HALF>;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), C::SMEM)) return 1;
   const int64_t pairs = a.batch * a.kv_heads;
-  // blocks of a cluster: as many as there is room for at once, at least a tile for each warp at full capacity
-  const int64_t room = (int64_t)std::max(1, sm_count()) * std::max(1, std::min(2, (227 << 10) / (C::SMEM + 1024)));
+  // blocks of a cluster: as many as leave all clusters running at once, at least a tile for each warp at full capacity
   int splits = 16;
-  while (splits > 1 && (pairs * splits > room || a.cap < (int64_t)splits * C::WK * C::KT)) splits--;
-  if (splits > 8) DYN_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  while (splits > 1 && (a.cap < (int64_t)splits * C::WK * C::KT || pairs > clusters_at_once<tree_attention_kernel<CT, TQ, D, HALF>, C::THREADS, C::SMEM>(splits))) splits--;
   a.splits = splits;
   DYN_CHECK(pairs * splits <= 0x7fffffff, "tree_attention: too many sequences for one call");
   cudaLaunchConfig_t cfg{};

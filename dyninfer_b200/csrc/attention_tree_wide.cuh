@@ -670,9 +670,12 @@ int run_wide(TreeArgs a, cudaStream_t s) {
   DYN_CHECK(launch_regs >= C::START, "tree_attention: built with %d registers a thread", launch_regs.load());
   const int64_t pairs = a.batch * a.kv_heads;
   const int64_t row_blocks = ((int64_t)a.rows * a.group + W_ROWS - 1) / W_ROWS;
-  // blocks of a cluster: as many as fit the SMs at once (a block takes an SM), at least two tiles each at full capacity
-  int splits = 8;
-  while (splits > 1 && (pairs * row_blocks * splits > std::max(1, sm_count()) || a.cap < (int64_t)splits * W_KEYS * 2)) splits--;
+  // blocks of a cluster: as many as leave all clusters running at once (a block takes an SM), at least two tiles each at full
+  // capacity, four for more than eight blocks
+  int splits = 16;
+  while (splits > 1 && (a.cap < (int64_t)splits * W_KEYS * (splits > 8 ? 4 : 2) ||
+                        pairs * row_blocks > clusters_at_once<tree_attention_wide_kernel<CT, TQ, D>, C::THREADS, C::SMEM>(splits)))
+    splits--;
   a.splits = splits;
   DYN_CHECK(pairs * splits <= 0x7fffffff && row_blocks <= 65535, "tree_attention: too many sequences or rows for one call");
   cudaLaunchConfig_t cfg{};
