@@ -21,9 +21,9 @@
 #pragma once
 
 #include <algorithm>
-#include <atomic>
 #include <type_traits>
 
+#include "clusters.cuh"
 #include "common.cuh"
 #include "kv_codes.cuh"
 #include "ring.cuh"
@@ -813,33 +813,6 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
     }
   }
   if (a.splits > 1) asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");  // others read this block's states
-}
-
-// Clusters of `size` blocks that the current device runs at once: a cluster stays within a part of the device whose SMs the size
-// rarely divides (a block per SM: 74 clusters of 2, 22 of 6, 15 of 7 to 9, 11 of 10, 7 of 11 to 16).
-template <auto KERNEL, int THREADS, int SMEM>
-int clusters_at_once(int size) {
-  static std::atomic<int> kept[16][17];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  std::atomic<int>* const slot = dev < 16 ? &kept[dev][size] : nullptr;
-  int n = slot ? slot->load(std::memory_order_relaxed) : 0;
-  if (n) return n;
-  const void* const kernel = reinterpret_cast<const void*>(KERNEL);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(size * 64)), cfg.blockDim = dim3(THREADS), cfg.dynamicSmemBytes = SMEM;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)size, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr, cfg.numAttrs = 1;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
-    cudaGetLastError();
-    if (size > 8) return 0;  // sizes up to eight can be launched everywhere
-    n = std::max(1, sm_count() / size);
-  }
-  if (slot) slot->store(n, std::memory_order_relaxed);
-  return n;
 }
 
 template <int CT, typename TQ, int D, bool HALF>

@@ -17,6 +17,7 @@
 // whose warp had the border in its run looks through that run once more, out of the caches.
 #include <algorithm>
 
+#include "clusters.cuh"
 #include "common.cuh"
 #include "ring.cuh"
 
@@ -28,6 +29,7 @@ namespace {
 
 // blocks of 256 against 512: 32 drawn trees 29.9 and 32.9 us, 64 trees 21.8 and 21.0
 constexpr int VD_THREADS = 256, VD_WARPS = VD_THREADS / 32;
+constexpr int VD_NODE = 5 * 8 + 3 * 4;  // bytes of shared memory of a node
 
 struct VdArgs {
   const int64_t *tokens, *parents;  // [batch][nodes]
@@ -328,12 +330,17 @@ __global__ void __launch_bounds__(VD_THREADS, 4) verify_draft_kernel(const __gri
 template <typename T, bool DRAFT>
 int vd_run(VdArgs a, int64_t batch, cudaStream_t s) {
   auto kernel = verify_draft_kernel<T, DRAFT>;
-  const int smem = a.nodes * (5 * 8 + 3 * 4);
-  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem)) return 1;
-  // blocks per sequence: up to four per SM, no run of fewer than 128 entries
+  // blocks of a sequence: as many as leave all sequences running at once (up to four blocks per SM), no run of fewer than 128
+  // entries. 32 drawn chains of 5 nodes (152000 entries): 14 blocks, of which 35 clusters fit, 15.5 us; 16, of which 31 do, 21.4. 48 bf16
+  // trees of 21: 10 blocks 14.5, 8 17.8
+  constexpr int FEW = 64 * VD_NODE, MANY = 1024 * VD_NODE;
+  const int smem = a.nodes * VD_NODE;
+  if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem <= FEW ? FEW : MANY)) return 1;
   int blocks = 16;
-  while (blocks > 1 && (batch * blocks > 4 * std::max(1, sm_count()) || a.vocab < (int64_t)blocks * VD_WARPS * 128)) blocks /= 2;
-  if (blocks > 8) DYN_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  while (blocks > 1 && (a.vocab < (int64_t)blocks * VD_WARPS * 128 ||
+                        batch > (smem <= FEW ? clusters_at_once<verify_draft_kernel<T, DRAFT>, VD_THREADS, FEW>(blocks)
+                                             : clusters_at_once<verify_draft_kernel<T, DRAFT>, VD_THREADS, MANY>(blocks))))
+    blocks--;
   a.blocks = blocks;
   a.run = ((a.vocab + blocks * VD_WARPS - 1) / (blocks * VD_WARPS) + 31) / 32 * 32;
   DYN_CHECK(batch * blocks <= 0x7fffffff, "verify_draft: %lld sequences are too many for one call", (long long)batch);
