@@ -312,6 +312,9 @@ ATTEND = [  # slots, rows, heads, kv heads, d, lengths, capacity
     (1, 33, 5, 5, 80, [255], 300), (1, 33, 4, 2, 96, [1], 34), (2, 64, 8, 2, 128, [513, 2], 600), (1, 70, 6, 1, 48, [129], 200),
     (1, 129, 2, 1, 128, [65], 194), (5, 2, 4, 1, 112, [-1, 3, 0, -5, 40], 50), (1, 1, 40, 1, 128, [5000], 5001),
     (1, 1, 8, 1, 128, [20000], 20001), (1, 4, 4, 1, 64, [9000], 9004), (40, 1, 16, 16, 64, list(range(0, 400, 10)), 420),
+    # clusters of sizes that are no power of two, and of sixteen blocks for many rows
+    (1, 20, 3, 1, 64, [5000], 5020), (1, 17, 10, 10, 128, [3000], 3017), (2, 30, 30, 5, 128, [4100, 0], 4140),
+    (2, 1, 8, 8, 128, [4000, 7], 4001), (1, 3, 68, 17, 64, [3000], 3003),
 ]
 
 
@@ -540,7 +543,8 @@ def drafted(seed, slots, nodes, vocab, kind, tree, sharp=2.0):
 @pytest.mark.parametrize("tree", [False, True])
 @pytest.mark.parametrize("with_draft", [False, True])
 @pytest.mark.parametrize("slots,nodes,vocab,kind", [(1, 1, 1, "f32"), (3, 2, 2, "f32"), (40, 9, 33, "f32"), (7, 5, 1000, "bf16"), (5, 30, 4097, "f16"),
-                                                    (300, 4, 257, "f32"), (1, 5, 151936, "f32"), (20, 6, 50001, "bf16")])
+                                                    (300, 4, 257, "f32"), (1, 5, 151936, "f32"), (20, 6, 50001, "bf16"),
+                                                    (33, 4, 20001, "f32"), (45, 3, 20001, "bf16"), (63, 3, 20003, "f16")])
 def test_verify_draft(native_lib, slots, nodes, vocab, kind, with_draft, tree):
     for seed in (1, 2):
         tokens, parents, target, u, draft = drafted(seed, slots, nodes, vocab, kind, tree)
