@@ -692,9 +692,10 @@ int run_wide(TreeArgs a, cudaStream_t s) {
 
 template <int CT, typename TQ, int D>
 int by_rows(const TreeArgs& a, cudaStream_t s) {
-  // us with 8 kv heads of 128, 4 query heads each; 16 rows here / there: q8 keys with f32 queries, 1 sequence of 500 14.3 / 17.9, of 4000
-  // 18.0 / 25.4, 8 of 500 19.5 / 19.4, 8 of 4000 35.4 / 57.3; bf16 for both 12.7 / 11.9, 16.2 / 17.6, 14.3 / 12.7, 33.6 / 35.4. 20 rows in
-  // two tiles of sixteen per warp / there: 20.6 / 18.5, 40.0 / 25.8, 22.3 / 19.7, 63.8 / 57.2, and 18.9 / 12.0, 23.5 / 17.5, 21.3 / 12.6, 50.7 / 35.4
+  // us with 8 kv heads of 128, 4 query heads each; 16 rows in run / run_wide: q8 keys with f32 queries, 1 sequence of 500 13.3 / 14.7, of
+  // 4000 17.7 / 22.9, of 32000 52 / 81, 8 of 500 19.1 / 15.7, 8 of 4000 35.0 / 56.1; bf16 for both 11.9 / 10.2, 16.2 / 16.1, 50.8 / 50.4, 13.6 / 11.2,
+  // 34.1 / 34.1, which is not worth the slower way of rows that are not finite. 20 rows in two tiles of sixteen per warp were slower
+  // than run_wide everywhere (8 of 4000: 63.8 / 56.9, bf16 50.7 / 34.1)
   const int64_t rows = (int64_t)a.rows * a.group;
   if (rows <= 8) return run<CT, TQ, D, true>(a, s);
   if (rows <= 16) return run<CT, TQ, D, false>(a, s);

@@ -22,7 +22,7 @@
 #include "ring.cuh"
 
 // On the device, 151936 entries: a chain of 5 nodes 10.4 us (f32, drawn), 64 trees of 21 (bf16, not drawn) 21 us, 32 trees of 13 (f32, drawn,
-// one to four passes each) 30 us. A pass is bound by latency and by the conversions to 64 bits, which an SM does sixteen of per cycle.
+// one to four passes each) 29 us. A pass is bound by latency and by the conversions to 64 bits, which an SM does sixteen of per cycle.
 namespace dyn {
 
 namespace {
