@@ -822,8 +822,7 @@ int run(TreeArgs a, cudaStream_t s) {
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), C::SMEM)) return 1;
   const int64_t pairs = a.batch * a.kv_heads;
   // blocks of a cluster: as many as leave all clusters running at once, at least a tile for each warp at full capacity
-  int splits = 16;
-  while (splits > 1 && (a.cap < (int64_t)splits * C::WK * C::KT || pairs > clusters_at_once<tree_attention_kernel<CT, TQ, D, HALF>, C::THREADS, C::SMEM>(splits))) splits--;
+  const int splits = blocks_per_cluster<tree_attention_kernel<CT, TQ, D, HALF>, C::THREADS, C::SMEM>(pairs, a.cap / (C::WK * C::KT));
   a.splits = splits;
   DYN_CHECK(pairs * splits <= 0x7fffffff, "tree_attention: too many sequences for one call");
   cudaLaunchConfig_t cfg{};

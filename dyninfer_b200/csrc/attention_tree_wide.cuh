@@ -672,10 +672,8 @@ int run_wide(TreeArgs a, cudaStream_t s) {
   const int64_t row_blocks = ((int64_t)a.rows * a.group + W_ROWS - 1) / W_ROWS;
   // blocks of a cluster: as many as leave all clusters running at once (a block takes an SM), at least two tiles each at full
   // capacity, four for more than eight blocks
-  int splits = 16;
-  while (splits > 1 && (a.cap < (int64_t)splits * W_KEYS * (splits > 8 ? 4 : 2) ||
-                        pairs * row_blocks > clusters_at_once<tree_attention_wide_kernel<CT, TQ, D>, C::THREADS, C::SMEM>(splits)))
-    splits--;
+  const int64_t most = std::max(a.cap / (4 * W_KEYS), std::min<int64_t>(8, a.cap / (2 * W_KEYS)));
+  const int splits = blocks_per_cluster<tree_attention_wide_kernel<CT, TQ, D>, C::THREADS, C::SMEM>(pairs * row_blocks, most);
   a.splits = splits;
   DYN_CHECK(pairs * splits <= 0x7fffffff && row_blocks <= 65535, "tree_attention: too many sequences or rows for one call");
   cudaLaunchConfig_t cfg{};

@@ -336,11 +336,9 @@ int vd_run(VdArgs a, int64_t batch, cudaStream_t s) {
   constexpr int FEW = 64 * VD_NODE, MANY = 1024 * VD_NODE;
   const int smem = a.nodes * VD_NODE;
   if (ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem <= FEW ? FEW : MANY)) return 1;
-  int blocks = 16;
-  while (blocks > 1 && (a.vocab < (int64_t)blocks * VD_WARPS * 128 ||
-                        batch > (smem <= FEW ? clusters_at_once<verify_draft_kernel<T, DRAFT>, VD_THREADS, FEW>(blocks)
-                                             : clusters_at_once<verify_draft_kernel<T, DRAFT>, VD_THREADS, MANY>(blocks))))
-    blocks--;
+  const int64_t most = a.vocab / (VD_WARPS * 128);
+  const int blocks = smem <= FEW ? blocks_per_cluster<verify_draft_kernel<T, DRAFT>, VD_THREADS, FEW>(batch, most)
+                                 : blocks_per_cluster<verify_draft_kernel<T, DRAFT>, VD_THREADS, MANY>(batch, most);
   a.blocks = blocks;
   a.run = ((a.vocab + blocks * VD_WARPS - 1) / (blocks * VD_WARPS) + 31) / 32 * 32;
   DYN_CHECK(batch * blocks <= 0x7fffffff, "verify_draft: %lld sequences are too many for one call", (long long)batch);
