@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
 
   // ---- the running state ----
   float out[NT][NE], top[H], sum[H];
-  int vex = 30;  // 8-bit: exponent that the values' scales are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
+  int vex[H];  // 8-bit: exponent that the scales of the values a row sees are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
   // Values that are not finite: weight 0, or a weight's zero second term, times one is not a number. Where a result is not finite
   // the keys are gone through once more, with such entries left out of the products and added one by one. (Codes of q8 are finite.)
   constexpr bool ODD = CT != TREE_Q8;
@@ -424,8 +424,7 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
 #pragma unroll
       for (int e = 0; e < NE; e++) out[n][e] = 0.f;
 #pragma unroll
-    for (int h = 0; h < H; h++) top[h] = -INFINITY, sum[h] = 0.f;
-    vex = 30;
+    for (int h = 0; h < H; h++) top[h] = -INFINITY, sum[h] = 0.f, vex[h] = 30;
     int stage = 0;
     for (int tile = first; tile < tiles; tile += step) {
       cp_wait<C::STAGES - 2>();
@@ -500,7 +499,7 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
       // scores in powers of two, masked
       const int64_t key0 = (int64_t)tile * KT;
       float vscale[C::WIDE ? 1 : NK][2];
-      float grow = 1.f;  // 8-bit: what the units of `out` change by
+      int ex[H];  // 8-bit: exponent of the largest scale of the values that a row sees
       if (!C::WIDE) {
         float most = 0.f;
 #pragma unroll
@@ -513,11 +512,8 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
 #pragma unroll
               for (int h = 0; h < H; h++) sc[j][2 * h + e] *= kscale;
           }
-        int ex = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23);
-        ex = ex < 30 ? 30 : ex > 240 ? 240 : ex;
-        if (ex > vex) grow = ex2((float)(vex - ex)), vex = ex;
+        ex[0] = ex[H - 1] = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(most)) >> 23);
       }
-      const float pmul = C::BF ? 1.f : C::WIDE ? (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(254 + C::PEXP - vex) << 23);
       const bool tail = key0 + KT > len;
       uint32_t vis[H];
 #pragma unroll
@@ -534,10 +530,26 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
               if (key < keys && sees(a, b, tr, key - len)) bits |= 1u << i;
             }
             vis[h] = bits;
+            if (!C::WIDE) {
+              // any other scale would push the row's weights out of f16's range
+              float most = 0.f;
+#pragma unroll
+              for (int i = 0; i < 2 * NK; i++) most = fmaxf(most, bits >> i & 1 ? vscale[C::WIDE ? 0 : i >> 1][i & 1] : 0.f);
+              most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+              ex[h] = (int)(__float_as_uint(fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2))) >> 23);
+            }
           }
       }
-      float decay[H];
-      bool change = grow != 1.f;
+      float decay[H];  // what a row's `out` is multiplied with
+      bool change = false;
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+          decay[h] = 1.f;
+          if (!C::WIDE) {
+            const int e = ex[h] < 30 ? 30 : ex[h] > 240 ? 240 : ex[h];
+            if (e > vex[h]) decay[h] = ex2((float)(vex[h] - e)), vex[h] = e, change = true;
+          }
+        }
 #pragma unroll
         for (int h = 0; h < H; h++) {
           // the maximum in powers of two; a score and its reference go through one fma, so that the score is not rounded before
@@ -552,7 +564,6 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
             }
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
           best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-          decay[h] = grow;
           if (best > top[h] + C::SLACK || top[h] == -INFINITY) {
             if (best > -INFINITY) decay[h] *= ex2(top[h] - best), change = true;
             sum[h] *= ex2(top[h] - (best == -INFINITY ? 0.f : best));
@@ -584,6 +595,7 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
           float w[NE];
 #pragma unroll
           for (int e = 0; e < NE; e++) {
+            const float pmul = C::BF ? 1.f : C::WIDE ? (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(254 + C::PEXP - vex[e >> 1]) << 23);
             w[e] = sc[j][e] * pmul;
             if (!C::WIDE) {
               w[e] *= vscale[C::WIDE ? 0 : j][e & 1];
@@ -719,11 +731,13 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
     begin();
   }
   // out in its own units again
-  const float unit = C::BF ? 1.f : C::WIDE ? 1.f / (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(vex - C::PEXP) << 23);
+  float unit[H];
+#pragma unroll
+    for (int h = 0; h < H; h++) unit[h] = C::BF ? 1.f : C::WIDE ? 1.f / (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(vex[h] - C::PEXP) << 23);
 #pragma unroll
     for (int n = 0; n < NT; n++)
 #pragma unroll
-      for (int e = 0; e < NE; e++) out[n][e] *= unit;
+      for (int e = 0; e < NE; e++) out[n][e] *= unit[e >> 1];
 #pragma unroll
     for (int h = 0; h < H; h++) {
       sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);

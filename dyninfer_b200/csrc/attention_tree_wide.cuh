@@ -46,6 +46,9 @@ struct Wide {
   // which 2^-9 does not see before some ten thousand tiles; rows whose reference moves are rescaled there. With f16 operands (one
   // term of P) there is room for P beside S, and the next tile's S is made under the present one's exponentials.
   static constexpr bool STAYS = QB, BESIDE = STAYS && PT == 1;
+  // tiles with keys that not every row sees in a loop of their own: 4 x 64 rows at 8192 over e4m3 68.9 us, in one loop 72.0. Results that are
+  // folded have more code, of which two copies cost short contexts more (2 x 8 at 500 over q8, f32: 20.4, in one loop 19.2)
+  static constexpr bool APART = STAYS && !WIDE;
   // tensor memory columns
   static constexpr int S_COLS = PT == 3 ? 96 : 64, P_COL = BESIDE ? 64 : 0, U_AT = BESIDE ? 96 : S_COLS;  // a stream: S, P, U
   static constexpr int STREAM = U_AT + D_, Q_COL = NS * STREAM;
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
     }
     // ---- softmax ----
     float out[D], top = -INFINITY, sum = 0.f, mult = 0.f;
-    int vex = 30;  // 8-bit: exponent that value scales are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
+    int vex = 30;  // 8-bit: exponent that the scales of the values that the row sees are taken relative to; `out` is in units of 2^(vex - 127 - PEXP)
 #pragma unroll
     for (int d = 0; d < D; d++) out[d] = 0.f;
     if (working) {
@@ -230,14 +233,25 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
     };
     int buf = stream;
     unsigned phase = 0, parity = 0;
-#pragma unroll 1
-    for (int i = stream; i < mine && working; i += C::NS) {
-      const int64_t key0 = ((int64_t)split + (int64_t)i * a.splits) * W_KEYS;
-      const bool tail = key0 + W_KEYS > len;  // a tile with keys that not every row sees
+    // tile i; `tail`: with keys that not every row sees
+    auto take = [&](int i, int64_t key0, auto tail) {
       uint32_t vis[2] = {0xffffffffu, 0xffffffffu};
+      // 8-bit: exponent of the largest scale of the values that the row sees. A scale that it does not see would push its weights out of f16's range
+      int seen_ex = 30;
       if (tail) {
 #pragma unroll
         for (int h = 0; h < 2; h++) vis[h] = seen_of<32>(a, b, tr, key0 + 32 * h, keys, len);
+        if (!C::WIDE) {
+          wait(kv_full + buf, phase, 2);
+          float most = 0.f;
+#pragma unroll(C::APART ? W_KEYS / 4 : 2)
+          for (int e = 0; e < W_KEYS; e += 4) {
+            const float4 v4 = *reinterpret_cast<const float4*>(&vscale[C::WIDE ? 0 : buf][e]);
+            const uint32_t of4 = (e < 32 ? vis[0] : vis[1]) >> (e & 31);
+            most = fmaxf(fmaxf(most, of4 & 1 ? v4.x : 0.f), fmaxf(of4 & 2 ? v4.y : 0.f, fmaxf(of4 & 4 ? v4.z : 0.f, of4 & 8 ? v4.w : 0.f)));
+          }
+          seen_ex = min(max((int)(__float_as_uint(most) >> 23), 30), 240);
+        }
       }
       if (!C::WIDE) wait(kv_full + buf, phase, 2);  // for the scales
       wait(s_full + stream, parity, 1);
@@ -245,7 +259,8 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
       tc_fence_after();
       float decay = 1.f;
       if (!C::WIDE) {
-        const int ex = max(vexp[buf][2], vexp[buf][3]);
+        int ex = max(vexp[buf][2], vexp[buf][3]);
+        if (tail) ex = seen_ex;
         if (ex > vex) decay = ex2((float)(vex - ex)), vex = ex;
       }
       const float pmul = C::BF ? 1.f : C::WIDE ? (float)(1 << C::PEXP) : __uint_as_float((uint32_t)(254 + C::PEXP - vex) << 23);
@@ -392,6 +407,17 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
       parity ^= 1u;
       buf += C::NS;
       if (buf >= C::TILES) buf -= C::TILES, phase ^= 1u;
+    };
+    int i = stream;
+    auto first_key = [&] { return ((int64_t)split + (int64_t)i * a.splits) * W_KEYS; };
+    if constexpr (C::APART) {
+#pragma unroll 1
+      for (; i < mine && working && first_key() + W_KEYS <= len; i += C::NS) take(i, first_key(), std::false_type{});
+#pragma unroll 1
+      for (; i < mine && working; i += C::NS) take(i, first_key(), std::true_type{});
+    } else {
+#pragma unroll 1
+      for (; i < mine && working; i += C::NS) take(i, first_key(), first_key() + W_KEYS > len);
     }
     if (C::STAYS && working && stream < mine) {
       wait(u_full + stream, parity ^ 1u, 3);

@@ -1,0 +1,65 @@
+"""The operators of speculative decoding at the ends of their ranges. Bounds as in `test_gpu_draft`, with absolute parts that
+count only the keys that a row sees.
+"""
+import math
+
+import pytest
+import torch
+
+from dyninfer_b200 import ops
+from test_gpu_draft import TYPES, half, make_cache, normal
+
+pytestmark = pytest.mark.gpu
+
+
+def attended_by_row(q, k, v, n, mask, scale):
+    """(result, bound) of q [rows, heads, d] over one sequence's k and v [kv heads, keys, d] in 64 bits."""
+    rows, heads, d = q.shape
+    group = heads // k.shape[0]
+    seen = torch.cat([torch.ones(rows, n, dtype=torch.bool, device="cuda"), mask], 1)
+    out, bound = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    for h in range(heads):
+        keys, values = k[h // group, :n + rows], torch.where(seen[..., None], v[h // group, :n + rows], 0.0)     # [row, key, d]
+        products = torch.where(seen[..., None], q[:, h].double()[:, None] * keys * scale, 0.0)
+        scores = products.sum(-1).masked_fill(~seen, -math.inf)
+        top = scores.amax(-1, keepdim=True)
+        w = torch.exp(scores - torch.where(top == -math.inf, 0.0, top)).masked_fill(~seen, 0)
+        w = w / w.sum(-1, keepdim=True).clamp(min=1e-300)
+        out[:, h] = torch.where(w[..., None] > 0, w[..., None] * values, 0.0).sum(1)
+        # a score: up to 24 accumulations, the query's terms and three f32 operations, relative to the sum of magnitudes; a weight:
+        # twice that, the exponential, and its rounding as an operand: one f16 term for bf16 queries (two for the others)
+        size = torch.where(products.isfinite(), products.abs(), 0.0).sum(-1).amax(-1, keepdim=True)
+        weight = 2 * (24 * 2.0 ** -23 + 2.0 ** -20) * size + 2.0 ** -18 + (2.0 ** -11 if q.dtype == torch.bfloat16 else 0)
+        # a weight's last f16 term is off by up to 2^-25, in units of 2^-13 (f32 queries) or 2^-5 of the largest value scale that
+        # the row sees
+        steps = (n + rows) * 2.0 ** (-38 if q.dtype == torch.float32 else -30) * values.abs().amax((1, 2))[:, None]
+        bound[:, h] = weight * torch.where(w[..., None] > 0, w[..., None] * values.abs(), 0.0).sum(1) + steps
+    return out, bound + half(q.dtype) * (out.abs() + bound)
+
+
+@pytest.mark.parametrize("cache", ["q8", "e4m3"])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,n", [(4, 50), (8, 50), (20, 50), (4, 500), (8, 500), (64, 500), (20, 0)])
+def test_value_scales_of_keys_that_are_not_seen(native_lib, cache, kind, rows, n):
+    """Two query heads share a kv head: up to 8 rows, up to 16, and more. A node that nobody sees, and one that a single row does."""
+    args, k, v = make_cache(cache, 43, 1, 2, n + rows + 3, 128)
+    q = normal(8, 1, rows, 4, 128).to(TYPES[kind])
+    mask = torch.rand(rows, rows, device="cuda", generator=torch.Generator("cuda").manual_seed(rows)) < 0.5
+    hidden, alone, seer = rows // 2, rows - 1, 1
+    mask[:, hidden] = mask[:, alone] = False
+    mask[seer, alone] = True
+    codes = args[1].float().double()
+    length = torch.tensor([n], device="cuda")
+    clean = None
+    for size in (1.0, 2.0 ** 25, 2.0 ** 40, 1e10, 1e30, math.inf):
+        args[3][0, :, n + hidden] = size
+        args[3][0, :, n + alone] = min(size, 1e10)
+        got = ops.tree_attention(q, args[0], args[1], length, mask, args[2], args[3])[0]
+        v = codes * args[3][..., None].double()
+        want, bound = attended_by_row(q[0], k[0], v[0], n, mask, 128 ** -0.5)
+        near = ((got.double() - want).abs() <= bound) | (got == want.to(got.dtype))       # the latter: infinity beyond f16's range
+        assert bool(near.all()), (size, float((got.double() - want)[~near].abs().max()))
+        # and those that see neither are what they are beside a small scale
+        rest = torch.arange(rows, device="cuda") != seer
+        clean = got if clean is None else clean
+        assert torch.equal(got[rest], clean[rest]), size
