@@ -160,7 +160,7 @@ unsafe extern "C" {
     // ---- speculative decoding (strides are host arrays that count elements)
     pub fn dyninfer_cuda_rotary(
         x_dev: *const c_void,
-        type: c_int,
+        value_type: c_int,
         x_strides: *const i64,
         positions_dev: *const i64,
         frequencies: *const f64,
@@ -178,7 +178,7 @@ unsafe extern "C" {
     pub fn dyninfer_cuda_kv_write(
         k_dev: *const c_void,
         v_dev: *const c_void,
-        type: c_int,
+        value_type: c_int,
         x_strides: *const i64,
         k_cache_dev: *mut c_void,
         v_cache_dev: *mut c_void,
@@ -199,7 +199,7 @@ unsafe extern "C" {
     pub fn dyninfer_cuda_kv_read(
         k_dev: *mut c_void,
         v_dev: *mut c_void,
-        type: c_int,
+        value_type: c_int,
         x_strides: *const i64,
         k_cache_dev: *const c_void,
         v_cache_dev: *const c_void,
@@ -248,7 +248,7 @@ unsafe extern "C" {
         target_strides: *const i64,
         draft_dev: *const c_void,
         draft_strides: *const i64,
-        type: c_int,
+        value_type: c_int,
         uniforms_dev: *const f32,
         batch: i64,
         nodes: i64,

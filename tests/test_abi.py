@@ -89,6 +89,19 @@ def test_rust_ffi_crate_follows_the_header():
     assert consts == _header_enums()
 
 
+def test_rust_names_are_not_keywords():
+    """Nothing compiles the crates here: a parameter, field or function named by a keyword would go unnoticed."""
+    keywords = set("""as async await break const continue crate dyn else enum extern false fn for if impl in let loop match mod move
+        mut pub ref return self Self static struct super trait true type unsafe use where while abstract become box do final gen
+        macro override priv try typeof unsized virtual yield""".split())
+    for crate in ("dyninfer-cuda-sys", "dyninfer-cuda"):
+        src = os.path.join(ROOT, "crates", crate, "src")
+        for name in os.listdir(src):
+            rs = re.sub(r'//[^\n]*|"(?:[^"\\]|\\.)*"', "", open(os.path.join(src, name)).read())
+            names = re.findall(r"[(,{]\s*(?:pub\s+)?(\w+)\s*:(?!:)", rs) + re.findall(r"\b(?:fn|struct|const|static|enum|mod)\s+(\w+)", rs)
+            assert names and not keywords & set(names), (crate, name, keywords & set(names))
+
+
 def test_python_encoding_ids_follow_the_header():
     enums = _header_enums()
     names = {"plain.f32": "F32", "plain.f16": "F16", "plain.bf16": "BF16", "gguf.q4_0": "Q4_0",
