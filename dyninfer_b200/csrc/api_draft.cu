@@ -148,7 +148,8 @@ int dyninfer_cuda_tree_attention(const void* q_dev, int q_type, const int64_t* q
   bool even = aligned(k_cache_dev, 16) && aligned(v_cache_dev, 16) && aligned(ctx_dev, 16);
   for (int64_t step : cache_steps.v) even = even && step * size % 16 == 0;
   DYN_CHECK(even, "tree_attention: caches, their strides and the output must be multiples of 16 bytes");
-  if (have_device()) return 1;
+  // the word that waits report to is allocated here, so that no row count does it first inside a capture
+  if (have_device() || !device_error_word()) return 1;
   TreeArgs a{};
   a.q = q_dev, a.out = ctx_dev, a.k = static_cast<const uint8_t*>(k_cache_dev), a.v = static_cast<const uint8_t*>(v_cache_dev);
   a.lengths = lengths_dev, a.mask = mask_dev;

@@ -2,6 +2,10 @@
 count only the keys that a row sees.
 """
 import math
+import os
+import subprocess
+import sys
+import textwrap
 
 import pytest
 import torch
@@ -10,6 +14,7 @@ from dyninfer_b200 import ops
 from test_gpu_draft import TYPES, half, make_cache, normal
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def attended_by_row(q, k, v, n, mask, scale):
@@ -63,3 +68,27 @@ def test_value_scales_of_keys_that_are_not_seen(native_lib, cache, kind, rows, n
         rest = torch.arange(rows, device="cuda") != seer
         clean = got if clean is None else clean
         assert torch.equal(got[rest], clean[rest]), size
+
+
+def test_a_form_is_captured_that_was_not_called_before(native_lib):
+    """One call of the operator has been made, with few rows; the captured one has many. In a process of its own, where no
+    other operator has set anything up."""
+    text = textwrap.dedent("""
+        import torch
+        from dyninfer_b200 import ops
+        q = torch.randn(1, 40, 4, 64, device="cuda")
+        k, v = (torch.randn(1, 2, 400, 64, device="cuda").bfloat16() for _ in range(2))
+        n = torch.tensor([300], device="cuda")
+        ops.tree_attention(q[:, :2].contiguous(), k, v, n)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.tree_attention(q, k, v, n)
+        graph.replay()
+        want = ops.tree_attention(q, k, v, n)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        print("same")
+    """)
+    done = subprocess.run([sys.executable, "-c", text], capture_output=True, text=True, timeout=300, cwd=ROOT)
+    assert done.returncode == 0 and done.stdout.split() == ["same"], done.stderr[-2000:]
