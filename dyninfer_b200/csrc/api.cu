@@ -151,7 +151,7 @@ int check_device_error(const char* what) {
   }
   if (!code) return 0;
   set_error("%s: a bounded wait inside a kernel expired (code %d: 1 single-row product weight ring, "
-            "2 tensor-core GEMM pipeline); the results of the call are invalid", what, code);
+            "2 tensor-core GEMM pipeline, 3 tensor-core attention pipeline); the results of the call are invalid", what, code);
   return 1;
 }
 

@@ -670,7 +670,7 @@ attention_prefill_kernel(const FaArgs a, const __grid_constant__ CUtensorMap qma
   }
   tc_fence_after();
   if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-  if (tid == 0 && s_abort) report_wait_expired(a.error, DEV_ERR_GEMM_PIPE);
+  if (tid == 0 && s_abort) report_wait_expired(a.error, DEV_ERR_ATTENTION_PIPE);
 }
 
 template <int KV, int NS>

@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
     asm volatile("barrier.cluster.arrive;\n\tbarrier.cluster.wait;" ::: "memory");  // others read this block's states
   tc_fence_after();
   if (warp == ISSUING) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-  if (tid == 0 && s_abort) report_wait_expired(error, DEV_ERR_GEMM_PIPE);
+  if (tid == 0 && s_abort) report_wait_expired(error, DEV_ERR_ATTENTION_PIPE);
 }
 
 template <int CT, typename TQ, int D>

@@ -117,7 +117,7 @@ int ensure_dynamic_smem(const void* kernel, int bytes);
 // make it before any launch or stream capture.
 int* device_error_word();
 int check_device_error(const char* what);  // 1 (message set, word cleared) when a wait expired
-enum { DEV_ERR_GEMV_RING = 1, DEV_ERR_GEMM_PIPE = 2 };
+enum { DEV_ERR_GEMV_RING = 1, DEV_ERR_GEMM_PIPE = 2, DEV_ERR_ATTENTION_PIPE = 3 };
 __device__ __forceinline__ void report_wait_expired(int* word, int code) {
   if (word) {
     *reinterpret_cast<volatile int*>(word) = code;

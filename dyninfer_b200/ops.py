@@ -483,6 +483,6 @@ def verify_draft(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tens
 
 
 def check_device_error():
-    """Call after synchronising: raises when a kernel's bounded wait (weight ring, GEMM pipeline)
+    """Call after synchronising: raises when a kernel's bounded wait (weight ring, GEMM or attention pipeline)
     expired since the last check, in which case the results produced since then are invalid."""
     check(lib().dyninfer_cuda_check_device_error())

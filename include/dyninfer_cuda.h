@@ -79,7 +79,7 @@ int dyninfer_cuda_device_count(int* out_count);
 uint64_t dyninfer_cuda_row_bytes(int encoding, int64_t cols);
 
 /* The operator entry points below are asynchronous on the caller's stream, so a kernel whose
- * bounded wait (weight ring, GEMM pipeline) gives up cannot fail the call that launched it: it
+ * bounded wait (weight ring, GEMM or attention pipeline) gives up cannot fail the call that launched it: it
  * leaves a code in a per-device error word instead. Call this after synchronising the stream:
  * non-zero (message via last_error, word cleared) means results since the last check are
  * invalid. Session calls check it themselves before they return. Error convention as

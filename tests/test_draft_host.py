@@ -1,11 +1,15 @@
 """Host side of the operators of speculative decoding: refusals, which answer before any device is touched, and frequencies."""
 import ctypes as C
 import math
+import os
+import re
 
 import pytest
 import torch
 
 from dyninfer_b200 import _lib, ops
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 def refused(kind, text, call, *args, **kwargs):
@@ -197,3 +201,15 @@ def test_frequencies_and_their_scalings():
                                        ((8, 1e4, "yarn", 2.0, 4096, 5.0, 2.0), "below high")])
 def test_frequency_refusals(args, text):
     refused(ValueError, text, ops.rotary_frequencies, *args)
+
+
+def test_waits_that_run_out_are_reported_under_their_own_name():
+    """Each file's bounded waits leave its own code in the device's error word, and the message names every code."""
+    csrc = os.path.join(ROOT, "dyninfer_b200", "csrc")
+    text = {f: open(os.path.join(csrc, f)).read() for f in os.listdir(csrc)}
+    codes = dict(re.findall(r"(DEV_ERR_\w+) = (\d+)", text["common.cuh"]))
+    message = re.search(r"a bounded wait inside a kernel expired.*?\)", re.sub(r'"\s*"', "", text["api.cu"]))[0]
+    assert len(codes) >= 3 and all(re.search(rf"\b{c} \w", message) for c in codes.values())
+    for name, source in text.items():
+        kind = "ATTENTION_PIPE" if name.startswith("attention") else "GEM"
+        assert all(kind in c for c in re.findall(r"report_wait_expired\([^,()]+, (DEV_ERR_\w+)\)", source)), name
