@@ -5,9 +5,10 @@
 //   a' = m (a cos - b sin),  b' = m (b cos + a sin);  elements from r on are copied.
 //
 // Angles. f32 loses them far out (position 200000 at f = 1: 0.008 rad). An angle matters modulo one turn only, so the host
-// turns f / 2 pi into a 64-bit fixed-point fraction of a turn; position * fraction in wrapping 64-bit integers is the exact
-// product modulo one turn (off by position * 2^-65 turns for the fraction's rounding), one integer multiplication and one
-// rounding to f32. Signed, in half turns, it is sincospif's argument.
+// turns f / 2 pi into a 64-bit fixed-point fraction of a turn, rounded; position * fraction in wrapping 64-bit integers is their
+// exact product modulo one turn, one integer multiplication and one rounding to f32. What is off is the fraction: by 2^-65 for its
+// rounding, and by f 2^-65 for the two roundings of f / 2 pi to 64 bits, so an angle by at most position * (1 + f) 2^-65 turns.
+// That is below f32's own rounding of it up to positions of 2^39. Signed, in half turns, it is sincospif's argument.
 //
 // What bounds it is memory: every element comes and goes once. A block takes one row or a few; its threads compute the row's
 // cosines and sines once, into shared memory, while the first head's elements are on their way, and then stay with their
@@ -173,7 +174,8 @@ int launch_rotary(const void* x, int type, int64_t batch, int64_t rows, int64_t 
     long double turns = (long double)frequencies[i] * 0.15915494309189533576888376337251436L;  // one over 2 pi
     turns -= fabsl(turns) < 4e18L ? (long double)(int64_t)turns : floorl(turns);
     if (turns < 0) turns += 1;
-    table.turn[i] = turns < 1.0L ? (uint64_t)(turns * 18446744073709551616.0L) : 0;
+    const long double fraction = rintl(turns * 18446744073709551616.0L);
+    table.turn[i] = fraction < 18446744073709551616.0L ? (uint64_t)fraction : 0;  // a whole turn is none
   }
   RotaryArgs a{};
   a.x = x, a.y = y, a.positions = positions, a.rows = rows, a.total = batch * rows;

@@ -218,8 +218,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     """Rotary positions of x [..., heads, d] (f32, f16 or bf16, up to two leading dimensions, any strides with a dense last
     dimension): pair i of the first 2 * len(frequencies) dimensions turns by positions[...] * frequencies[i] and is multiplied by
     `magnitude`; the other dimensions are copied. `layout` is "half" (pairs i, i + r/2) or "interleaved" (2i, 2i + 1).
-    `frequencies` is a float64 tensor in host memory (`rotary_frequencies` makes one); angles are exact modulo a turn at any
-    position. `out` may be x itself: a view of the leading heads of fused [q | k | v] rows turns q and k where they lie."""
+    `frequencies` is a float64 tensor in host memory (`rotary_frequencies` makes one); angles are taken modulo a turn in 64-bit
+    fixed point, off by at most 2^-65 * position * (1 + frequency) turns. `out` may be x itself: a view of the leading heads of fused [q | k | v] rows turns q and k where they lie."""
     kind, shape, sx = _WT.get(x.dtype), x.shape, x.stride()
     if kind is None:
         raise TypeError(f"x must be float32, float16 or bfloat16, not {x.dtype}")

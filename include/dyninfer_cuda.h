@@ -166,8 +166,9 @@ enum {
  * rotary_dim dimensions -- (i, i + rotary_dim / 2), or (2i, 2i + 1) when `interleaved` -- turns by
  * positions[batch, row] * frequencies[i] and is multiplied by `magnitude`; other dimensions are
  * copied. `frequencies` (rotary_dim / 2 values) lies in host memory and is read before the call
- * returns; angles are exact modulo a turn for any 64-bit position. y may be x itself with the same
- * strides, but must not overlap it otherwise. d <= 256. */
+ * returns; angles are taken modulo a turn in 64-bit fixed point, off by at most 2^-65 * position *
+ * (1 + frequency) turns. y may be x itself with the same strides, but must not overlap it otherwise.
+ * d <= 256. */
 int dyninfer_cuda_rotary(const void* x_dev, int type, const int64_t* x_strides, const int64_t* positions_dev,
                          const double* frequencies, int64_t rotary_dim, int interleaved, double magnitude,
                          int64_t batch, int64_t rows, int64_t heads, int64_t d, void* y_dev,

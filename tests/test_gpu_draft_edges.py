@@ -6,6 +6,7 @@ import os
 import subprocess
 import sys
 import textwrap
+from fractions import Fraction
 
 import pytest
 import torch
@@ -92,3 +93,18 @@ def test_a_form_is_captured_that_was_not_called_before(native_lib):
     """)
     done = subprocess.run([sys.executable, "-c", text], capture_output=True, text=True, timeout=300, cwd=ROOT)
     assert done.returncode == 0 and done.stdout.split() == ["same"], done.stderr[-2000:]
+
+
+def test_rotary_fractions_are_rounded(native_lib):
+    """At 2^60 a fraction of a turn that is off by 2^-65 moves the angle by 2^-5 turns, one off by 2^-64 by 2^-4."""
+    f, _ = ops.rotary_frequencies(128, 1e4)
+    pi = Fraction(3141592653589793238462643383279502884197169399, 10 ** 45)
+    position = 2 ** 60
+    want = [float((Fraction(position) * Fraction(float(w)) / (2 * pi)) % 1) for w in f]
+    x = torch.cat([torch.ones(1, 1, 64, device="cuda"), torch.zeros(1, 1, 64, device="cuda")], -1)
+    got = ops.rotary(x, torch.tensor([position], device="cuda"), f)[0, 0].double().cpu()
+    turns = torch.atan2(got[64:], got[:64]) / (2 * math.pi)
+    off = (turns - torch.tensor(want, dtype=torch.float64)).remainder(1)
+    # the fraction's rounding to 2^-64; one over 2 pi, and the product with it, both below a quarter, rounded to 64 bits: 2^-67 each.
+    # Then cosine and sine in f32, 2^-22 radians at most
+    assert float(torch.minimum(off, 1 - off).max()) <= position * (2.0 ** -65 + 2 * 2.0 ** -67) + 2.0 ** -22
