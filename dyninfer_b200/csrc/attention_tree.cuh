@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
         for (int h = 0; h < H; h++) {
           decay[h] = 1.f;
           if (!C::WIDE) {
-            const int e = ex[h] < 30 ? 30 : ex[h] > 240 ? 240 : ex[h];
+            const int e = min(max(ex[h], 30), 254);
             if (e > vex[h]) decay[h] = ex2((float)(vex[h] - e)), vex[h] = e, change = true;
           }
         }

@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
             const uint32_t of4 = (e < 32 ? vis[0] : vis[1]) >> (e & 31);
             most = fmaxf(fmaxf(most, of4 & 1 ? v4.x : 0.f), fmaxf(of4 & 2 ? v4.y : 0.f, fmaxf(of4 & 4 ? v4.z : 0.f, of4 & 8 ? v4.w : 0.f)));
           }
-          seen_ex = min(max((int)(__float_as_uint(most) >> 23), 30), 240);
+          seen_ex = min(max((int)(__float_as_uint(most) >> 23), 30), 254);
         }
       }
       if (!C::WIDE) wait(kv_full + buf, phase, 2);  // for the scales
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
         if (ft < W_KEYS) kscale[C::WIDE ? 0 : to][ft] = scale;
         else vscale[C::WIDE ? 0 : to][ft - W_KEYS] = scale;
         int ex = (int)(__reduce_max_sync(0xffffffffu, scale > 0.f ? __float_as_uint(scale) : 0u) >> 23);  // NaN compares false
-        ex = ex < 30 ? 30 : ex > 240 ? 240 : ex;
+        ex = min(max(ex, 30), 254);
         if (lane == 0) vexp[to][fw] = fw < 2 ? 30 : ex;
       }
       fence_async_smem();

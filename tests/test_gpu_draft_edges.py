@@ -108,3 +108,17 @@ def test_rotary_fractions_are_rounded(native_lib):
     # the fraction's rounding to 2^-64; one over 2 pi, and the product with it, both below a quarter, rounded to 64 bits: 2^-67 each.
     # Then cosine and sine in f32, 2^-22 radians at most
     assert float(torch.minimum(off, 1 - off).max()) <= position * (2.0 ** -65 + 2 * 2.0 ** -67) + 2.0 ** -22
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [2, 8, 20])
+@pytest.mark.parametrize("cache", ["q8", "e4m3"])
+def test_value_scales_near_the_end_of_f32(native_lib, cache, kind, rows):
+    """Values up to 2^126; a row sees four keys, so that their sum is a number as well."""
+    args, k, v = make_cache(cache, 44, 1, 1, 3 + rows, 64)
+    args[3].mul_(2.0 ** 124)
+    v = v * 2.0 ** 124
+    q, mask = normal(9, 1, rows, 2, 64).to(TYPES[kind]), torch.eye(rows, dtype=torch.bool, device="cuda")
+    got = ops.tree_attention(q, args[0], args[1], torch.tensor([3], device="cuda"), mask, args[2], args[3])[0]
+    want, bound = attended_by_row(q[0], k[0], v[0], 3, mask, 0.125)
+    assert bool(((got.double() - want).abs() <= bound).all())
