@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
           // the largest element to 127 * 2^16: three signed bytes. A row that is not finite gets scores that are not numbers
           odd += __shfl_xor_sync(0xffffffffu, odd, 1);
           odd += __shfl_xor_sync(0xffffffffu, odd, 2);
-          most = fminf(fmaxf(most, 1e-31f), 3e38f);
+          most = fminf(fmaxf(most, 1e-31f), 3.402823466e38f);  // (f32's largest)
           mul = odd == 0.f ? 127.f * 65536.f / most : 0.f, inv = odd == 0.f ? most / (127.f * 65536.f) : __uint_as_float(0x7fc00000u);
         } else {
           // the row's largest element to 2^8 .. 2^9; zeros, infinities and extremes of f32 keep a bounded factor

@@ -122,3 +122,15 @@ def test_value_scales_near_the_end_of_f32(native_lib, cache, kind, rows):
     got = ops.tree_attention(q, args[0], args[1], torch.tensor([3], device="cuda"), mask, args[2], args[3])[0]
     want, bound = attended_by_row(q[0], k[0], v[0], 3, mask, 0.125)
     assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("rows", [2, 8, 20])
+def test_queries_near_the_end_of_f32(native_lib, rows):
+    args, k, v = make_cache("q8", 45, 1, 1, 60 + rows, 128)
+    args[2].mul_(2.0 ** -110)
+    q, mask = normal(9, 1, rows, 2, 128), torch.eye(rows, dtype=torch.bool, device="cuda")
+    q *= 3.39e38 / q.abs().amax(-1, keepdim=True)
+    k, scale = k * 2.0 ** -110, 2.0 ** -17
+    got = ops.tree_attention(q, args[0], args[1], torch.tensor([60], device="cuda"), mask, args[2], args[3], scale=scale)[0]
+    want, bound = attended_by_row(q[0], k[0], v[0], 60, mask, scale)
+    assert bool(((got.double() - want).abs() <= bound).all())
