@@ -229,6 +229,16 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int64_t b, int row, int6
   return a.mask ? a.mask[b * a.ms[0] + row * a.ms[1] + j] != 0 : j <= row;
 }
 
+// What a row's output is multiplied with, from the sum of its weights. Without weights it is zero where the row sees no key, and not a
+// number where all its scores are minus infinity.
+__device__ __forceinline__ float over_sum(const TreeArgs& a, int64_t b, int row, int64_t len, int64_t keys, float sum) {
+  if (sum != 0.f) return 1.f / sum;
+  bool some = len > 0;
+#pragma unroll 1
+  for (int64_t j = 0; j < keys && !some; j++) some = sees(a, b, row, j);  // (there are no keys in front of the tree)
+  return some ? __uint_as_float(0x7fc00000u) : 0.f;
+}
+
 // Bit e: whether a row sees key key0 + e, of N <= 32. Sixteen bytes of the mask are asked for at once.
 template <int N>
 __device__ __forceinline__ uint32_t seen_of(const TreeArgs& a, int64_t b, int row, int64_t key0, int64_t keys, int64_t len) {
@@ -820,7 +830,7 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
     }
     const int tr = r / a.group, gh = r - tr * a.group;
     TQ* to = static_cast<TQ*>(a.out) + ((b * a.rows + tr) * a.heads + (int64_t)kvh * a.group + gh) * a.d + c;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = over_sum(a, b, tr, len, keys, l);
     if (c < a.d) {
 #pragma unroll
       for (int e = 0; e < 4; e++) kv_store(o[e] * inv, to + e);

@@ -198,7 +198,7 @@ int dyninfer_cuda_kv_read(void* k_dev, void* v_dev, int type, const int64_t* x_s
  * entry b sees keys 0 .. lengths[b] - 1, and key lengths[b] + j (the tree's row j) where
  * mask[b, r, j] is not zero (strides: batch, row; a batch stride of 0 shares one mask); mask NULL:
  * where j <= r. Keys from kv_cap on do not exist; a row that sees nothing gets zeros, and so do all
- * rows of an entry whose length is below zero. ctx [batch, rows, heads, d] is dense, of q's type.
+ * rows of an entry whose length is below zero (one whose scores are all minus infinity: NaN). ctx [batch, rows, heads, d] is dense, of q's type.
  * kv_type F16, BF16, or an 8-bit type with its scales (as kv_write lays them out). scale is above
  * zero. d is a multiple of 16 up to 128. */
 int dyninfer_cuda_tree_attention(const void* q_dev, int q_type, const int64_t* q_strides, const void* k_cache_dev,

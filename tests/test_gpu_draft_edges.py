@@ -134,3 +134,21 @@ def test_queries_near_the_end_of_f32(native_lib, rows):
     got = ops.tree_attention(q, args[0], args[1], torch.tensor([60], device="cuda"), mask, args[2], args[3], scale=scale)[0]
     want, bound = attended_by_row(q[0], k[0], v[0], 60, mask, scale)
     assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("cache", ["bf16", "f16", "q8", "e4m3"])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [3, 8, 20])
+def test_infinite_queries_whose_scores_are_all_minus_infinity(native_lib, cache, kind, rows):
+    """No weights come of them: such a row is not a number, wherever it sees a key, and zeros where it sees none."""
+    args, k, v = make_cache(cache, 47, 1, 1, 1 + rows, 64)
+    q = normal(9, 1, rows, 2, 64).to(TYPES[kind])
+    first = int((k[0, 0, 0] < 0).nonzero()[0])               # a dimension in which the only key is below zero
+    q[0, 1, :, first] = math.inf
+    mask = torch.zeros(rows, rows, dtype=torch.bool, device="cuda")
+    want, bound = attended_by_row(q[0].nan_to_num(posinf=0.0), k[0], v[0], 1, mask, 0.125)
+    got = ops.tree_attention(q, args[0], args[1], torch.tensor([1], device="cuda"), mask, args[2], args[3])[0]
+    rest = torch.arange(rows, device="cuda") != 1
+    assert bool(got[1].isnan().all()) and bool(((got.double() - want).abs() <= bound)[rest].all())
+    got = ops.tree_attention(q, args[0], args[1], torch.tensor([0], device="cuda"), mask, args[2], args[3])
+    assert bool((got == 0).all())
