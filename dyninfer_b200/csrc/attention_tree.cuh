@@ -506,6 +506,40 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
             for (int e = 0; e < NE; e++) sc[j][e] = C::HALF ? acc[j][e] + acc[j][e + 4 - NE] : acc[j][e];
       }
 
+      // An infinite key entry against a term of the query that is zero, or of the other sign, is no score. Such scores are
+      // computed once more, entry by entry (in units that do not matter: what comes of an infinity is none or infinite).
+      if constexpr (C::WIDE) {
+        if (careful) {
+#pragma unroll 1
+          for (int key = 0; key < KT; key++) {
+#pragma unroll
+            for (int h = 0; h < H; h++) {
+              const int r = g + 8 * h < total_rows ? g + 8 * h : 0, tr = r / a.group, gh = r - tr * a.group;
+              bool lost = false;
+#pragma unroll
+              for (int j = 0; j < NK; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                  if (j * 8 + 2 * t + e == key) lost = !(fabsf(sc[j][2 * h + e]) <= INFINITY);
+              if (!lost) continue;
+              const TQ* const of = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
+              float s = 0.f;
+#pragma unroll 1
+              for (int dim = 0; dim < a.d; dim++) {
+                unsigned short bits;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(kt + k_chunk<C>(key, dim / 8) + (uint32_t)(dim % 8 * 2)));
+                s = fmaf(kv_float(of[dim]), C::BF ? __bfloat162float(__ushort_as_bfloat16(bits)) : __half2float(__ushort_as_half(bits)), s);
+              }
+#pragma unroll
+              for (int j = 0; j < NK; j++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                  if (j * 8 + 2 * t + e == key) sc[j][2 * h + e] = s;
+            }
+          }
+        }
+      }
+
       // scores in powers of two, masked
       const int64_t key0 = (int64_t)tile * KT;
       float vscale[C::WIDE ? 1 : NK][2];

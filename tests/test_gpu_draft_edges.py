@@ -152,3 +152,24 @@ def test_infinite_queries_whose_scores_are_all_minus_infinity(native_lib, cache,
     assert bool(got[1].isnan().all()) and bool(((got.double() - want).abs() <= bound)[rest].all())
     got = ops.tree_attention(q, args[0], args[1], torch.tensor([0], device="cuda"), mask, args[2], args[3])
     assert bool((got == 0).all())
+
+
+@pytest.mark.parametrize("cache", ["bf16", "f16"])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows", [3, 8, 20])
+def test_infinite_keys_that_are_seen(native_lib, cache, kind, rows):
+    """A score of minus infinity is a weight of zero; one of plus infinity, or an infinity against a zero, spoils the row."""
+    args, k, v = make_cache(cache, 46, 1, 1, 90 + rows, 64)
+    q = normal(9, 1, rows, 2, 64).to(TYPES[kind])
+    q[0, :, :, 5] = q[0, :, :, 5].abs() + 0.1
+    q[0, 0, 0, 9], q[0, 1, 1, 9] = 0.0, -1.0
+    q[0, 2:, :, 9] = 1.0
+    q[0, 0, 1, 9] = q[0, 1, 0, 9] = 1.0
+    args[0][0, 0, 7, 5] = args[0][0, 0, 70, 9] = args[0][0, 0, 90, 5] = -math.inf
+    mask = torch.eye(rows, dtype=torch.bool, device="cuda")
+    mask[:, 0] = True
+    got = ops.tree_attention(q, args[0], args[1], torch.tensor([90], device="cuda"), mask, scale=0.125)[0]
+    spoilt = torch.zeros(rows, 2, dtype=torch.bool, device="cuda")
+    spoilt[0, 0] = spoilt[1, 1] = True                       # 0 times, and -1 times, minus infinity
+    want, bound = attended_by_row(q[0], args[0][0].double(), v[0], 90, mask, 0.125)
+    assert bool(got[spoilt].isnan().all()) and bool(((got.double() - want).abs() <= bound)[~spoilt].all())
