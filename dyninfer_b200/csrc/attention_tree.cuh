@@ -14,10 +14,19 @@
 //              bytes are interleaved on the way to f16; the value's scale goes into P. 2-byte values come by ldmatrix.trans.
 // Precision. Operands are f16 (bf16 for bf16 caches); what does not fit goes as two or three terms (an f32 query: 22 or 24
 // bits). A row of Q enters times a power of two that brings its largest element to 2^8 .. 2^9 (f16 has five bits of
-// exponent) or, for whole-number products, as 24-bit numbers; P relative to the largest value scale so far. An mma truncates where
-// it adds to its accumulator, always toward zero, so a tile's P V starts from zero and joins the running output by rounded adds.
-// This header: up to sixteen rows. 8 x 1 rows of 64 heads at 32768 over q8 98 us, 76 % of the copy bandwidth; what bounds it is the
-// latency of instructions at eight warps per SM (219 registers). 1 x 5 rows of 16 heads at 600, bf16: 10.3 us.
+// exponent) or, for whole-number products, as 24-bit numbers. An mma truncates where it adds to its accumulator, always toward zero,
+// so a tile's P V starts from zero and joins the running output by rounded adds.
+// P has two terms (22 bits; over bf16 caches 16, and three terms for f32 queries), but one of 11 bits for bf16 queries over f16 and
+// 8-bit caches: a weight is off by 2^-11 of itself at most and by about 2e-4 in the mean, independently of the others, which moves a
+// result by about as much of its size; its own rounding to bf16 moves it by 1.7e-3. (4 x 64 rows at 8192 over e4m3: error against 64
+// bits 1.67e-3, with a plain f32 computation 1.66e-3. With two terms 85.7 us instead of 67.6, 8 x 2 rows at 8192 68.3 instead of 49.4.)
+// Over 8-bit caches P takes the values' scales, relative to the largest of those that its row has seen so far: f16 ends at 2^-24, so
+// what is below 2^-38 (f32 queries) or 2^-30 (others) of the largest value that a row sees is lost, however small that value's own
+// weight is.
+// This header: up to sixteen rows. 8 x 1 rows of 64 heads at 32768 over q8 98 us, 465 MB at 73 % of the copy bandwidth; what bounds it
+// is the latency of instructions at eight warps per SM (217 registers). 1 x 5 rows of 16 heads at 600, bf16: 10.4 us. The forms for
+// nine to sixteen rows over e4m3 keep registers in local memory (232 to 328 bytes are loaded back): 8 x 2 rows of 64 heads at 8192,
+// f16, 68.5 us, over q8 52.3.
 #pragma once
 
 #include <algorithm>
@@ -575,7 +584,7 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
             }
             vis[h] = bits;
             if (!C::WIDE) {
-              // any other scale would push the row's weights out of f16's range
+              // a scale that the row does not see would push its weights out of f16's range
               float most = 0.f;
 #pragma unroll
               for (int i = 0; i < 2 * NK; i++) most = fmaxf(most, bits >> i & 1 ? vscale[C::WIDE ? 0 : i >> 1][i & 1] : 0.f);

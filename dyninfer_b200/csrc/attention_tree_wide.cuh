@@ -12,7 +12,7 @@
 // Scores, references, slack, terms and units are those of attention_tree.cuh. Where a result is not finite (weight 0 times
 // an infinity in a key that a row does not see), such rows are computed once more one by one, without tensor cores.
 // All waits are bounded; one that runs out leaves a code in the device's error word.
-// 4 x 64 rows of 32 heads at 8192 over e4m3, bf16: 70 us, 26 % of the measured bf16 rate; 8 x 13 at 2048 over q8, f32 (two terms of Q and P): 39.5.
+// 4 x 64 rows of 32 heads at 8192 over e4m3, bf16: 68 us, 27 % of the measured bf16 rate; 8 x 13 at 2048 over q8, f32 (two terms of Q and P): 40.
 // A stream's tile takes 3800 (bf16) to 5000 cycles (f32): maximum 750, weights 1500, the wait for U 700 to 1000 and its fold 330 with
 // f32; issue and latency bound it, the tensor pipe is a quarter busy.
 #pragma once
@@ -46,7 +46,7 @@ struct Wide {
   // which 2^-9 does not see before some ten thousand tiles; rows whose reference moves are rescaled there. With f16 operands (one
   // term of P) there is room for P beside S, and the next tile's S is made under the present one's exponentials.
   static constexpr bool STAYS = QB, BESIDE = STAYS && PT == 1;
-  // tiles with keys that not every row sees in a loop of their own: 4 x 64 rows at 8192 over e4m3 68.9 us, in one loop 72.0. Results that are
+  // tiles with keys that not every row sees in a loop of their own: 4 x 64 rows at 8192 over e4m3 67.7 us, in one loop 72.0. Results that are
   // folded have more code, of which two copies cost short contexts more (2 x 8 at 500 over q8, f32: 20.4, in one loop 19.2)
   static constexpr bool APART = STAYS && !WIDE;
   // tensor memory columns

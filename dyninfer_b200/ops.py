@@ -219,7 +219,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     dimension): pair i of the first 2 * len(frequencies) dimensions turns by positions[...] * frequencies[i] and is multiplied by
     `magnitude`; the other dimensions are copied. `layout` is "half" (pairs i, i + r/2) or "interleaved" (2i, 2i + 1).
     `frequencies` is a float64 tensor in host memory (`rotary_frequencies` makes one); angles are taken modulo a turn in 64-bit
-    fixed point, off by at most 2^-65 * position * (1 + frequency) turns. `out` may be x itself: a view of the leading heads of fused [q | k | v] rows turns q and k where they lie."""
+    fixed point, off by at most 2^-65 * position * (1 + frequency) turns. `out` may be x itself (a view of the leading heads of
+    fused [q | k | v] rows turns q and k where they lie) but must not overlap it otherwise."""
     kind, shape, sx = _WT.get(x.dtype), x.shape, x.stride()
     if kind is None:
         raise TypeError(f"x must be float32, float16 or bfloat16, not {x.dtype}")
@@ -393,7 +394,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     bf16, or 8-bit codes with their scales. Row r of a slot sees keys 0 .. lengths[slot] - 1, and of the rows' own keys, which
     stand at lengths[slot] + j, those with mask[slot, r, j] (bool, [rows, rows] for all slots or [slots, rows, rows]); without a
     mask, those with j <= r: a chain, or the plain decode step. A row that sees nothing, or whose length is below zero, gets
-    zeros. `scale` is 1 / sqrt(d) unless given. Returns [slots, rows, heads, d] of q's type."""
+    zeros. `scale` is 1 / sqrt(d) unless given. Returns [slots, rows, heads, d] of q's type. Sums are held in 32 bits; softmax
+    weights of bf16 queries over f16 and 8-bit caches enter their products with 11 bits (others 16 to 24), and over 8-bit caches
+    what is below 2^-38 (f32 queries) or 2^-30 (others) of the largest value that a row sees is lost."""
     kind, cache = _WT.get(q.dtype), _KV.get(k_cache.dtype)
     if kind is None:
         raise TypeError(f"q must be float32, float16 or bfloat16, not {q.dtype}")
@@ -445,7 +448,8 @@ def verify_draft(tokens: torch.Tensor, parents: torch.Tensor, target: torch.Tens
     distinct tokens chosen without chance. uniforms [slots, nodes] are f32 in [0, 1): node i is tried with its own, and node 0's
     draws the last token. From node 0 on the children of the node reached are tried in order; a refusal takes the draft's
     probabilities (without a draft, the child's entry) from what the next child or the last token is drawn from. The
-    target's distribution is kept. next is -1 where a row has no finite positive sum."""
+    target's distribution is kept where rows of target and draft sum to one; they are taken as they are, so rows rounded to 16
+    bits keep it to about that rounding. next is -1 where a row has no finite positive sum."""
     if target.dim() != 3:
         raise ValueError(f"target must be [slots, nodes, vocab], not {tuple(target.shape)}")
     kind = _WT.get(target.dtype)

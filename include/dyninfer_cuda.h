@@ -200,7 +200,10 @@ int dyninfer_cuda_kv_read(void* k_dev, void* v_dev, int type, const int64_t* x_s
  * where j <= r. Keys from kv_cap on do not exist; a row that sees nothing gets zeros, and so do all
  * rows of an entry whose length is below zero (one whose scores are all minus infinity: NaN). ctx [batch, rows, heads, d] is dense, of q's type.
  * kv_type F16, BF16, or an 8-bit type with its scales (as kv_write lays them out). scale is above
- * zero. d is a multiple of 16 up to 128. */
+ * zero. d is a multiple of 16 up to 128. Maxima, sums and outputs are held in 32 bits; softmax weights
+ * of bf16 queries over f16 and 8-bit caches enter their products with 11 bits (others 16 to 24). Over
+ * 8-bit caches what is below 2^-38 (f32 queries) or 2^-30 (others) of the largest value that a row
+ * sees is lost. */
 int dyninfer_cuda_tree_attention(const void* q_dev, int q_type, const int64_t* q_strides, const void* k_cache_dev,
                                  const void* v_cache_dev, int kv_type, const int64_t* cache_strides,
                                  const float* k_scale_dev, const float* v_scale_dev, const int64_t* scale_strides,
@@ -217,7 +220,9 @@ int dyninfer_cuda_tree_attention(const void* q_dev, int q_type, const int64_t* q
  * and Z = 1 at first and a refusal leaves r = max(r / Z - q, 0) (without a draft: q = 1 in the test,
  * and r loses c's entry) and Z = its sum. The token behind is the first v at which the running sum
  * of r passes uniforms[b, 0] times its total; where nothing is left, of the target's row; -1 where
- * that has no finite positive sum. Tokens outside the vocabulary are refused. accepted [batch] = the
+ * that has no finite positive sum. Rows are taken as they are: the target's distribution is kept where
+ * target's rows (and draft's) sum to one, which rows rounded to 16 bits do only about (Z = 1 at first
+ * whatever p's sum is). Tokens outside the vocabulary are refused. accepted [batch] = the
  * number of tokens taken, path [batch, nodes] = the nodes from node 0 on, then -1, next [batch] =
  * the token. Sums are in 64 bits. Up to 1024 nodes. */
 int dyninfer_cuda_verify_draft(const int64_t* tokens_dev, const int64_t* parents_dev, int64_t parents_stride,
