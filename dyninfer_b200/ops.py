@@ -365,7 +365,7 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, k_cache: to
 def kv_read(starts: torch.Tensor, rows: int, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
             v_scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows starts[slot] .. starts[slot] + rows - 1 of an 8-bit cache as values (k, v), each [slots, rows, kv_heads, d] of
-    `dtype`: what `kv_write` takes. Zeros for rows outside the cache."""
+    `dtype`: what `kv_write` takes. Zeros for rows outside the cache; infinity where a code's rounding passes dtype's largest."""
     kind = _WT.get(dtype)
     if kind is None:
         raise TypeError(f"dtype must be float32, float16 or bfloat16, not {dtype}")

@@ -187,7 +187,8 @@ int dyninfer_cuda_kv_write(const void* k_dev, const void* v_dev, int type, const
                            const int64_t* starts_dev, const int64_t* counts_dev, int64_t batch, int64_t rows,
                            int64_t kv_heads, int64_t d, int64_t kv_cap, void* stream);
 
-/* The reverse: rows starts[b] + r as values of `type`; zeros for rows outside the cache. */
+/* The reverse: rows starts[b] + r as values of `type`; zeros for rows outside the cache. A value whose
+ * rounding to its code takes it past the largest of `type` reads back as infinity. */
 int dyninfer_cuda_kv_read(void* k_dev, void* v_dev, int type, const int64_t* x_strides, const void* k_cache_dev,
                           const void* v_cache_dev, int kv_type, const int64_t* cache_strides,
                           const float* k_scale_dev, const float* v_scale_dev, const int64_t* scale_strides,
