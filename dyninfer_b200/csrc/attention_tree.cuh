@@ -238,16 +238,6 @@ __device__ __forceinline__ bool sees(const TreeArgs& a, int64_t b, int row, int6
   return a.mask ? a.mask[b * a.ms[0] + row * a.ms[1] + j] != 0 : j <= row;
 }
 
-// What a row's output is multiplied with, from the sum of its weights. Without weights it is zero where the row sees no key, and not a
-// number where all its scores are minus infinity.
-__device__ __forceinline__ float over_sum(const TreeArgs& a, int64_t b, int row, int64_t len, int64_t keys, float sum) {
-  if (sum != 0.f) return 1.f / sum;
-  bool some = len > 0;
-#pragma unroll 1
-  for (int64_t j = 0; j < keys && !some; j++) some = sees(a, b, row, j);  // (there are no keys in front of the tree)
-  return some ? __uint_as_float(0x7fc00000u) : 0.f;
-}
-
 // Bit e: whether a row sees key key0 + e, of N <= 32. Sixteen bytes of the mask are asked for at once.
 template <int N>
 __device__ __forceinline__ uint32_t seen_of(const TreeArgs& a, int64_t b, int row, int64_t key0, int64_t keys, int64_t len) {
@@ -276,12 +266,28 @@ __device__ __forceinline__ uint32_t seen_of(const TreeArgs& a, int64_t b, int ro
   return bits;
 }
 
+// What a row's output is multiplied with, from the sum of its weights. Without weights it is zero where the row sees no key, and not a
+// number where all its scores are minus infinity. LANES neighbours hold the same row and look for a key together.
+template <int LANES>
+__device__ __forceinline__ float over_sum(const TreeArgs& a, int64_t b, int row, int64_t len, int64_t keys, float sum) {
+  if (sum != 0.f) return 1.f / sum;
+  bool some = len > 0;
+  if (!some) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int64_t key = lane % LANES; key < keys; key += LANES) some = some || sees(a, b, row, key - len);
+    some = __any_sync(LANES == 32 ? 0xffffffffu : ((1u << LANES % 32) - 1) << (lane & ~(LANES - 1)), some);
+  }
+  return some ? __uint_as_float(0x7fc00000u) : 0.f;
+}
+
 template <int CT, typename TQ, int D, bool HALF>
 __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, HALF>::BLOCKS) tree_attention_kernel(const __grid_constant__ TreeArgs a) {
   using C = Cfg<CT, TQ, D, HALF>;
   using O = Op<C::BF>;
   constexpr int KT = C::KT, NT = D / 8, KS = D / 16, NK = KT / 8, WK = C::WK, H = C::H, NE = 2 * H;  // NE: a thread's entries of an n8 tile
   extern __shared__ __align__(128) uint8_t tree_shared[];
+  __shared__ bool odd_query[C::RB];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
   const int split = (int)blockIdx.x % a.splits;
   const int64_t pair = blockIdx.x / a.splits;
@@ -518,33 +524,35 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
       // An infinite key entry against a term of the query that is zero, or of the other sign, is no score. Such scores are
       // computed once more, entry by entry (in units that do not matter: what comes of an infinity is none or infinite).
       if constexpr (C::WIDE) {
+        bool lost = false;
         if (careful) {
-#pragma unroll 1
-          for (int key = 0; key < KT; key++) {
 #pragma unroll
-            for (int h = 0; h < H; h++) {
-              const int r = g + 8 * h < total_rows ? g + 8 * h : 0, tr = r / a.group, gh = r - tr * a.group;
-              bool lost = false;
+          for (int h = 0; h < H; h++)
+            if (g + 8 * h < total_rows && !odd_query[g + 8 * h]) {
 #pragma unroll
-              for (int j = 0; j < NK; j++)
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-                  if (j * 8 + 2 * t + e == key) lost = !(fabsf(sc[j][2 * h + e]) <= INFINITY);
-              if (!lost) continue;
-              const TQ* const of = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
-              float s = 0.f;
-#pragma unroll 1
-              for (int dim = 0; dim < a.d; dim++) {
-                unsigned short bits;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(kt + k_chunk<C>(key, dim / 8) + (uint32_t)(dim % 8 * 2)));
-                s = fmaf(kv_float(of[dim]), C::BF ? __bfloat162float(__ushort_as_bfloat16(bits)) : __half2float(__ushort_as_half(bits)), s);
-              }
-#pragma unroll
-              for (int j = 0; j < NK; j++)
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-                  if (j * 8 + 2 * t + e == key) sc[j][2 * h + e] = s;
+              for (int j = 0; j < NK; j++) lost = lost || !(fabsf(sc[j][2 * h]) <= INFINITY && fabsf(sc[j][2 * h + 1]) <= INFINITY);
             }
+        }
+        if (lost) {
+#pragma unroll
+          for (int h = 0; h < H; h++) {
+            const int r = min(g + 8 * h, total_rows - 1), tr = r / a.group, gh = r - tr * a.group;
+            if (odd_query[r]) continue;
+            const TQ* const of = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
+#pragma unroll
+            for (int j = 0; j < NK; j++)
+#pragma unroll
+              for (int e = 0; e < 2; e++)
+                if (!(fabsf(sc[j][2 * h + e]) <= INFINITY)) {
+                  float s = 0.f;
+#pragma unroll 1
+                  for (int dim = 0; dim < a.d && s == s; dim++) {
+                    unsigned short bits;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(bits) : "r"(kt + k_chunk<C>(j * 8 + 2 * t + e, dim / 8) + (uint32_t)(dim % 8 * 2)));
+                    s = fmaf(kv_float(of[dim]), C::BF ? __bfloat162float(__ushort_as_bfloat16(bits)) : __half2float(__ushort_as_half(bits)), s);
+                  }
+                  sc[j][2 * h + e] = s;
+                }
           }
         }
       }
@@ -781,6 +789,17 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
 #pragma unroll
         for (int e = 0; e < NE; e++) finite = finite && fabsf(out[n][e]) < INFINITY;
     if (!__syncthreads_or(!finite)) break;
+    if (C::WIDE) {  // rows whose query is not finite are what they are
+      for (int r = warp; r < total_rows; r += WK) {
+        const int tr = r / a.group, gh = r - tr * a.group;
+        const TQ* const of = static_cast<const TQ*>(a.q) + b * a.qs[0] + tr * a.qs[1] + (int64_t)(kvh * a.group + gh) * a.qs[2];
+        bool odd = false;
+        for (int dim = lane; dim < a.d; dim += 32) odd = odd || !(fabsf(kv_float(of[dim])) < INFINITY);
+        odd = __any_sync(0xffffffffu, odd);
+        if (lane == 0) odd_query[r] = odd;
+      }
+      __syncthreads();
+    }
     begin();
   }
   // out in its own units again
@@ -873,7 +892,7 @@ __global__ void __launch_bounds__(Cfg<CT, TQ, D, HALF>::THREADS, Cfg<CT, TQ, D, 
     }
     const int tr = r / a.group, gh = r - tr * a.group;
     TQ* to = static_cast<TQ*>(a.out) + ((b * a.rows + tr) * a.heads + (int64_t)kvh * a.group + gh) * a.d + c;
-    const float inv = over_sum(a, b, tr, len, keys, l);
+    const float inv = over_sum<D / 4>(a, b, tr, len, keys, l);
     if (c < a.d) {
 #pragma unroll
       for (int e = 0; e < 4; e++) kv_store(o[e] * inv, to + e);

@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(Wide<CT, TQ, D>::THREADS, 1) tree_attention_wi
     }
     const int t2 = (row0 + r) / a.group, g2 = row0 + r - t2 * a.group;
     TQ* to = static_cast<TQ*>(a.out) + ((b * a.rows + t2) * a.heads + (int64_t)kvh * a.group + g2) * a.d + c;
-    const float over = over_sum(a, b, t2, len, keys, l);
+    const float over = over_sum<D / 4>(a, b, t2, len, keys, l);
     if (c < a.d) {
 #pragma unroll
       for (int e = 0; e < 4; e++) kv_store(o[e] * over, to + e);
