@@ -25,7 +25,7 @@
 // weight is.
 // This header: up to sixteen rows. 8 x 1 rows of 64 heads at 32768 over q8 98 us, 465 MB at 73 % of the copy bandwidth; what bounds it
 // is the latency of instructions at eight warps per SM (217 registers). 1 x 5 rows of 16 heads at 600, bf16: 10.4 us. The forms for
-// nine to sixteen rows over e4m3 keep registers in local memory (232 to 328 bytes are loaded back): 8 x 2 rows of 64 heads at 8192,
+// nine to sixteen rows over e4m3 keep registers in local memory (156 to 356 bytes are loaded back): 8 x 2 rows of 64 heads at 8192,
 // f16, 68.5 us, over q8 52.3.
 #pragma once
 
